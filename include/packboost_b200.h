@@ -388,6 +388,89 @@ typedef struct pb_round_log_header {
 } pb_round_log_header;
 /* The log is a pb_round_log_header followed by (1 << max_depth) - 1 pb_winner records. */
 
+/* ---- objectives: losses on the scores of rows, with their gradients --------------------------
+ * The reference learns from one loss, half the squared difference to a target
+ * (packboost/booster.py:2149-2154), and has nothing to cite here.
+ *
+ *  PB_OBJECTIVE_PREFERENCE  pairs of rows, the first preferred to the second: with
+ *      d = (s_c - r_c) - (s_j - r_j), r the scores of a reference, and z = beta d,
+ *      w (softplus(-z) + smoothing z), or w (d - 1 / (2 beta))^2 with `squared`.
+ *  PB_OBJECTIVE_CHOICE      groups of rows with log-probabilities l = s - log sum exp s over the
+ *      group: - target l.
+ *  PB_OBJECTIVE_POLICY      groups as above, rows with an advantage A != 0 were taken by a policy of
+ *      log-probabilities `old`: with q = exp(l - old), -min(q A, clamp(q, 1 - clip_low,
+ *      1 + clip_high) A), and kl_coef times the sum over the group of exp(l) (l - reference).
+ *
+ * The sum over pairs or groups is multiplied by `scale`.  A row with the score -inf is masked: in
+ * groups its probability is 0 and, in a policy, nothing else of it is looked at. */
+#define PB_OBJECTIVE_PREFERENCE 0
+#define PB_OBJECTIVE_CHOICE 1
+#define PB_OBJECTIVE_POLICY 2
+
+#define PB_SCORE_F32 0
+#define PB_SCORE_F16 1
+#define PB_SCORE_BF16 2
+
+/* Pairs by row: a pair is one item of each of its two rows.  Items of a row are neighbours. */
+typedef struct pb_pairs {
+    int64_t n_rows;
+    int64_t n_items;             /* two per pair */
+    const int32_t* item_offsets; /* [n_rows + 1] */
+    const uint32_t* other;       /* [n_items] the other row; bit 31: the item's own row is the rejected one */
+    const float* offset;         /* [n_items] reference score of the own row minus the other's, or NULL */
+    const float* weight;         /* [n_items], or NULL: 1 */
+} pb_pairs;
+
+/* Groups of rows: those that have any, `rows` lists their rows (NULL: the rows in order). */
+typedef struct pb_groups {
+    int64_t n_rows;
+    int64_t n_groups;
+    const int32_t* offsets;      /* [n_groups + 1] */
+    const int32_t* rows;         /* [n_rows], or NULL */
+} pb_groups;
+
+typedef struct pb_objective {
+    int64_t kind;
+    const pb_pairs* pairs;       /* host pointers; the one that the kind needs */
+    const pb_groups* groups;
+    double beta;
+    double smoothing;
+    int64_t squared;
+    const float* target;         /* [n_rows] each, on the device */
+    const float* advantage;
+    const float* old;
+    const float* reference;      /* may be NULL: no divergence */
+    double clip_low;
+    double clip_high;
+    double kl_coef;
+    double scale;
+} pb_objective;
+
+/* sizeof of the three, so that a binding can verify its mirrors: 0 pairs, 1 groups, 2 objective. */
+int64_t pb_objective_struct_bytes(int64_t which);
+
+/* Scratch of one evaluation. */
+int64_t pb_objective_workspace_bytes(const pb_objective* o);
+
+/* Gradient with respect to the scores [n_rows] (of the scores' type), the loss and, for a policy, the
+ * scaled divergence and the number of rows whose ratio is beyond its border.  `loss`, `kl` and
+ * `clipped` are on the device and may be NULL. */
+int pb_objective_evaluate(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss,
+                          float* kl, int64_t* clipped, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Log-probabilities of the rows in their groups (of the scores' type; -inf where the score is). */
+int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* stream);
+
+/* pb_round_begin with the gradient of an objective in the place of g = preds - y (`y` is not read);
+ * the rows of the objective are the state's. */
+int pb_round_begin_objective(const pb_train_state* st, const pb_objective* o, int64_t apply_previous, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* pb_loop_submit with such a round; objective and workspace stay the same for all rounds of a loop. */
+int pb_loop_submit_objective(void* loop, const pb_train_state* st, const pb_objective* o, void* workspace,
+                             int64_t workspace_bytes, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
+                             int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream);
+
 /* ---- kernel-level entry points (used directly by the parity tests and the benchmark) ---- */
 
 /* Histogram pass alone (packboost/booster.py:933-977, counts and gradient sums; the

@@ -74,6 +74,28 @@ class Model(C.Structure):
     ]
 
 
+class Pairs(C.Structure):
+    """Mirror of ``pb_pairs``."""
+
+    _fields_ = [("n_rows", i64), ("n_items", i64), ("item_offsets", vp), ("other", vp), ("offset", vp), ("weight", vp)]
+
+
+class Groups(C.Structure):
+    """Mirror of ``pb_groups``."""
+
+    _fields_ = [("n_rows", i64), ("n_groups", i64), ("offsets", vp), ("rows", vp)]
+
+
+class Objective(C.Structure):
+    """Mirror of ``pb_objective``."""
+
+    _fields_ = [
+        ("kind", i64), ("pairs", C.POINTER(Pairs)), ("groups", C.POINTER(Groups)), ("beta", C.c_double),
+        ("smoothing", C.c_double), ("squared", i64), ("target", vp), ("advantage", vp), ("old", vp), ("reference", vp),
+        ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double), ("scale", C.c_double),
+    ]
+
+
 _PROTOS: dict[str, tuple[Any, list[Any]]] = {
     "pb_last_error": (C.c_char_p, []),
     "pb_abi_version": (C.c_int, []),
@@ -124,6 +146,12 @@ _PROTOS: dict[str, tuple[Any, list[Any]]] = {
     "pb_loop_wait": (C.c_int, [vp, i64]),
     "pb_loop_counts": (C.c_int, [vp, vp, vp]),
     "pb_tree_from_log": (C.c_int, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp]),
+    "pb_objective_struct_bytes": (i64, [i64]),
+    "pb_objective_workspace_bytes": (i64, [C.POINTER(Objective)]),
+    "pb_objective_evaluate": (C.c_int, [C.POINTER(Objective), vp, i64, vp, vp, vp, vp, vp, i64, vp]),
+    "pb_group_log_probs": (C.c_int, [C.POINTER(Groups), vp, i64, vp, vp]),
+    "pb_round_begin_objective": (C.c_int, [C.POINTER(TrainState), C.POINTER(Objective), i64, vp, i64, vp]),
+    "pb_loop_submit_objective": (C.c_int, [vp, vp, C.POINTER(Objective), vp, i64, i64, vp, vp, i64, vp, i64, i64, vp]),
     "pb_hist_build": (C.c_int, [C.POINTER(TrainState), vp, i64, i64, i64, vp, vp, vp]),
     "pb_score_node_general": (C.c_int, [vp, vp, vp, i64, i64, i64, vp, i64, C.c_float, C.c_float, C.c_float, C.c_float,
                                         C.c_float, C.c_float, i64, i64, i64, i64, vp, vp]),
@@ -159,7 +187,8 @@ def lib() -> C.CDLL:
         fn = getattr(handle, name)
         fn.restype = res
         fn.argtypes = args
-    if handle.pb_abi_version() != 1 or handle.pb_train_state_bytes() != C.sizeof(TrainState):
+    if handle.pb_abi_version() != 1 or handle.pb_train_state_bytes() != C.sizeof(TrainState) or any(
+            handle.pb_objective_struct_bytes(i) != C.sizeof(t) for i, t in enumerate((Pairs, Groups, Objective))):
         raise RuntimeError("libpackboost_b200.so ABI mismatch; rebuild it with `python -m packboost_b200.build`")
     _LIB = handle
     return handle

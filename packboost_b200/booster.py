@@ -260,6 +260,8 @@ _RING = 4  # staging slots: at most three rounds are in flight (previous, a disc
 class _DeviceTrainer:
     """Owns the device buffers of one fit and launches the round phases."""
 
+    objective = None   # what the rounds learn from in the place of the squared difference to y (objectives.py)
+
     def __init__(self, cfg: PackBoostConfig, matrix: PackedMatrix, y_sorted: np.ndarray | torch.Tensor, era_offsets: np.ndarray,
                  n_features_total: int, feat_local: np.ndarray, rank: int, world: int,
                  workspace_bytes: int | None = None, replicated: bool = False):
@@ -516,8 +518,12 @@ class _DeviceTrainer:
             lists = self.feat_np[slot]
             lists[:, 0, :] = subsets
             lists[:, 1, :] = lists[:, 0, :]                  # one GPU holds the features in order
-            B.check(lib.pb_loop_submit(self.loop, st, slot, lists.ctypes.data, self.feat_dev.data_ptr(), k,
-                                       self.log_host[slot].data_ptr(), apply_previous, 1 if self.use_graph else 0, stream))
+            rest = (slot, lists.ctypes.data, self.feat_dev.data_ptr(), k, self.log_host[slot].data_ptr(), apply_previous,
+                    1 if self.use_graph else 0, stream)
+            if self.objective is None:
+                B.check(lib.pb_loop_submit(self.loop, st, *rest))
+            else:
+                B.check(lib.pb_loop_submit_objective(self.loop, st, *self._objective_args(), *rest))
             self.pending_delta = True
             self.enqueued += 1
             if not redo:
@@ -619,11 +625,19 @@ class _DeviceTrainer:
             self.rounds_done += 1
         return self.enqueued - 1
 
+    def _objective_args(self) -> tuple:
+        o = self.objective
+        return C.byref(o.struct), o.workspace.data_ptr(), o.workspace.numel()
+
     def _enqueue_phases(self, k: int, n_local: list[int], apply_previous: int) -> None:
         lib, st = self.lib, C.byref(self.st)
         stream = torch.cuda.current_stream().cuda_stream
         D = self.D
-        B.check(lib.pb_round_begin(st, apply_previous, stream))
+        if self.objective is None:
+            B.check(lib.pb_round_begin(st, apply_previous, stream))
+        else:
+            struct, scratch, nbytes = self._objective_args()
+            B.check(lib.pb_round_begin_objective(st, struct, apply_previous, scratch, nbytes, stream))
         for d in range(D):
             sampled = self.feat_dev[d, 0].data_ptr()
             rows = self.feat_dev[d, 1].data_ptr()
@@ -780,9 +794,15 @@ class PackBoost:
         feature_names: Sequence[str] | None = None,
         eval_sets: Sequence[tuple[str, np.ndarray, np.ndarray, Iterable[int] | None]] | None = None,
         round_callback: Callable[[int, dict[str, float]], None] | None = None,
+        objective=None,
     ) -> "PackBoost":
-        """Squared-loss boosting with pack-synchronous growth and DES (``packboost/booster.py:375-656``)."""
-        self._start(X, y, era, feature_names=feature_names, eval_sets=eval_sets)
+        """Squared-loss boosting with pack-synchronous growth and DES (``packboost/booster.py:375-656``).
+
+        ``objective`` (a ``PreferenceObjective``, ``ChoiceObjective`` or ``PolicyObjective`` of
+        :mod:`packboost_b200.objectives`, on the rows of ``X``) takes the place of the squared loss; ``y``
+        then only serves the correlations of ``round_metrics``, which have a ``train_loss`` beside them, and
+        may be ``None``."""
+        self._start(X, y, era, feature_names=feature_names, eval_sets=eval_sets, objective=objective)
         for round_idx in range(num_rounds):
             metrics = self._boost_one_round(round_idx, num_rounds, round_callback is not None)
             if round_callback is not None:
@@ -791,12 +811,14 @@ class PackBoost:
         return self
 
     # -- fit, step by step (the benchmark times _boost_one_round) -------------
-    def _start(self, X, y, era, *, feature_names=None, eval_sets=None) -> None:
+    def _start(self, X, y, era, *, feature_names=None, eval_sets=None, objective=None) -> None:
         """Validate, bin, pack and upload the data; allocate the device state."""
         cfg = self.config
         # torch tensors (device-resident, or pinned host memory) are consumed without conversion
         on_device = isinstance(X, torch.Tensor)
         X_np = X.detach() if on_device else np.asarray(X)
+        if y is None and objective is not None:
+            y = np.zeros(X_np.shape[0], dtype=np.float32)
         # (targets that are on the GPU stay there: they are gathered and copied on the device)
         if isinstance(y, torch.Tensor) and y.is_cuda:
             y_np = y.detach().to(device=self._device, dtype=torch.float32)
@@ -817,6 +839,7 @@ class PackBoost:
             if era.shape[0] != N:
                 raise ValueError("era must align with X rows")
         uniq, era_offsets, order = sort_eras(era, N)
+        bound = None if objective is None else objective._bind(N, era_offsets, order, self._device)
         self._era_unique = uniq
         self._feature_names = list(feature_names) if feature_names is not None else [f"f{i}" for i in range(F)]
 
@@ -903,6 +926,7 @@ class PackBoost:
             y_sorted = y_np[torch.from_numpy(order).to(self._device) if isinstance(y_np, torch.Tensor) else order]
         self._trainer = _DeviceTrainer(cfg, matrix, y_sorted, era_offsets, F, feat_local, rank, world,
                                        replicated=replicate)
+        self._trainer.objective = bound
         self._row_order = order
         self._fit_ctx = {"F": F}
 
@@ -964,6 +988,8 @@ class PackBoost:
         if want_metrics:
             trainer.flush_predictions()
             metrics["train_corr"] = trainer.era_correlation()
+            if trainer.objective is not None:
+                metrics["train_loss"] = trainer.objective.loss(trainer.preds)
         else:
             metrics["train_corr"] = float("nan")
         try:
@@ -1461,6 +1487,17 @@ class PackBoost:
         out = self._predict_packed(rows, self._current_forest()).cpu().numpy()
         self._check_top(top, X)
         return out
+
+    def predict_log_probs(self, X: np.ndarray, group) -> np.ndarray:
+        """Log-probabilities of the rows of ``X`` under the softmax of the scores within their groups
+        (``group``: a group id per row), as the choice and policy objectives train them; those of an
+        earlier model are the old or reference log-probabilities of a ``PolicyObjective``."""
+        from .objectives import RowGroups, group_log_probs
+        groups = RowGroups(group, device=self._device)
+        if X.shape[0] != groups.n_rows:
+            raise ValueError("group must align with X rows")
+        scores = torch.from_numpy(self.predict(X)).to(self._device)
+        return group_log_probs(scores, groups).cpu().numpy()
 
     def predict_packwise(self, X: np.ndarray, block_size_trees: int = 8) -> np.ndarray:
         if block_size_trees <= 0:

@@ -139,6 +139,51 @@ __global__ void __launch_bounds__(kRowThreads) quantise_kernel(
     }
 }
 
+// The same two steps for a gradient that an objective left, as float32 bits, in the place of gq.
+__global__ void __launch_bounds__(kRowThreads) gradient_absmax_kernel(const int32_t* __restrict__ gq, int64_t n, CtlHead* head) {
+    float m = 0.f;
+    const int64_t n4 = (n + 3) >> 2;   // (gq is padded beyond n; what lies there is not looked at)
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i << 2;
+        const int4 v = *reinterpret_cast<const int4*>(gq + r);
+        const int q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (r + u < n) m = fmaxf(m, fabsf(__int_as_float(q[u])));
+    }
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    if ((threadIdx.x & 31) == 0) atomicMax(&head->max_abs_bits, __float_as_uint(m));
+}
+
+__global__ void __launch_bounds__(kRowThreads) quantise_gradient_kernel(int32_t* __restrict__ gq, uint16_t* __restrict__ slot,
+                                                                        uint16_t* __restrict__ leaf, int64_t n, int64_t n_pad,
+                                                                        CtlHead* head, int gq_bits) {
+    float inv;
+    const float scale = scale_from_max(__uint_as_float(head->max_abs_bits), gq_bits, &inv);
+    const float most = ldexpf(1.f, gq_bits);   // (only a gradient that is not finite is beyond it)
+    long long acc = 0;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (n_pad >> 2); i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i << 2;
+        const int4 v = *reinterpret_cast<const int4*>(gq + r);
+        int q[4] = {v.x, v.y, v.z, v.w};
+        uint32_t sl[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool in = r + u < n;
+            const float g = __fmul_rn(__int_as_float(q[u]), scale);
+            q[u] = in && g == g ? __float2int_rn(fminf(fmaxf(g, -most), most)) : 0;
+            sl[u] = in ? 0u : kSlotNone;
+            acc += q[u];
+        }
+        *reinterpret_cast<int4*>(gq + r) = make_int4(q[0], q[1], q[2], q[3]);
+        *reinterpret_cast<uint2*>(slot + r) = make_uint2(sl[0] | (sl[1] << 16), sl[2] | (sl[3] << 16));
+        *reinterpret_cast<uint2*>(leaf + r) = make_uint2(0u, 0u);
+    }
+    for (int d = 16; d > 0; d >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFu, acc, d);
+    if ((threadIdx.x & 31) == 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&head->root_gq), (unsigned long long)acc);
+}
+
 __global__ void root_kernel(Ctl c, int64_t n, int min_leaf, double lambda, int gq_bits) {
     if (threadIdx.x != 0 || blockIdx.x != 0) return;
     float inv;
@@ -931,6 +976,30 @@ extern "C" int pb_round_begin(const pb_train_state* st, int64_t apply_previous, 
     prof_end(st->profile, kProfRound, stream);
     count_launch(4);
     PB_LAUNCH_CHECK("round_begin");
+    return PB_OK;
+}
+
+extern "C" int pb_round_begin_objective(const pb_train_state* st, const pb_objective* o, int64_t apply_previous,
+                                        void* workspace, int64_t workspace_bytes, void* stream_) {
+    NvtxRange nvtx("pb.round_begin_objective apply=%lld", (long long)apply_previous);
+    PB_TRY(check_state(st));
+    PB_TRY(objective_check(o, st->n_rows));
+    cudaStream_t stream = (cudaStream_t)stream_;
+    Ctl c = ctl_view(st->ctl);
+    const int g = row_grid(st->n_rows);
+    prof_begin(st->profile, kProfRound, stream);
+    round_reset_kernel<<<1, 32, 0, stream>>>(c);
+    if (apply_previous)
+        apply_delta_kernel<<<g, kRowThreads, 0, stream>>>(st->preds, st->leaf, c.delta, st->n_rows);
+    const int rc = objective_gradient(o, st->preds, PB_SCORE_F32, st->gq, nullptr, nullptr, nullptr, workspace, workspace_bytes, stream);
+    gradient_absmax_kernel<<<g, kRowThreads, 0, stream>>>(st->gq, st->n_rows, c.head);
+    quantise_gradient_kernel<<<g, kRowThreads, 0, stream>>>(st->gq, st->slot, st->leaf, st->n_rows, rows_padded(st->n_rows),
+                                                            c.head, (int)st->gq_bits);
+    root_kernel<<<1, 32, 0, stream>>>(c, st->n_rows, (int)st->min_samples_leaf, st->lambda_l2, (int)st->gq_bits);
+    prof_end(st->profile, kProfRound, stream);
+    count_launch(apply_previous ? 5 : 4);
+    if (rc) return rc;
+    PB_LAUNCH_CHECK("round_begin_objective");
     return PB_OK;
 }
 

@@ -25,9 +25,17 @@ struct RoundLoop {
     }
 };
 
+// What a round learns from: the squared difference to the targets, or an objective with its scratch.
+struct RoundLoss {
+    const pb_objective* objective;
+    void* workspace;
+    int64_t workspace_bytes;
+};
+
 // lists: device [max_depth][3][k]: global ids, local rows, positions of the sampled features
-int enqueue_round(const pb_train_state* st, const int32_t* lists, int64_t k, int64_t apply_previous, void* stream) {
-    int rc = pb_round_begin(st, apply_previous, stream);
+int enqueue_round(const pb_train_state* st, const RoundLoss& loss, const int32_t* lists, int64_t k, int64_t apply_previous, void* stream) {
+    int rc = loss.objective ? pb_round_begin_objective(st, loss.objective, apply_previous, loss.workspace, loss.workspace_bytes, stream)
+                            : pb_round_begin(st, apply_previous, stream);
     for (int64_t d = 0; d < st->max_depth && rc == PB_OK; ++d) {
         const int32_t* l = lists + d * 3 * k;
         rc = pb_depth_hist_score(st, d, l + k, l + 2 * k, k, k, stream);
@@ -37,7 +45,7 @@ int enqueue_round(const pb_train_state* st, const int32_t* lists, int64_t k, int
     return rc == PB_OK ? pb_round_end(st, stream) : rc;
 }
 
-int capture_round(RoundLoop* loop, const pb_train_state* st, const int32_t* lists, int64_t k) {
+int capture_round(RoundLoop* loop, const pb_train_state* st, const RoundLoss& loss, const int32_t* lists, int64_t k) {
     cudaStream_t side = nullptr;
     PB_CUDA_TRY(cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking));
     const int64_t before = pb_launch_count();
@@ -45,7 +53,7 @@ int capture_round(RoundLoop* loop, const pb_train_state* st, const int32_t* list
     cudaError_t e = cudaStreamBeginCapture(side, cudaStreamCaptureModeThreadLocal);
     int rc = PB_OK;
     if (e == cudaSuccess) {
-        rc = enqueue_round(st, lists, k, 1, side);
+        rc = enqueue_round(st, loss, lists, k, 1, side);
         const cudaError_t end = cudaStreamEndCapture(side, &graph);
         e = rc ? cudaSuccess : end;
     }
@@ -78,8 +86,8 @@ extern "C" void* pb_loop_create(void) {
 
 extern "C" void pb_loop_destroy(void* loop) { delete static_cast<RoundLoop*>(loop); }
 
-extern "C" int pb_loop_submit(void* loop_, const pb_train_state* st, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
-                              int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream_) {
+static int submit_round(void* loop_, const pb_train_state* st, const RoundLoss& loss, int64_t slot, const int32_t* lists_host,
+                        int32_t* lists_dev, int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream_) {
     RoundLoop* loop = static_cast<RoundLoop*>(loop_);
     PB_REQUIRE(loop && st && lists_host && lists_dev && log_host, "null argument");
     PB_REQUIRE(slot >= 0 && slot < kLoopSlots, "slot out of range");
@@ -95,7 +103,7 @@ extern "C" int pb_loop_submit(void* loop_, const pb_train_state* st, int64_t slo
     if (graph && !loop->no_graph && (!loop->exec || loop->graph_k != k)) {
         if (loop->exec) cudaGraphExecDestroy(loop->exec);
         loop->exec = nullptr;
-        if (capture_round(loop, st, lists_dev, k) != PB_OK) {
+        if (capture_round(loop, st, loss, lists_dev, k) != PB_OK) {
             loop->no_graph = true;
             cudaGetLastError();  // (an argument error shows again in the launches below)
         }
@@ -104,12 +112,25 @@ extern "C" int pb_loop_submit(void* loop_, const pb_train_state* st, int64_t slo
         PB_CUDA_TRY(cudaGraphLaunch(loop->exec, stream));
         ++loop->replays;
     } else {
-        rc = enqueue_round(st, lists_dev, k, apply_previous, stream_);
+        rc = enqueue_round(st, loss, lists_dev, k, apply_previous, stream_);
         if (rc) return rc;
     }
     PB_CUDA_TRY(cudaMemcpyAsync(log_host, log_dev, (size_t)log_bytes, cudaMemcpyDeviceToHost, stream));
     PB_CUDA_TRY(cudaEventRecord(loop->logged[slot], stream));
     return PB_OK;
+}
+
+extern "C" int pb_loop_submit(void* loop, const pb_train_state* st, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
+                              int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream) {
+    return submit_round(loop, st, RoundLoss{nullptr, nullptr, 0}, slot, lists_host, lists_dev, k, log_host, apply_previous, use_graph, stream);
+}
+
+extern "C" int pb_loop_submit_objective(void* loop, const pb_train_state* st, const pb_objective* o, void* workspace,
+                                        int64_t workspace_bytes, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
+                                        int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream) {
+    PB_REQUIRE(o != nullptr, "objective is null");
+    return submit_round(loop, st, RoundLoss{o, workspace, workspace_bytes}, slot, lists_host, lists_dev, k, log_host, apply_previous,
+                        use_graph, stream);
 }
 
 extern "C" int pb_loop_wait(void* loop, int64_t slot) {

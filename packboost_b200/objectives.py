@@ -1,0 +1,454 @@
+"""Losses on the scores of rows, each with its gradient, and the objectives that ``PackBoost.fit`` takes.
+
+The booster's own loss is half the squared difference to a target.  The ones here are those a model of scores
+is trained on after or instead of that: which of two rows was preferred, which rows of a group were chosen, and
+what a policy that chooses among the rows of a group earned.  All are differentiated with respect to the
+scores; hessians are 1, as everywhere in the booster, so a leaf's value is the mean of its rows' negative
+gradients (with ``lambda_l2``).
+
+As operators on CUDA tensors::
+
+    pairs = RowPairs(chosen, rejected, n_rows, reference=reference_scores)     # laid out once
+    loss, grad = preference_loss(scores, pairs, beta=0.1)
+    groups = RowGroups(group_of_row)
+    loss, grad = choice_loss(scores, groups, target)
+    loss, grad, kl, clipped = policy_loss(scores, groups, advantage, old_log_probs,
+                                          reference_log_probs=reference, kl_coef=0.05)
+    log_probs = group_log_probs(scores, groups)
+
+and as what a fit learns from::
+
+    booster.fit(X, None, era, num_rounds=100, objective=PreferenceObjective(chosen, rejected, beta=1.0))
+
+Scores are float32, float16 or bfloat16 and gradients have their type; sums are held in 64 bits or, over the few
+pairs of a row, in 32, in an order that does not change from run to run.  The results are not attached to an
+autograd graph: the gradient is there already.  Calls only enqueue work on the current stream of the scores'
+device and may be captured into a CUDA graph; ``RowPairs`` and ``RowGroups`` wait for their own layout, may be
+used from any stream, and have to outlive the graphs that use them.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import backends as B
+
+_SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_MOST = (1 << 31) - 2    # rows, and items (two per pair): 32-bit indices, bit 31 of a row id is a flag
+_PREFERENCE, _CHOICE, _POLICY = 0, 1, 2
+
+
+class LossAndGradient(NamedTuple):
+    loss: torch.Tensor       # float32, no dimensions
+    grad: torch.Tensor       # like the scores
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor       # float32, no dimensions
+    grad: torch.Tensor       # like the scores
+    kl: torch.Tensor         # float32, no dimensions: divergence from the reference, reduced like the loss
+    clipped: torch.Tensor    # int64, no dimensions: taken rows whose ratio is beyond its border
+
+
+# ---- arguments -----------------------------------------------------------------------------------
+
+
+def _indices(values, name: str) -> torch.Tensor:
+    t = values.detach() if isinstance(values, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(np.asarray(values)))
+    if t.numel() == 0 and not isinstance(values, torch.Tensor):
+        t = t.to(torch.int64)   # (an empty list has no integer type)
+    if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool:
+        raise TypeError(f"{name} must hold integers")
+    if t.dim() != 1:
+        raise ValueError(f"{name} must be 1-D")
+    return t.to(torch.int64)
+
+
+def _numbers(values, name: str, length: int, device) -> torch.Tensor:
+    """1-D numbers of a caller, in the type they have."""
+    t = values.detach() if isinstance(values, torch.Tensor) else torch.from_numpy(np.array(values, ndmin=1))
+    if t.dtype.is_complex or t.dtype == torch.bool:
+        raise TypeError(f"{name} must hold real numbers")
+    if t.dim() != 1 or t.shape[0] != length:
+        raise ValueError(f"{name} must be 1-D with {length} entries")
+    return t.to(device)
+
+
+def _count(value, name: str) -> int:
+    if isinstance(value, bool) or not isinstance(value, (int, np.integer)):
+        raise TypeError(f"{name} must be an integer")
+    if not 0 <= value <= _MOST:
+        raise ValueError(f"{name}={value} outside [0, {_MOST}]")
+    return int(value)
+
+
+def _home(*values, device=None) -> torch.device:
+    """Where a layout lives: the given device, that of a CUDA tensor among the values, or the current one."""
+    if device is None:
+        device = next((v.device for v in values if isinstance(v, torch.Tensor) and v.is_cuda), None)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("objectives live on a CUDA device")
+    if not B.cuda_available():
+        raise RuntimeError("packboost_b200: libpackboost_b200.so is not built or no sm_100 device is visible")
+    return torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+
+
+# ---- layouts ---------------------------------------------------------------------------------------
+
+
+def _check_pairs(chosen, rejected, n_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    chosen, rejected = _indices(chosen, "chosen"), _indices(rejected, "rejected")
+    if chosen.shape[0] != rejected.shape[0]:
+        raise ValueError("chosen and rejected differ in length")
+    if 2 * chosen.shape[0] > _MOST:
+        raise ValueError(f"more than {_MOST // 2} pairs")
+    rejected = rejected.to(chosen.device)
+    if chosen.shape[0]:
+        low = min(int(chosen.min()), int(rejected.min()))
+        high = max(int(chosen.max()), int(rejected.max()))
+        if low < 0 or high >= n_rows:
+            raise ValueError(f"pairs name rows outside [0, {n_rows})")
+        if bool((chosen == rejected).any()):
+            raise ValueError("a pair compares a row with itself")
+    return chosen, rejected
+
+
+def _check_weight(weight, n_pairs: int, device) -> torch.Tensor:
+    weight = _numbers(weight, "weight", n_pairs, device).to(torch.float32)
+    if n_pairs and not bool((torch.isfinite(weight) & (weight >= 0)).all()):
+        raise ValueError("weights must be finite and not negative")
+    return weight
+
+
+def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict[str, torch.Tensor | None]:
+    """The items of every row, neighbours in the order in which the pairs were given (chosen side first)."""
+    own, other = torch.cat([chosen, rejected]), torch.cat([rejected, chosen])
+    flag = torch.cat([torch.zeros_like(chosen), torch.full_like(rejected, 1 << 31)])
+    own, order = torch.sort(own, stable=True)
+    counts = torch.bincount(own, minlength=n_rows)[:n_rows]
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
+    offset = None
+    if reference is not None:
+        r = reference.to(torch.float64)
+        offset = (r[own] - r[other[order]]).to(torch.float32)
+    word = (other | flag)[order]
+    word = torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32)   # the bits of an unsigned word
+    return {"item_offsets": offsets, "other": word, "offset": offset,
+            "weight": None if weight is None else torch.cat([weight, weight])[order]}
+
+
+def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
+    group = _indices(group, "group")
+    if group.shape[0] > _MOST:
+        raise ValueError(f"more than {_MOST} rows")
+    low, high = (int(group.min()), int(group.max())) if group.shape[0] else (0, -1)
+    n_groups = high + 1 if n_groups is None else _count(n_groups, "n_groups")
+    if low < 0 or high >= n_groups:
+        raise ValueError(f"group ids outside [0, {n_groups})")
+    if n_groups > _MOST:
+        raise ValueError(f"more than {_MOST} groups")
+    return group, n_groups
+
+
+def _lay_out_groups(group: torch.Tensor) -> dict[str, torch.Tensor | None]:
+    """Offsets of the groups that have rows, and the rows by group where they are in another order."""
+    rows = None
+    if group.shape[0] and not bool((group[1:] >= group[:-1]).all()):
+        group, order = torch.sort(group, stable=True)
+        rows = order.to(torch.int32)
+    starts = torch.nonzero(torch.cat([group.new_ones(min(1, group.shape[0])), (group[1:] != group[:-1]).to(group.dtype)]))[:, 0]
+    offsets = torch.cat([starts, starts.new_full((1,), group.shape[0])]).to(torch.int32)
+    return {"offsets": offsets, "rows": rows}
+
+
+class _Layout:
+    """Tensors on one device that calls from any stream may read."""
+
+    def _settle(self, device: torch.device, tensors: dict) -> None:
+        self.device = device
+        self._tensors = [t for t in tensors.values() if t is not None]
+        stream = torch.cuda.current_stream(device)
+        self._stream = stream.cuda_stream
+        stream.synchronize()
+
+    def _used_on(self, stream: torch.cuda.Stream) -> None:
+        if stream.cuda_stream != self._stream:
+            for t in self._tensors:
+                t.record_stream(stream)
+
+
+class RowPairs(_Layout):
+    """Pairs of rows, the first preferred to the second, laid out for :func:`preference_loss`.
+
+    ``weight`` counts a pair so many times; ``reference`` holds the scores of a reference model for all rows
+    (those of compared rows finite), so that differences of scores become differences of log ratios: where the
+    scores are log-probabilities, or differ from them by something the two rows share, that is the paired log
+    ratio of the model to the reference.  A pair may occur more than once; a row is not compared with itself."""
+
+    def __init__(self, chosen, rejected, n_rows: int, *, weight=None, reference=None, device=None) -> None:
+        n_rows = _count(n_rows, "n_rows")
+        c, r = _check_pairs(chosen, rejected, n_rows)
+        if weight is not None:
+            weight = _check_weight(weight, c.shape[0], c.device)
+        if reference is not None:
+            reference = _numbers(reference, "reference", n_rows, c.device)
+        home = _home(chosen, rejected, weight, reference, device=device)
+        with torch.cuda.device(home):
+            parts = _lay_out_pairs(c.to(home), r.to(home), n_rows, None if weight is None else weight.to(home),
+                                   None if reference is None else reference.to(home))
+            if parts["offset"] is not None and not bool(torch.isfinite(parts["offset"]).all()):
+                raise ValueError("reference scores of compared rows must be finite")
+            self.n_rows, self.n_pairs = n_rows, int(c.shape[0])
+            self.total_weight = float(self.n_pairs) if weight is None else float(weight.to(torch.float64).sum())
+            self._settle(home, parts)
+        ptr = {k: B._ptr(t) or None for k, t in parts.items()}
+        self._struct = B.Pairs(n_rows, 2 * self.n_pairs, ptr["item_offsets"], ptr["other"], ptr["offset"], ptr["weight"])
+
+
+class RowGroups(_Layout):
+    """Groups of rows (the candidates among which one chooses, the rows of an era), laid out for
+    :func:`choice_loss`, :func:`policy_loss` and :func:`group_log_probs`.  ``group`` holds the group id of
+    every row, in any order; groups without rows are allowed and count in means (``n_groups``, by default one
+    more than the largest id)."""
+
+    def __init__(self, group, n_groups: int | None = None, *, device=None) -> None:
+        g, n_groups = _check_groups(group, n_groups)
+        home = _home(group, device=device)
+        with torch.cuda.device(home):
+            parts = _lay_out_groups(g.to(home))
+            self.n_rows, self.n_groups = int(g.shape[0]), n_groups
+            self._settle(home, parts)
+        ptr = {k: B._ptr(t) or None for k, t in parts.items()}
+        self._struct = B.Groups(self.n_rows, parts["offsets"].shape[0] - 1, ptr["offsets"], ptr["rows"])
+
+
+# ---- operators --------------------------------------------------------------------------------------
+
+
+def _check_scores(scores, layout, name: str = "scores") -> torch.Tensor:
+    if not isinstance(scores, torch.Tensor) or scores.dtype not in _SCORE_TYPES:
+        raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
+    if scores.device != layout.device:
+        raise ValueError(f"{name} are on {scores.device}, the layout on {layout.device}")
+    if scores.dim() != 1 or scores.shape[0] != layout.n_rows:
+        raise ValueError(f"{name} must be 1-D with {layout.n_rows} entries")
+    return scores.detach().contiguous()
+
+
+def _per_row(values, name: str, layout) -> torch.Tensor:
+    if not isinstance(values, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if values.device != layout.device:
+        raise ValueError(f"{name} is on {values.device}, the layout on {layout.device}")
+    return _numbers(values, name, layout.n_rows, layout.device).to(torch.float32).contiguous()
+
+
+def _scale(reduction: str, total: float, what: str) -> float:
+    if reduction == "sum":
+        return 1.0
+    if reduction != "mean":
+        raise ValueError(f"unknown reduction {reduction!r}")
+    if not total > 0:
+        raise ValueError(f"the mean over no {what} is not defined")
+    return 1.0 / total
+
+
+def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) -> B.Objective:
+    beta, smoothing = float(beta), float(label_smoothing)
+    if not (beta > 0 and math.isfinite(beta)):
+        raise ValueError("beta must be positive")
+    if not 0 <= smoothing < 0.5:
+        raise ValueError("label_smoothing outside [0, 0.5)")
+    if kind not in ("logistic", "squared"):
+        raise ValueError(f"unknown kind {kind!r}")
+    if kind == "squared" and smoothing:
+        raise ValueError("the squared form has no label smoothing")
+    return B.Objective(kind=_PREFERENCE, pairs=C.pointer(pairs._struct), beta=beta, smoothing=smoothing,
+                       squared=int(kind == "squared"), scale=_scale(reduction, pairs.total_weight, "pairs"))
+
+
+def _choice_struct(groups: RowGroups, target: torch.Tensor, reduction) -> B.Objective:
+    return B.Objective(kind=_CHOICE, groups=C.pointer(groups._struct), target=B._ptr(target) or None,
+                       scale=_scale(reduction, groups.n_groups, "groups"))
+
+
+def _policy_struct(groups: RowGroups, advantage, old, reference, clip, kl_coef, reduction) -> B.Objective:
+    low, high = (float(c) for c in clip)
+    if not (0 <= low <= 1 and high >= 0):
+        raise ValueError("clip must be (low, high) with low in [0, 1] and high not negative")
+    kl_coef = float(kl_coef)
+    if not math.isfinite(kl_coef):
+        raise ValueError("kl_coef must be finite")
+    if reference is None and kl_coef:
+        raise ValueError("kl_coef needs reference_log_probs")
+    return B.Objective(kind=_POLICY, groups=C.pointer(groups._struct), advantage=B._ptr(advantage) or None,
+                       old=B._ptr(old) or None, reference=B._ptr(reference) or None, clip_low=low, clip_high=high,
+                       kl_coef=kl_coef, scale=_scale(reduction, groups.n_groups, "groups"))
+
+
+def _evaluate(struct: B.Objective, layout: _Layout, scores: torch.Tensor, policy: bool = False):
+    lib, dev = B.lib(), layout.device
+    nbytes = lib.pb_objective_workspace_bytes(C.byref(struct))
+    if nbytes < 0:
+        B.check(int(nbytes))
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream(dev)
+        layout._used_on(stream)
+        grad = torch.empty_like(scores)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        kl = torch.empty((), dtype=torch.float32, device=dev) if policy else None
+        clipped = torch.empty((), dtype=torch.int64, device=dev) if policy else None
+        scratch = torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
+        B.check(lib.pb_objective_evaluate(C.byref(struct), scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(),
+                                          loss.data_ptr(), B._ptr(kl), B._ptr(clipped), scratch.data_ptr(), nbytes,
+                                          stream.cuda_stream))
+    return PolicyLoss(loss, grad, kl, clipped) if policy else LossAndGradient(loss, grad)
+
+
+def preference_loss(scores: torch.Tensor, pairs: RowPairs, *, beta: float = 1.0, label_smoothing: float = 0.0,
+                    kind: str = "logistic", reduction: str = "sum") -> LossAndGradient:
+    """Loss of paired log ratios and its gradient with respect to the scores.
+
+    With ``d = (s_c - r_c) - (s_j - r_j)`` for a pair of chosen row c and rejected row j (r: the reference
+    scores, or 0), a pair costs, times its weight,
+
+    * ``"logistic"``: ``-(1 - e) log sigmoid(beta d) - e log sigmoid(-beta d)``, e the label smoothing: the
+      share of pairs taken to be the wrong way round;
+    * ``"squared"``: ``(d - 1 / (2 beta))^2``.
+
+    ``reduction``: ``"sum"``, or ``"mean"`` over the weights.  Rows in no pair get the gradient 0."""
+    struct = _preference_struct(pairs, beta, label_smoothing, kind, reduction)
+    return _evaluate(struct, pairs, _check_scores(scores, pairs))
+
+
+def choice_loss(scores: torch.Tensor, groups: RowGroups, target: torch.Tensor, *, reduction: str = "sum") -> LossAndGradient:
+    """Negative log-likelihood ``-sum_i target_i l_i`` of targets under the softmax of each group,
+    ``l = s - log sum exp s``, and its gradient ``exp(l_i) T - target_i`` with T the group's sum of targets.
+
+    A target is 1 for a chosen row, or any share that is not negative; groups without one contribute nothing.
+    A row with the score -inf has the probability 0 (a target on it makes the loss infinite).  ``reduction``:
+    ``"sum"``, or ``"mean"`` over the groups."""
+    target = _per_row(target, "target", groups)
+    struct = _choice_struct(groups, target, reduction)
+    return _evaluate(struct, groups, _check_scores(scores, groups))
+
+
+def policy_loss(scores: torch.Tensor, groups: RowGroups, advantage: torch.Tensor, old_log_probs: torch.Tensor, *,
+                reference_log_probs: torch.Tensor | None = None, clip: tuple[float, float] = (0.2, 0.2),
+                kl_coef: float = 0.0, reduction: str = "sum") -> PolicyLoss:
+    """Clipped policy loss of the softmax over each group, with the divergence from a reference policy.
+
+    Rows with an advantage that is not 0 are the ones an earlier policy took.  With l the log-probability of a
+    row and ``q = exp(l - old)``, such a row costs ``-min(q A, clamp(q, 1 - low, 1 + high) A)``; its gradient
+    is cut off where the clamped ratio is the smaller of the two.  A group costs ``kl_coef`` times
+    ``sum_i exp(l_i) (l_i - reference_i)``, over all its rows.
+
+    A row with the score -inf is masked: its probability is 0, its gradient is 0, and whatever else is given
+    for it is not looked at; neither is the old log-probability of a row that was not taken.  ``reduction``:
+    ``"sum"``, or ``"mean"`` over the groups."""
+    advantage = _per_row(advantage, "advantage", groups)
+    old = _per_row(old_log_probs, "old_log_probs", groups)
+    reference = None if reference_log_probs is None else _per_row(reference_log_probs, "reference_log_probs", groups)
+    struct = _policy_struct(groups, advantage, old, reference, clip, kl_coef, reduction)
+    return _evaluate(struct, groups, _check_scores(scores, groups), policy=True)
+
+
+def group_log_probs(scores: torch.Tensor, groups: RowGroups) -> torch.Tensor:
+    """``s - log sum exp s`` over each row's group, in the scores' type; -inf where the score is."""
+    scores = _check_scores(scores, groups)
+    with torch.cuda.device(groups.device):
+        stream = torch.cuda.current_stream(groups.device)
+        groups._used_on(stream)
+        out = torch.empty_like(scores)
+        B.check(B.lib().pb_group_log_probs(C.byref(groups._struct), scores.data_ptr(), _SCORE_TYPES[scores.dtype],
+                                           out.data_ptr(), stream.cuda_stream))
+    return out
+
+
+# ---- what a fit learns from --------------------------------------------------------------------------
+
+
+class _FitObjective:
+    """An objective on the rows of a fit, in the order in which the trainer holds them."""
+
+    def __init__(self, struct: B.Objective, layout: _Layout, kept: tuple) -> None:
+        self.struct, self.layout, self._kept = struct, layout, kept
+        nbytes = int(B.lib().pb_objective_workspace_bytes(C.byref(struct)))
+        if nbytes < 0:
+            B.check(nbytes)
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=layout.device)
+
+    def loss(self, preds: torch.Tensor) -> float:
+        return float(_evaluate(self.struct, self.layout, preds).loss)
+
+
+def _trainer_groups(group, n_rows: int, era_offsets: np.ndarray, order, device) -> RowGroups:
+    """Groups of a fit: the given ones, or the eras."""
+    if group is None:
+        n = len(era_offsets) - 1
+        return RowGroups(np.repeat(np.arange(n), np.diff(era_offsets)), n, device=device)
+    group, n_groups = _check_groups(group, None)
+    if group.shape[0] != n_rows:
+        raise ValueError("group must align with X rows")
+    return RowGroups(group if order is None else group[torch.from_numpy(order).to(group.device)], n_groups, device=device)
+
+
+def _trainer_rows(values, name: str, n_rows: int, order, device) -> torch.Tensor:
+    values = _numbers(values, name, n_rows, device).to(torch.float32).contiguous()
+    return values if order is None else values[torch.from_numpy(order).to(device)]
+
+
+class PreferenceObjective:
+    """``fit(..., objective=...)``: :func:`preference_loss` of the rows of X, whose numbers the pairs hold."""
+
+    def __init__(self, chosen, rejected, *, weight=None, reference=None, beta: float = 1.0, label_smoothing: float = 0.0,
+                 kind: str = "logistic", reduction: str = "sum") -> None:
+        self.chosen, self.rejected, self.weight, self.reference = chosen, rejected, weight, reference
+        self.options = (beta, label_smoothing, kind, reduction)
+
+    def _bind(self, n_rows: int, era_offsets, order, device) -> _FitObjective:
+        chosen, rejected = _check_pairs(self.chosen, self.rejected, n_rows)
+        reference = self.reference
+        if order is not None:
+            place = torch.empty(n_rows, dtype=torch.int64)
+            place[torch.from_numpy(order)] = torch.arange(n_rows)
+            place = place.to(chosen.device)
+            chosen, rejected = place[chosen], place[rejected]
+            if reference is not None:
+                reference = _numbers(reference, "reference", n_rows, device)[torch.from_numpy(order).to(device)]
+        pairs = RowPairs(chosen, rejected, n_rows, weight=self.weight, reference=reference, device=device)
+        return _FitObjective(_preference_struct(pairs, *self.options), pairs, ())
+
+
+class ChoiceObjective:
+    """``fit(..., objective=...)``: :func:`choice_loss` of the rows of X; ``group=None`` takes the eras."""
+
+    def __init__(self, target, *, group=None, reduction: str = "sum") -> None:
+        self.target, self.group, self.reduction = target, group, reduction
+
+    def _bind(self, n_rows: int, era_offsets, order, device) -> _FitObjective:
+        groups = _trainer_groups(self.group, n_rows, era_offsets, order, device)
+        target = _trainer_rows(self.target, "target", n_rows, order, device)
+        return _FitObjective(_choice_struct(groups, target, self.reduction), groups, (target,))
+
+
+class PolicyObjective:
+    """``fit(..., objective=...)``: :func:`policy_loss` of the rows of X; ``group=None`` takes the eras."""
+
+    def __init__(self, advantage, old_log_probs, *, group=None, reference_log_probs=None,
+                 clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0, reduction: str = "sum") -> None:
+        self.advantage, self.old_log_probs, self.reference_log_probs = advantage, old_log_probs, reference_log_probs
+        self.group, self.options = group, (clip, kl_coef, reduction)
+
+    def _bind(self, n_rows: int, era_offsets, order, device) -> _FitObjective:
+        groups = _trainer_groups(self.group, n_rows, era_offsets, order, device)
+        rows = [None if v is None else _trainer_rows(v, name, n_rows, order, device)
+                for v, name in ((self.advantage, "advantage"), (self.old_log_probs, "old_log_probs"),
+                                (self.reference_log_probs, "reference_log_probs"))]
+        return _FitObjective(_policy_struct(groups, *rows, *self.options), groups, tuple(rows))

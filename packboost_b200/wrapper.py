@@ -48,9 +48,10 @@ class PackBoostRegressor:
         return self
 
     def fit(self, X, y, era: Iterable[int] | None = None, *, eval_set=None, log_evaluation: int | None = None,
-            round_callback=None) -> "PackBoostRegressor":
+            round_callback=None, objective=None) -> "PackBoostRegressor":
         """``eval_set=(X_valid, y_valid, era_valid)`` adds a ``valid_corr`` entry to
-        ``booster_.round_metrics``; ``log_evaluation=n`` prints it every ``n`` rounds."""
+        ``booster_.round_metrics``; ``log_evaluation=n`` prints it every ``n`` rounds; ``objective``
+        as in :meth:`PackBoost.fit`."""
         from .booster import PackBoost
         self.booster_ = PackBoost(PackBoostConfig(**self._params))
         eval_sets = None
@@ -65,7 +66,8 @@ class PackBoostRegressor:
                 round_callback(round_idx, metrics)
 
         use_cb = cb if (log_evaluation or round_callback is not None) else None
-        self.booster_.fit(X, y, era, num_rounds=self.num_rounds, eval_sets=eval_sets, round_callback=use_cb)
+        self.booster_.fit(X, y, era, num_rounds=self.num_rounds, eval_sets=eval_sets, round_callback=use_cb,
+                          objective=objective)
         return self
 
     def predict(self, X) -> np.ndarray:

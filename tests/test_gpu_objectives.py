@@ -1,0 +1,500 @@
+"""Objectives on the GPU against their definitions in float64 (objective_util.py derives the bounds)."""
+
+import numpy as np
+import pytest
+import torch
+
+import objective_util as ref
+from objective_util import assert_close
+from packboost_b200 import PackBoost, PackBoostConfig, PackBoostRegressor
+from packboost_b200 import objectives as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _cuda(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _scores(rng, n, dtype, spread=1.0):
+    """Scores of the type, and the same numbers in float64."""
+    s = torch.from_numpy((rng.normal(size=n) * spread).astype(np.float32)).to(dtype)
+    return s.cuda(), s.double().numpy()
+
+
+# ---- preferences ---------------------------------------------------------------------------------
+
+# rows, pairs, rows that pairs choose from (hubs), rows that pairs touch
+SHAPES = [(2, 1, 0, 2), (5, 0, 0, 5), (7, 40, 0, 4), (257, 500, 0, 257), (1000, 4095, 1, 1000), (4099, 4096, 3, 4099),
+          (3000, 100_003, 2, 900), (70_001, 150_000, 0, 70_001), (100_000, 333, 0, 100_000), (20_000, 300_000, 1, 20_000)]
+
+
+def _pairs(rng, rows, pairs, hubs, touched):
+    c = rng.integers(0, hubs or touched, pairs)
+    j = rng.integers(0, max(touched - 1, 1), pairs)
+    return c, j + (j >= c)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_preference(shape, dtype):
+    rows, pairs = shape[:2]
+    rng = np.random.default_rng(rows + pairs)
+    c, j = _pairs(rng, *shape)
+    x, s = _scores(rng, rows, dtype)
+    w, r = rng.random(pairs).astype(np.float32), rng.normal(size=rows)
+    for opts in (dict(beta=0.5, smoothing=0.1), dict(beta=2.0, kind="squared"), dict(weight=w, reference=r),
+                 dict(weight=w, kind="squared"), dict(reference=r, reduction="mean")):
+        if opts.get("reduction") == "mean" and pairs == 0:
+            continue
+        plan = O.RowPairs(c, j, rows, weight=opts.get("weight"), reference=opts.get("reference"))
+        kw = {k: v for k, v in opts.items() if k in ("beta", "kind", "reduction")}
+        got = O.preference_loss(x, plan, label_smoothing=opts.get("smoothing", 0.0), **kw)
+        loss, grad, err_l, err_g = ref.pair_loss(s, c, j, **opts)
+        assert got.grad.dtype == dtype and got.loss.dtype == torch.float32 and got.loss.shape == ()
+        assert_close(got.loss, loss, err_l)
+        assert_close(got.grad, grad, err_g)
+
+
+def test_preference_far_scores_and_infinities():
+    """Differences in the tails of the sigmoid, and scores that are not finite: only rows compared with them feel it."""
+    s = np.array([0.0, 30.0, -30.0, 200.0, -np.inf, np.inf, np.nan, 1.0, 2.0, 5.0])
+    c = np.array([1, 2, 3, 0, 7, 5, 8, 7])
+    j = np.array([0, 0, 0, 3, 4, 8, 7, 8])
+    plan = O.RowPairs(np.r_[c, 6], np.r_[j, 0], 10)
+    got = O.preference_loss(_cuda(s.astype(np.float32)), plan)
+    assert torch.isnan(got.loss) and torch.isnan(got.grad[6]) and torch.isnan(got.grad[0])
+    plan = O.RowPairs(c, j, 10)
+    got = O.preference_loss(_cuda(s.astype(np.float32)), plan)
+    finite = np.array([1, 2, 3, 0, 8, 7])   # the pairs (7, 4) and (5, 8) are settled beyond doubt: no loss, no gradient
+    keep = np.array([0, 1, 2, 3, 6, 7])
+    with np.errstate(invalid="ignore"):
+        loss, grad, err_l, err_g = ref.pair_loss(np.where(np.isfinite(s), s, 0.0), c[keep], j[keep])
+    assert_close(got.loss, loss, err_l)
+    assert_close(got.grad[finite.tolist()], grad[finite], err_g[finite])
+    assert got.grad[[4, 5, 6, 9]].tolist() == [0.0] * 4
+
+
+def test_preference_does_not_depend_on_the_run():
+    rng = np.random.default_rng(0)
+    c, j = _pairs(rng, 30_000, 400_000, 2, 30_000)
+    x, _ = _scores(rng, 30_000, torch.float32)
+    a = O.preference_loss(x, O.RowPairs(c, j, 30_000))
+    for _ in range(3):
+        b = O.preference_loss(x, O.RowPairs(c, j, 30_000))
+        assert torch.equal(a.loss, b.loss) and torch.equal(a.grad, b.grad)
+
+
+# ---- groups ----------------------------------------------------------------------------------------
+
+LENGTHS = [
+    [1], [2], [1, 1, 1], [0, 3, 0, 0, 2, 0], [31, 32, 33], [127, 128, 129, 1, 1], [255, 256, 257], [511, 512, 513],
+    [1023], [1024], [1025], [1, 1023, 1, 1024, 1025, 3], [2047, 2048, 2049], [4095, 4096, 4097, 5], [5000] * 3,
+    [8191], [8192, 8193], [16383, 16384, 16385], [1, 70_001, 2], [32_768, 1, 33_000], list(range(1, 90)) * 3,
+    [4] * 5000, [300_000], [1] * 3000 + [9000] + [7] * 500,
+]
+
+
+def _groups(rng, lengths, mixed):
+    group = np.repeat(np.arange(len(lengths)), lengths)
+    return rng.permutation(group) if mixed else group
+
+
+@pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: f"{len(v)}x{max(v)}")
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+def test_groups(lengths, dtype, mixed):
+    n, n_groups = sum(lengths), len(lengths)
+    rng = np.random.default_rng(n + n_groups)
+    group = _groups(rng, lengths, mixed)
+    plan = O.RowGroups(group, n_groups)
+    assert (plan.n_rows, plan.n_groups) == (n, n_groups)
+    for masked in (0.0, 0.3):
+        x, s = _scores(rng, n, dtype, 2.0)
+        off = rng.random(n) < masked
+        if masked:
+            off |= group == group[0]            # a group with nothing left
+            x[_cuda(off)] = -np.inf
+            s[off] = -np.inf
+        l = ref.log_probs(s, group, n_groups)
+        got = O.group_log_probs(x, plan)
+        assert got.dtype == dtype
+        assert_close(got, l, ref.U * np.where(np.isfinite(l), np.abs(l), 0))
+
+        t = np.where(off | (rng.random(n) < 0.5), 0.0, rng.random(n)).astype(np.float32)
+        for reduction in ("sum", "mean"):
+            got = O.choice_loss(x, plan, _cuda(t), reduction=reduction)
+            loss, grad, err_l, err_g = ref.choice(s, group, n_groups, t, reduction)
+            assert got.grad.dtype == dtype
+            assert_close(got.loss, loss, err_l)
+            assert_close(got.grad, grad, err_g)
+
+        a = np.where(rng.random(n) < 0.4, 0.0, rng.normal(size=n)).astype(np.float32)
+        live = np.where(off, 0.0, s)
+        old = ref.log_probs(live + 0.3 * rng.normal(size=n), group, n_groups).astype(np.float32)
+        prior = ref.log_probs(live + 0.5 * rng.normal(size=n), group, n_groups).astype(np.float32)
+        old[off | (a == 0)] = np.nan            # never looked at
+        prior[off] = np.nan
+        a[off & (rng.random(n) < 0.5)] = np.nan
+        for opts in (dict(), dict(reference=prior, kl_coef=0.1, clip=(0.1, 0.3), reduction="mean"),
+                     dict(reference=prior), dict(clip=(1.0, np.inf)), dict(clip=(0.0, 0.0))):
+            kw = {k: v for k, v in opts.items() if k != "reference"}
+            got = O.policy_loss(x, plan, _cuda(a), _cuda(old),
+                                reference_log_probs=_cuda(prior) if "reference" in opts else None, **kw)
+            loss, grad, kl, clipped, err_l, err_g, err_k = ref.policy(s, group, n_groups, np.where(off, 0, a), old, **opts)
+            assert int(got.clipped) == clipped and got.clipped.dtype == torch.int64
+            assert_close(got.loss, loss, err_l)
+            assert_close(got.kl, kl, err_k)
+            assert_close(got.grad, grad, err_g)
+
+
+def test_ratios_at_their_borders():
+    """Ratios a few steps of float32 from a border fall on the side on which the definition has them."""
+    n = 4096
+    rng = np.random.default_rng(1)
+    s = rng.normal(size=n).astype(np.float32)
+    group = np.repeat(np.arange(8), n // 8)
+    l = ref.log_probs(s, group, 8)
+    a = np.where(np.arange(n) % 2 == 0, 1.0, -1.0).astype(np.float32)
+    old = (l - np.where(a > 0, np.log1p(0.2), np.log1p(-0.2))).astype(np.float32)
+    old = np.where(np.arange(n) % 3 == 0, np.nextafter(old, np.float32(9)), old)
+    plan = O.RowGroups(group)
+    got = O.policy_loss(_cuda(s), plan, _cuda(a), _cuda(old))
+    loss, grad, _, clipped, err_l, err_g, _ = ref.policy(s, group, 8, a, old)
+    assert 0 < clipped < n and int(got.clipped) == clipped
+    assert_close(got.loss, loss, err_l)
+    assert_close(got.grad, grad, err_g)
+
+
+def test_reference_equal_to_the_policy():
+    """The divergence from itself is 0 but for the rounding of the given log-probabilities."""
+    rng = np.random.default_rng(2)
+    group = np.repeat(np.arange(3), 5000)
+    s = rng.normal(size=15_000).astype(np.float32)
+    prior = ref.log_probs(s, group, 3).astype(np.float32)
+    a = np.zeros(15_000, np.float32)
+    got = O.policy_loss(_cuda(s), O.RowGroups(group), _cuda(a), _cuda(a), reference_log_probs=_cuda(prior), kl_coef=1.0)
+    loss, grad, kl, clipped, err_l, err_g, err_k = ref.policy(s, group, 3, a, a, prior, kl_coef=1.0)
+    assert clipped == int(got.clipped) == 0
+    assert_close(got.kl, kl, err_k)
+    assert_close(got.grad, grad, err_g)
+
+
+def test_scores_that_are_not_finite_stay_in_their_group():
+    group = np.repeat(np.arange(4), 300)
+    s = np.random.default_rng(3).normal(size=1200).astype(np.float32)
+    s[5], s[310], s[311] = np.nan, np.inf, -np.inf
+    t = np.zeros(1200, np.float32)
+    t[[7, 320, 700, 1000]] = 1.0
+    plan, x = O.RowGroups(group), _cuda(s)
+    l = O.group_log_probs(x, plan).cpu().numpy()
+    want = ref.log_probs(s[600:], group[600:] - 2, 2)
+    assert_close(torch.from_numpy(l[600:]), want, ref.U * np.abs(want))
+    assert np.isnan(l[:300]).all() and np.isnan(np.delete(l[300:600], 11)).all()
+    got = O.choice_loss(x, plan, _cuda(t))
+    assert torch.isnan(got.loss) and torch.isnan(got.grad[:300]).all()
+    _, grad, _, err = ref.choice(s[600:], group[600:] - 2, 2, t[600:])
+    assert_close(got.grad[600:], grad, err)
+    # a target on a masked row
+    s = np.zeros(4, np.float32)
+    s[0] = -np.inf
+    got = O.choice_loss(_cuda(s), O.RowGroups([0] * 4), _cuda(np.array([1, 0, 0, 0], np.float32)))
+    assert got.loss.item() == np.inf and got.grad[0].item() == -1.0
+
+
+def test_far_scores():
+    """Scores far apart, far from zero and at the ends of the type."""
+    for s in ([1e30, 0.0, -1e30], [-1e30, -1e30, -3e38], [800.0, 100.0, 799.0, -700.0], [-5e4, -5e4 + 1.0], [3e38, 3e38, -3e38]):
+        s = np.array(s, np.float32)
+        group = np.zeros(len(s), int)
+        l = ref.log_probs(s, group, 1)
+        plan = O.RowGroups(group)
+        assert_close(O.group_log_probs(_cuda(s), plan), l, ref.U * np.abs(l))
+        t = np.ones(len(s), np.float32)
+        got = O.choice_loss(_cuda(s), plan, _cuda(t))
+        loss, grad, err_l, err_g = ref.choice(s, group, 1, t)
+        assert_close(got.loss, loss, err_l)
+        assert_close(got.grad, grad, err_g)
+
+
+def test_no_rows():
+    plan = O.RowGroups([], 3)
+    e = torch.empty(0, device="cuda")
+    assert O.group_log_probs(e, plan).shape == (0,)
+    got = O.policy_loss(e, plan, e, e, reference_log_probs=e, kl_coef=0.5, reduction="mean")
+    assert (got.loss.item(), got.kl.item(), got.clipped.item()) == (0.0, 0.0, 0) and got.grad.shape == (0,)
+    got = O.preference_loss(e, O.RowPairs([], [], 0))
+    assert got.loss.item() == 0.0 and got.grad.shape == (0,)
+
+
+# ---- calls ---------------------------------------------------------------------------------------------
+
+
+def _problem(seed, n=50_000):
+    rng = np.random.default_rng(seed)
+    group = np.sort(rng.integers(0, 40, n))
+    group[:9000] = 0
+    x, _ = _scores(rng, n, torch.float32)
+    a, old = _cuda(rng.normal(size=n).astype(np.float32)), _cuda(rng.normal(size=n).astype(np.float32) - 7)
+    c, j = _pairs(rng, n, 90_000, 3, n)
+    return x, O.RowGroups(group), a, old, O.RowPairs(c, j, n)
+
+
+def _all(x, groups, a, old, pairs):
+    return [*O.preference_loss(x, pairs), *O.choice_loss(x, groups, a.abs()), *O.policy_loss(x, groups, a, old, reference_log_probs=old, kl_coef=0.1),
+            O.group_log_probs(x, groups)]
+
+
+def test_strided_and_offset_arguments():
+    x, groups, a, old, pairs = _problem(5)
+    want = _all(x, groups, a, old, pairs)
+    wide = torch.stack([x, -x], 1)
+    shifted = torch.cat([x.new_zeros(1), x])[1:]
+    for scores in (wide[:, 0], shifted):
+        got = _all(scores, groups, a.double(), torch.stack([old, old], 1)[:, 1], pairs)
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+    h = x.half()
+    want = _all(h, groups, a, old, pairs)
+    got = _all(torch.cat([h.new_zeros(1), h])[1:], groups, a, old, pairs)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_streams_and_graphs():
+    x, groups, a, old, pairs = _problem(6)
+    y = x * 0.7 - 0.1
+    want_x, want_y = _all(x, groups, a, old, pairs), _all(y, groups, a, old, pairs)
+    torch.cuda.synchronize()
+    # two streams at once, the layouts shared
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i, (s, v) in enumerate(zip(streams, (x, y))):
+            with torch.cuda.stream(s):
+                got[i].append(_all(v, groups, a, old, pairs))
+    torch.cuda.synchronize()
+    for runs, want in zip(got, (want_x, want_y)):
+        for run in runs:
+            assert all(torch.equal(g, w) for g, w in zip(run, want))
+    # two captured graphs of the same layouts, replayed in turn and at once
+    graphs, outs, ins = [], [], [x.clone(), y.clone()]
+    for v in ins:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_all(v, groups, a, old, pairs))
+        graphs.append(g)
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, (want_x, want_y)):
+            assert all(torch.equal(o, w) for o, w in zip(out, want))
+    ins[0].copy_(y)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs[0], want_y))
+
+
+def test_a_layout_may_go_while_its_call_runs():
+    want = _all(*_problem(7))
+    side = torch.cuda.Stream()
+    args = _problem(7)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = _all(*args)
+    del args
+    torch.cuda.current_stream().synchronize()
+    junk = [torch.full((200_000,), 7, dtype=torch.int32, device="cuda") for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want)) and len(junk) == 20
+
+
+# ---- fits ------------------------------------------------------------------------------------------------
+
+CFG = dict(pack_size=4, max_depth=4, learning_rate=0.1, lambda_l2=1.0, lambda_dro=0.3, min_samples_leaf=5, max_bins=32,
+           random_state=11, layer_feature_fraction=0.7)
+
+
+def _table(n=6000, f=12, eras=7, mixed=False, seed=0):
+    rng = np.random.default_rng(seed)
+    X = rng.normal(size=(n, f)).astype(np.float32)
+    era = np.sort(rng.integers(0, eras, n)).astype(np.int16)
+    if mixed:
+        era = rng.permutation(era)
+    return X, era, rng
+
+
+def _objectives(n, era, rng):
+    c = rng.integers(0, n, 3 * n)
+    j = (c + rng.integers(1, n, 3 * n)) % n
+    group = rng.integers(0, n // 9, n)
+    t, a = rng.random(n).astype(np.float32), rng.normal(size=n).astype(np.float32)
+    old = ref.log_probs(rng.normal(size=n) * 0.3, group, n // 9 + 1).astype(np.float32)
+    r, w = rng.normal(size=n) * 0.2, rng.random(3 * n).astype(np.float32)
+    era_ids = np.unique(era, return_inverse=True)[1]
+    old_era = ref.log_probs(rng.normal(size=n) * 0.3, era_ids, era_ids.max() + 1).astype(np.float32)
+
+    def preference(s):
+        return ref.pair_loss(s, c, j, weight=w, reference=r, beta=0.8)[:2]
+
+    def choice(s):
+        return ref.choice(s, era_ids, era_ids.max() + 1, t)[:2]
+
+    def policy(s):
+        return ref.policy(s, group, n // 9 + 1, a, old, old, (0.2, 0.2), 0.2)[:2]
+
+    def policy_era(s):
+        return ref.policy(s, era_ids, era_ids.max() + 1, a, old_era)[:2]
+
+    return [(O.PreferenceObjective(c, j, weight=w, reference=r, beta=0.8), preference), (O.ChoiceObjective(t), choice),
+            (O.PolicyObjective(a, old, group=group, reference_log_probs=old, kl_coef=0.2), policy),
+            (O.PolicyObjective(_cuda(a), _cuda(old_era)), policy_era)]
+
+
+def _same_trees(a, b):
+    assert len(a.trees) == len(b.trees)
+    for x, y in zip(a.trees, b.trees):
+        p, q = x.arrays(), y.arrays()
+        assert all(np.array_equal(p[k], q[k]) for k in p)
+
+
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+@pytest.mark.parametrize("which", range(4))
+def test_fit_learns_from_the_objective(mixed, which):
+    """Every round's leaves hold the mean negative gradient of the objective at the predictions before it, and the first
+    tree is, bit for bit, that of the squared loss on those gradients."""
+    X, era, rng = _table(mixed=mixed)
+    objective, formula = _objectives(len(X), era, rng)[which]
+    seen = []
+    b = PackBoost(PackBoostConfig(**CFG))
+    b.fit(X, None, era, num_rounds=3, objective=objective, round_callback=lambda r, m: seen.append(m["train_loss"]))
+    bins = torch.from_numpy(np.stack([np.searchsorted(b._binner.bin_edges[:, k], X[:, k]) for k in range(X.shape[1])], 1)
+                            .clip(0, 31).astype(np.uint8)).cuda()
+    preds = np.zeros(len(X))
+    for r, (tree, repeat) in enumerate(b._distinct):
+        loss, grad = formula(preds)
+        value = tree.predict_bins(bins).cpu().numpy()
+        for v in np.unique(value):
+            rows = value == v
+            g, size = grad[rows].sum(), np.abs(grad[rows]).sum()
+            # rows whose leaves have the same value by chance share a check; 1e-5: the predictions and the quantised
+            # gradients of earlier rounds are float32
+            lam = CFG["lambda_l2"]
+            assert abs(v * (rows.sum() + lam) + g) <= 1e-5 * size + 1e-6 or _several_leaves(tree, v)
+        preds = preds + CFG["learning_rate"] * repeat * value.astype(np.float64)
+        assert abs(seen[r] - formula(preds)[0]) <= 1e-5 * (abs(seen[r]) + len(X) * 1e-2)
+    np.testing.assert_allclose(b.train_predictions(), preds, rtol=1e-5, atol=1e-6)
+
+    one = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=1, objective=objective)
+    plain = PackBoost(PackBoostConfig(**CFG))
+    plain._start(X, np.zeros(len(X), np.float32), era)
+    bound = objective._bind(len(X), *_order(era), torch.device("cuda", 0))
+    g = O._evaluate(bound.struct, bound.layout, torch.zeros(len(X), device="cuda")).grad
+    plain._trainer.y.copy_(-g)
+    plain._boost_one_round(0, 1)
+    plain._finish()
+    _same_trees(one, plain)
+
+
+def _order(era):
+    from packboost_b200.data import sort_eras
+    _, offsets, order = sort_eras(era, len(era))
+    return offsets, order
+
+
+def _several_leaves(tree, v):
+    a = tree.arrays()
+    return ((a["value"] == np.float32(v)) & (a["is_leaf"] != 0)).sum() > 1
+
+
+@pytest.mark.parametrize("env", [{"PACKBOOST_CUDA_GRAPH": "0"}, {"PACKBOOST_RUN_AHEAD": "0"}, {"PACKBOOST_TRAIN_METRICS": "1"}])
+@pytest.mark.parametrize("which", [0, 2])
+def test_fit_is_the_same_however_it_is_launched(env, which, monkeypatch):
+    X, era, rng = _table(seed=3)
+    objective, _ = _objectives(len(X), era, rng)[which]
+    want = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=6, objective=objective)
+    for k, v in env.items():
+        monkeypatch.setenv(k, v)
+    got = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=6, objective=objective)
+    _same_trees(want, got)
+    assert np.array_equal(want.train_predictions(), got.train_predictions())
+
+
+def test_fit_phase_by_phase_is_the_loop():
+    """The launches of several GPUs' ranks, which go phase by phase, on one."""
+    X, era, rng = _table(seed=4)
+    objective, _ = _objectives(len(X), era, rng)[0]
+    want = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=4, objective=objective)
+    got = PackBoost(PackBoostConfig(**CFG))
+    got._start(X, None, era, objective=objective)
+    tr = got._trainer
+    loop, tr.loop, tr.use_graph = tr.loop, None, False
+    tr.log_event = [torch.cuda.Event() for _ in range(len(tr.log_host))]
+    for r in range(4):
+        got._boost_one_round(r, 4)
+    got._finish()
+    tr.loop = loop
+    _same_trees(want, got)
+
+
+def test_fit_that_stops_early_is_taken_again():
+    """Frontiers that empty before the last depth make the round after them be enqueued twice."""
+    X, era, rng = _table(n=300, seed=5)
+    objective, _ = _objectives(len(X), era, rng)[0]
+    cfg = dict(CFG, min_samples_leaf=70, max_depth=5)
+    got = PackBoost(PackBoostConfig(**cfg)).fit(X, None, era, num_rounds=5, objective=objective)
+    calm = PackBoost(PackBoostConfig(**cfg))
+    calm.fit(X, None, era, num_rounds=5, objective=objective, round_callback=lambda r, m: None)
+    assert min(got._round_depths) < 5
+    _same_trees(got, calm)
+
+
+def test_from_choices_to_preferences_to_a_policy():
+    """The three one after the other, as they are used: log-probabilities of a model are the reference of the next."""
+    X, era, rng = _table(n=4000, seed=6)
+    n = len(X)
+    group = rng.integers(0, 500, n)
+    quality = X[:, 0] + 0.5 * X[:, 1] ** 2
+    first = PackBoostRegressor(num_rounds=5, **CFG).fit(X, None, era, objective=O.ChoiceObjective((quality > 1).astype(np.float32), group=group))
+    prior = first.booster_.predict_log_probs(X, group)
+    want = ref.log_probs(first.predict(X), group, 500)
+    assert_close(torch.from_numpy(prior), want, ref.U * np.abs(want))
+    c = rng.integers(0, n, 8000)
+    j = (c + rng.integers(1, n, 8000)) % n
+    c, j = np.where(quality[c] > quality[j], c, j), np.where(quality[c] > quality[j], j, c)
+    second = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=5, objective=O.PreferenceObjective(c, j, reference=prior, beta=0.5))
+    old = second.predict_log_probs(X, group)
+    a = np.where(rng.random(n) < 0.3, quality - quality.mean(), 0).astype(np.float32)
+    third = PackBoost(PackBoostConfig(**CFG))
+    third.fit(X, quality, era, num_rounds=5, objective=O.PolicyObjective(a, old, group=group, reference_log_probs=prior, kl_coef=0.05),
+              eval_sets=[("valid", X[:500], quality[:500], era[:500])], round_callback=lambda r, m: None)
+    assert all(np.isfinite(m["train_loss"]) and "valid_corr" in m for m in third.round_metrics)
+    with pytest.raises(ValueError):
+        third.predict_log_probs(X, group[:-1])
+    # and the squared loss after them, on the same booster, as ever
+    third._rng.manual_seed(CFG["random_state"])
+    third.fit(X, quality, era, num_rounds=3)
+    _same_trees(third, PackBoost(PackBoostConfig(**CFG)).fit(X, quality, era, num_rounds=3))
+    assert "train_loss" not in third.round_metrics[0]
+
+
+def test_refused_fits():
+    X, era, rng = _table(n=200)
+    b = PackBoost(PackBoostConfig(**CFG))
+    for objective, error in ((O.PreferenceObjective([0], [200]), ValueError), (O.ChoiceObjective(np.zeros(199)), ValueError),
+                             (O.ChoiceObjective(np.zeros(200), group=[0] * 199), ValueError),
+                             (O.PolicyObjective(np.zeros(200), np.zeros(200), kl_coef=1.0), ValueError),
+                             (O.PreferenceObjective([0], [1], beta=-1), ValueError)):
+        with pytest.raises(error):
+            b.fit(X, None, era, num_rounds=1, objective=objective)
+    with pytest.raises(ValueError):
+        b.fit(X, None, era, num_rounds=1)
+    x = torch.zeros(200, device="cuda")
+    with pytest.raises(ValueError):
+        O.choice_loss(x, O.RowGroups([0] * 200), x.cpu())
+    with pytest.raises(ValueError):
+        O.preference_loss(x.cpu(), O.RowPairs([0], [1], 200))
