@@ -411,22 +411,51 @@ typedef struct pb_round_log_header {
 #define PB_SCORE_F16 1
 #define PB_SCORE_BF16 2
 
-/* Pairs by row: a pair is one item of each of its two rows.  Items of a row are neighbours. */
+/* Pairs by row.  A pair is one item of each of its two rows; a row without pairs has one item that names
+ * the row itself, and so have the places that fill the last tile of PB_PAIR_TILE items.  Items are in the
+ * order of their rows.  A run of `run_tiles` tiles is one CTA's; a cut is a row whose items lie in several
+ * runs: row, first run, last run. */
+#define PB_PAIR_ITEMS 8
+#define PB_PAIR_TILE 1024
 typedef struct pb_pairs {
     int64_t n_rows;
-    int64_t n_items;             /* two per pair */
-    const int32_t* item_offsets; /* [n_rows + 1] */
-    const uint32_t* other;       /* [n_items] the other row; bit 31: the item's own row is the rejected one */
-    const float* offset;         /* [n_items] reference score of the own row minus the other's, or NULL */
-    const float* weight;         /* [n_items], or NULL: 1 */
+    int64_t n_items;              /* a multiple of PB_PAIR_TILE */
+    const uint32_t* other;        /* [n_items] the other row; bit 31: the item's own row is the rejected one; 16-byte aligned */
+    const float* offset;          /* [n_items] reference score of the own row minus the other's, or NULL; aligned alike */
+    const float* weight;          /* [n_items], or NULL: 1; aligned alike */
+    const int32_t* chunk_rows;    /* [n_items / 8] row of the first of eight items */
+    const uint8_t* chunk_heads;   /* [n_items / 8] which of the eight are the first of their row */
+    int64_t run_tiles;
+    int64_t n_cuts;
+    const int32_t* cuts;          /* [n_cuts][3] */
 } pb_pairs;
 
-/* Groups of rows: those that have any, `rows` lists their rows (NULL: the rows in order). */
+/* Groups of rows: those that have any, `rows` lists their rows (NULL: the rows in order).  By length:
+ * up to PB_SHORT_ROWS rows in windows of PB_WINDOW_ROWS places that start PB_WINDOW_STEP apart, a group
+ * belonging to the window k that its first place is in, k * PB_WINDOW_STEP <= place < (k + 1) *
+ * PB_WINDOW_STEP, with a word for every four places (bits 0-3: first places of groups of the window, 4-7:
+ * places of its groups, 8-11: last ones, from 12: its groups that begin before the four); up to
+ * PB_MEDIUM_ROWS and up to PB_LARGE_ROWS rows, by the group's number; longer ones in pieces of up to
+ * PB_PIECE_ROWS: first place, places, number of the group's first piece, how many it has. */
+#define PB_SHORT_ROWS 128
+#define PB_WINDOW_ROWS 1024
+#define PB_WINDOW_STEP 896
+#define PB_MEDIUM_ROWS 1024
+#define PB_LARGE_ROWS 8192
+#define PB_PIECE_ROWS 4096
 typedef struct pb_groups {
     int64_t n_rows;
     int64_t n_groups;
-    const int32_t* offsets;      /* [n_groups + 1] */
-    const int32_t* rows;         /* [n_rows], or NULL */
+    const int32_t* offsets;       /* [n_groups + 1] */
+    const int32_t* rows;          /* [n_rows], or NULL */
+    int64_t n_windows;
+    const int32_t* windows;       /* [n_windows] k */
+    const uint32_t* window_words; /* [n_windows][PB_WINDOW_ROWS / 4] */
+    int64_t n_medium;
+    int64_t n_large;
+    const int32_t* listed;        /* [n_medium + n_large] */
+    int64_t n_pieces;
+    const int32_t* pieces;        /* [n_pieces][4] */
 } pb_groups;
 
 typedef struct pb_objective {
@@ -458,8 +487,11 @@ int64_t pb_objective_workspace_bytes(const pb_objective* o);
 int pb_objective_evaluate(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss,
                           float* kl, int64_t* clipped, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Log-probabilities of the rows in their groups (of the scores' type; -inf where the score is). */
-int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* stream);
+/* Log-probabilities of the rows in their groups (of the scores' type; -inf where the score is), with
+ * scratch of pb_group_log_probs_bytes(g) bytes. */
+int64_t pb_group_log_probs_bytes(const pb_groups* g);
+int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /* pb_round_begin with the gradient of an objective in the place of g = preds - y (`y` is not read);
  * the rows of the objective are the state's. */

@@ -77,13 +77,19 @@ class Model(C.Structure):
 class Pairs(C.Structure):
     """Mirror of ``pb_pairs``."""
 
-    _fields_ = [("n_rows", i64), ("n_items", i64), ("item_offsets", vp), ("other", vp), ("offset", vp), ("weight", vp)]
+    _fields_ = [
+        ("n_rows", i64), ("n_items", i64), ("other", vp), ("offset", vp), ("weight", vp), ("chunk_rows", vp),
+        ("chunk_heads", vp), ("run_tiles", i64), ("n_cuts", i64), ("cuts", vp),
+    ]
 
 
 class Groups(C.Structure):
     """Mirror of ``pb_groups``."""
 
-    _fields_ = [("n_rows", i64), ("n_groups", i64), ("offsets", vp), ("rows", vp)]
+    _fields_ = [
+        ("n_rows", i64), ("n_groups", i64), ("offsets", vp), ("rows", vp), ("n_windows", i64), ("windows", vp),
+        ("window_words", vp), ("n_medium", i64), ("n_large", i64), ("listed", vp), ("n_pieces", i64), ("pieces", vp),
+    ]
 
 
 class Objective(C.Structure):
@@ -149,7 +155,8 @@ _PROTOS: dict[str, tuple[Any, list[Any]]] = {
     "pb_objective_struct_bytes": (i64, [i64]),
     "pb_objective_workspace_bytes": (i64, [C.POINTER(Objective)]),
     "pb_objective_evaluate": (C.c_int, [C.POINTER(Objective), vp, i64, vp, vp, vp, vp, vp, i64, vp]),
-    "pb_group_log_probs": (C.c_int, [C.POINTER(Groups), vp, i64, vp, vp]),
+    "pb_group_log_probs_bytes": (i64, [C.POINTER(Groups)]),
+    "pb_group_log_probs": (C.c_int, [C.POINTER(Groups), vp, i64, vp, vp, i64, vp]),
     "pb_round_begin_objective": (C.c_int, [C.POINTER(TrainState), C.POINTER(Objective), i64, vp, i64, vp]),
     "pb_loop_submit_objective": (C.c_int, [vp, vp, C.POINTER(Objective), vp, i64, i64, vp, vp, i64, vp, i64, i64, vp]),
     "pb_hist_build": (C.c_int, [C.POINTER(TrainState), vp, i64, i64, i64, vp, vp, vp]),

@@ -106,8 +106,8 @@ def _check_pairs(chosen, rejected, n_rows: int) -> tuple[torch.Tensor, torch.Ten
     chosen, rejected = _indices(chosen, "chosen"), _indices(rejected, "rejected")
     if chosen.shape[0] != rejected.shape[0]:
         raise ValueError("chosen and rejected differ in length")
-    if 2 * chosen.shape[0] > _MOST:
-        raise ValueError(f"more than {_MOST // 2} pairs")
+    if 2 * chosen.shape[0] + n_rows + _PAIR_TILE > _MOST:
+        raise ValueError("more rows and sides of pairs than 32-bit numbers count")
     rejected = rejected.to(chosen.device)
     if chosen.shape[0]:
         low = min(int(chosen.min()), int(rejected.min()))
@@ -126,21 +126,52 @@ def _check_weight(weight, n_pairs: int, device) -> torch.Tensor:
     return weight
 
 
-def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict[str, torch.Tensor | None]:
-    """The items of every row, neighbours in the order in which the pairs were given (chosen side first)."""
-    own, other = torch.cat([chosen, rejected]), torch.cat([rejected, chosen])
-    flag = torch.cat([torch.zeros_like(chosen), torch.full_like(rejected, 1 << 31)])
-    own, order = torch.sort(own, stable=True)
-    counts = torch.bincount(own, minlength=n_rows)[:n_rows]
-    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32)
-    offset = None
+# (the layouts below are the ones of include/packboost_b200.h; they are made by torch, on any device)
+_PAIR_ITEMS, _PAIR_TILE = 8, 1024
+_RUNS_PER_SM = 8
+
+
+def _lay_out_pairs(chosen, rejected, n_rows, weight, reference, n_sm: int = 148) -> dict:
+    """Items by row, in the order in which the pairs were given (chosen side first)."""
+    dev = chosen.device
+    if n_rows == 0:
+        return {"n_items": 0, "run_tiles": 1, "n_cuts": 0}
+    touched = torch.zeros(n_rows, dtype=torch.bool, device=dev)
+    touched[chosen] = True
+    touched[rejected] = True
+    alone = torch.nonzero(~touched)[:, 0]
+    n_pairs = chosen.shape[0]
+    n_real = 2 * n_pairs + alone.shape[0]
+    fill = torch.full((-n_real % _PAIR_TILE,), n_rows - 1, dtype=torch.int64, device=dev)
+    own, order = torch.sort(torch.cat([chosen, rejected, alone, fill]).to(torch.int32), stable=True)
+    other = torch.cat([rejected, chosen, alone, fill])
+    other[n_pairs: 2 * n_pairs] |= 1 << 31
+    other = torch.where(other >= 1 << 31, other - (1 << 32), other).to(torch.int32)[order]   # bits of an unsigned word
+    out = {"n_items": own.shape[0], "other": other, "offset": None, "weight": None}
     if reference is not None:
         r = reference.to(torch.float64)
-        offset = (r[own] - r[other[order]]).to(torch.float32)
-    word = (other | flag)[order]
-    word = torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32)   # the bits of an unsigned word
-    return {"item_offsets": offsets, "other": word, "offset": offset,
-            "weight": None if weight is None else torch.cat([weight, weight])[order]}
+        away = r[chosen] - r[rejected]
+        none = away.new_zeros(own.shape[0] - 2 * n_pairs)
+        out["offset"] = torch.cat([away, -away, none]).to(torch.float32)[order]
+    if weight is not None:
+        out["weight"] = torch.cat([weight, weight, weight.new_zeros(own.shape[0] - 2 * n_pairs)])[order]
+    heads = torch.ones_like(own, dtype=torch.bool)
+    heads[1:] = own[1:] != own[:-1]
+    out["chunk_rows"] = own[::_PAIR_ITEMS].contiguous()
+    bits = heads.view(-1, _PAIR_ITEMS).to(torch.uint8) << torch.arange(_PAIR_ITEMS, dtype=torch.uint8, device=dev)
+    out["chunk_heads"] = bits.sum(1, dtype=torch.uint8)
+    n_tiles = own.shape[0] // _PAIR_TILE
+    out["run_tiles"] = run_tiles = -(-n_tiles // (n_sm * _RUNS_PER_SM))
+    # rows that go on over the border of two runs, each with its first and its last run
+    border = torch.arange(run_tiles, n_tiles, run_tiles, device=dev) * _PAIR_TILE
+    rows = own[border].cpu().numpy()
+    runs = np.flatnonzero(rows == own[border - 1].cpu().numpy()) + 1
+    rows = rows[runs - 1]
+    first = np.flatnonzero(np.r_[True, rows[1:] != rows[:-1]][: len(rows)])
+    last = np.r_[first[1:] - 1, len(rows) - 1][: len(first)]
+    out["n_cuts"] = len(first)
+    out["cuts"] = torch.from_numpy(np.stack([rows[first], runs[first] - 1, runs[last]], 1).astype(np.int32)).to(dev)
+    return out
 
 
 def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
@@ -156,23 +187,76 @@ def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
     return group, n_groups
 
 
-def _lay_out_groups(group: torch.Tensor) -> dict[str, torch.Tensor | None]:
-    """Offsets of the groups that have rows, and the rows by group where they are in another order."""
+_SHORT, _WINDOW, _STEP, _MEDIUM, _LARGE, _PIECE = 128, 1024, 896, 1024, 8192, 4096
+
+
+def _lay_out_groups(group: torch.Tensor) -> dict:
+    """Offsets of the groups that have rows, the rows by group where they are in another order, and the groups by
+    length: windows of short ones, lists of those a CTA holds, pieces of long ones."""
+    n, dev = group.shape[0], group.device
+    if n == 0:
+        return {"n_groups": 0, "n_windows": 0, "n_medium": 0, "n_large": 0, "n_pieces": 0}
     rows = None
-    if group.shape[0] and not bool((group[1:] >= group[:-1]).all()):
+    if not bool((group[1:] >= group[:-1]).all()):
         group, order = torch.sort(group, stable=True)
         rows = order.to(torch.int32)
-    starts = torch.nonzero(torch.cat([group.new_ones(min(1, group.shape[0])), (group[1:] != group[:-1]).to(group.dtype)]))[:, 0]
-    offsets = torch.cat([starts, starts.new_full((1,), group.shape[0])]).to(torch.int32)
-    return {"offsets": offsets, "rows": rows}
+    heads = torch.ones(n, dtype=torch.bool, device=dev)
+    heads[1:] = group[1:] != group[:-1]
+    starts = torch.nonzero(heads)[:, 0]
+    offsets = torch.cat([starts, starts.new_full((1,), n)])
+    lengths = offsets[1:] - offsets[:-1]
+    out = {"rows": rows, "offsets": offsets.to(torch.int32), "n_groups": starts.shape[0], "windows": None,
+           "window_words": None}
+
+    short = lengths <= _SHORT
+    windows = torch.unique(starts[short] // _STEP)
+    out["n_windows"] = windows.shape[0]
+    if out["n_windows"]:
+        number = heads.cumsum(0) - 1                       # group of a place
+        home = torch.where(short, starts // _STEP, torch.full_like(starts, -1))[number]
+        place = windows[:, None] * _STEP + torch.arange(_WINDOW, device=dev)
+        inside = place < n
+        place = place.clamp_max(n - 1)
+        mine = inside & (home[place] == windows[:, None])
+        first = mine & heads[place]
+        last = mine & (place + 1 == offsets[1:][number[place]])
+        shape = (out["n_windows"], _WINDOW // 4, 4)
+        bit = torch.arange(4, device=dev)
+        word = ((first.view(shape) << bit) | (mine.view(shape) << (bit + 4)) | (last.view(shape) << (bit + 8))).sum(2)
+        begun = first.view(shape).sum(2)
+        out["window_words"] = (word | ((begun.cumsum(1) - begun) << 12)).to(torch.int32)
+        out["windows"] = windows.to(torch.int32)
+
+    medium = torch.nonzero(~short & (lengths <= _MEDIUM))[:, 0]
+    large = torch.nonzero((lengths > _MEDIUM) & (lengths <= _LARGE))[:, 0]
+    out["n_medium"], out["n_large"] = medium.shape[0], large.shape[0]
+    out["listed"] = torch.cat([medium, large]).to(torch.int32)
+    long = lengths > _LARGE
+    begin, length = starts[long].cpu().numpy(), lengths[long].cpu().numpy()
+    count = -(-length // _PIECE)
+    first = np.cumsum(count) - count
+    which = np.repeat(np.arange(len(count)), count)
+    step = (np.arange(len(which)) - first[which]) * _PIECE
+    table = np.stack([begin[which] + step, np.minimum(length[which] - step, _PIECE), first[which], count[which]], 1)
+    out["n_pieces"] = len(which)
+    out["pieces"] = torch.from_numpy(table.astype(np.int32)).to(dev)
+    return out
 
 
 class _Layout:
-    """Tensors on one device that calls from any stream may read."""
+    """Tensors on one device that calls from any stream may read, and the structure that points at them."""
+
+    def _point(self, struct: type, tables: dict, **numbers):
+        fields = dict(numbers)
+        for name, _ in struct._fields_:
+            v = tables.get(name)
+            if v is not None:
+                fields[name] = (v.data_ptr() or None) if isinstance(v, torch.Tensor) else v
+        return struct(**fields)
 
     def _settle(self, device: torch.device, tensors: dict) -> None:
         self.device = device
-        self._tensors = [t for t in tensors.values() if t is not None]
+        self._tensors = [t for t in tensors.values() if isinstance(t, torch.Tensor)]
         stream = torch.cuda.current_stream(device)
         self._stream = stream.cuda_stream
         stream.synchronize()
@@ -201,14 +285,14 @@ class RowPairs(_Layout):
         home = _home(chosen, rejected, weight, reference, device=device)
         with torch.cuda.device(home):
             parts = _lay_out_pairs(c.to(home), r.to(home), n_rows, None if weight is None else weight.to(home),
-                                   None if reference is None else reference.to(home))
-            if parts["offset"] is not None and not bool(torch.isfinite(parts["offset"]).all()):
+                                   None if reference is None else reference.to(home),
+                                   torch.cuda.get_device_properties(home).multi_processor_count)
+            if parts.get("offset") is not None and not bool(torch.isfinite(parts["offset"]).all()):
                 raise ValueError("reference scores of compared rows must be finite")
             self.n_rows, self.n_pairs = n_rows, int(c.shape[0])
             self.total_weight = float(self.n_pairs) if weight is None else float(weight.to(torch.float64).sum())
             self._settle(home, parts)
-        ptr = {k: B._ptr(t) or None for k, t in parts.items()}
-        self._struct = B.Pairs(n_rows, 2 * self.n_pairs, ptr["item_offsets"], ptr["other"], ptr["offset"], ptr["weight"])
+        self._struct = self._point(B.Pairs, parts, n_rows=n_rows)
 
 
 class RowGroups(_Layout):
@@ -224,8 +308,7 @@ class RowGroups(_Layout):
             parts = _lay_out_groups(g.to(home))
             self.n_rows, self.n_groups = int(g.shape[0]), n_groups
             self._settle(home, parts)
-        ptr = {k: B._ptr(t) or None for k, t in parts.items()}
-        self._struct = B.Groups(self.n_rows, parts["offsets"].shape[0] - 1, ptr["offsets"], ptr["rows"])
+        self._struct = self._point(B.Groups, parts, n_rows=self.n_rows)
 
 
 # ---- operators --------------------------------------------------------------------------------------
@@ -366,8 +449,11 @@ def group_log_probs(scores: torch.Tensor, groups: RowGroups) -> torch.Tensor:
         stream = torch.cuda.current_stream(groups.device)
         groups._used_on(stream)
         out = torch.empty_like(scores)
-        B.check(B.lib().pb_group_log_probs(C.byref(groups._struct), scores.data_ptr(), _SCORE_TYPES[scores.dtype],
-                                           out.data_ptr(), stream.cuda_stream))
+        lib, struct = B.lib(), C.byref(groups._struct)
+        nbytes = int(lib.pb_group_log_probs_bytes(struct))
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=groups.device)
+        B.check(lib.pb_group_log_probs(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], out.data_ptr(),
+                                       scratch.data_ptr(), nbytes, stream.cuda_stream))
     return out
 
 

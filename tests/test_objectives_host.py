@@ -63,15 +63,89 @@ def test_group_formulas_against_differences(reduction):
     np.testing.assert_allclose(loss(s)[1], _differences(lambda v: loss(v)[0], s), rtol=0, atol=_DIFF)
 
 
-@pytest.mark.parametrize("ids,in_order", [([], True), ([4], True), ([0, 0, 3, 3, 3, 7], True), ([3, 0, 3, 7, 0, 3], False)])
-def test_layout_of_groups(ids, in_order):
-    lay = O._lay_out_groups(torch.tensor(ids, dtype=torch.int64))
-    rows = np.arange(len(ids)) if lay["rows"] is None else lay["rows"].numpy()
-    assert (lay["rows"] is None) == in_order
+def _pairs(rng, rows, pairs, hubs, touched):
+    c = rng.integers(0, hubs or touched, pairs)
+    j = rng.integers(0, max(touched - 1, 1), pairs)
+    return c, j + (j >= c)
+
+
+@pytest.mark.parametrize("rows,pairs,hubs,touched,n_sm", [(1, 0, 0, 1, 148), (9, 23, 0, 7, 148), (5000, 2000, 0, 5000, 148),
+                                                          (400, 9000, 1, 300, 1), (30_000, 40_000, 2, 30_000, 1),
+                                                          (2, 20_000, 0, 2, 1), (8192, 0, 0, 8192, 1)])
+def test_layout_of_pairs(rows, pairs, hubs, touched, n_sm):
+    rng = np.random.default_rng(rows + pairs)
+    c, j = _pairs(rng, rows, pairs, hubs, touched)
+    w, r = rng.random(pairs).astype(np.float32), rng.normal(size=rows)
+    lay = O._lay_out_pairs(torch.from_numpy(c), torch.from_numpy(j), rows, torch.from_numpy(w), torch.from_numpy(r), n_sm)
+    n = lay["n_items"]
+    assert n % O._PAIR_TILE == 0
+    word = lay["other"].numpy().view(np.uint32)
+    other, rejected = (word & 0x7FFFFFFF).astype(np.int64), word >> 31 == 1
+    heads = np.unpackbits(lay["chunk_heads"].numpy(), bitorder="little").astype(bool)
+    own = np.cumsum(heads) - 1                      # every row has items
+    assert heads[0] and own[-1] == rows - 1
+    np.testing.assert_array_equal(lay["chunk_rows"].numpy(), own[::8])
+    real = other != own
+    assert real.sum() == 2 * pairs and not rejected[~real].any() and ((0 <= other) & (other < rows)).all()
+    np.testing.assert_array_equal(lay["offset"].numpy()[real], (r[own] - r[other]).astype(np.float32)[real])
+    for side, a, b in ((False, own, other), (True, other, own)):
+        at = real & (rejected == side)
+        got = np.lexsort((lay["weight"].numpy()[at], b[at], a[at]))
+        want = np.lexsort((w, j, c))
+        np.testing.assert_array_equal(a[at][got], c[want])
+        np.testing.assert_array_equal(b[at][got], j[want])
+        np.testing.assert_array_equal(lay["weight"].numpy()[at][got], w[want])
+    # a row is in the cuts if, and as, its items lie in several runs
+    run = np.arange(n) // (lay["run_tiles"] * O._PAIR_TILE)
+    first, last = run[np.flatnonzero(heads)], run[np.r_[np.flatnonzero(heads)[1:] - 1, n - 1]]
+    cut = np.flatnonzero(first != last)
+    np.testing.assert_array_equal(lay["cuts"].numpy(), np.stack([cut, first[cut], last[cut]], 1))
+    assert lay["n_cuts"] == len(cut) and run[-1] < n_sm * O._RUNS_PER_SM
+
+
+@pytest.mark.parametrize("lengths", [[], [1], [1] * 5000, [128] * 40, [129, 1, 128, 1024, 1025, 3, 8192, 8193, 5, 4096 * 3, 1],
+                                     [7, 13, 127, 2] * 400, [20_000], [895, 1, 1, 128, 900, 128]])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_layout_of_groups(lengths, mixed):
+    rng = np.random.default_rng(len(lengths))
+    ids = np.repeat(np.arange(len(lengths)) * 3, lengths)       # (ids without rows between)
+    if mixed:
+        ids = rng.permutation(ids)
+    lay = O._lay_out_groups(torch.from_numpy(ids.astype(np.int64)))
+    n = len(ids)
+    assert lay["n_groups"] == len(lengths)
+    if n == 0:
+        return
+    rows = np.arange(n) if lay["rows"] is None else lay["rows"].numpy()
+    assert (lay["rows"] is None) == bool((np.diff(ids) >= 0).all())
     off = lay["offsets"].numpy()
-    got = [sorted(rows[a:b]) for a, b in zip(off[:-1], off[1:])]
-    assert got == [np.flatnonzero(np.array(ids) == g).tolist() for g in sorted(set(ids))]
-    assert off[0] == 0 and off[-1] == len(ids)
+    for g, (a, b) in enumerate(zip(off[:-1], off[1:])):
+        assert b - a == lengths[g] and (ids[rows[a:b]] == 3 * g).all()
+    assert off[0] == 0 and off[-1] == n
+    done = np.zeros(n, int)                                     # every place is somebody's, once
+    if lay["n_windows"]:
+        words = lay["window_words"].numpy().view(np.uint32)
+        for k, word in zip(lay["windows"].numpy(), words):
+            bits = (word[:, None] >> np.arange(12, dtype=np.uint32)) & 1
+            head, mine, last = (bits[:, i: i + 4].reshape(-1).astype(bool) for i in (0, 4, 8))
+            place = k * O._STEP + np.arange(O._WINDOW)
+            assert place[mine].max() < n and mine.any()
+            done[place[mine]] += 1
+            np.testing.assert_array_equal(place[head], off[:-1][np.isin(off[:-1], place[mine])])
+            np.testing.assert_array_equal(place[last] + 1, off[1:][np.isin(off[1:] - 1, place[mine])])
+            np.testing.assert_array_equal(word >> 12, np.cumsum(head.reshape(-1, 4).sum(1)) - head.reshape(-1, 4).sum(1))
+            for a, b in zip(np.flatnonzero(head), np.flatnonzero(last)):
+                assert b - a < O._SHORT and mine[a: b + 1].all()
+    listed = lay["listed"].numpy()
+    for i, g in enumerate(listed):
+        low, high = (O._SHORT, O._MEDIUM) if i < lay["n_medium"] else (O._MEDIUM, O._LARGE)
+        assert low < lengths[g] <= high
+        done[off[g]: off[g + 1]] += 1
+    for i, (begin, size, first, count) in enumerate(lay["pieces"].numpy()):
+        assert 0 < size <= O._PIECE and first <= i < first + count
+        assert begin - (i - first) * O._PIECE in off and (i == first + count - 1) == (begin + size in off)
+        done[begin: begin + size] += 1
+    assert (done == 1).all() and lay["n_pieces"] == len(lay["pieces"])
 
 
 @pytest.mark.parametrize("args,kw,error", [
@@ -126,7 +200,7 @@ def test_refused_scores_and_rows():
     dict(smoothing=-0.1), dict(kind="hinge"), dict(kind="squared", smoothing=0.1), dict(reduction="none"),
 ])
 def test_refused_preference_options(kw):
-    pairs = _Stub(2, struct=B.Pairs(2, 0), total_weight=1.0)
+    pairs = _Stub(2, struct=B.Pairs(n_rows=2), total_weight=1.0)
     with pytest.raises(ValueError):
         O._preference_struct(pairs, kw.get("beta", 1.0), kw.get("smoothing", 0.0), kw.get("kind", "logistic"),
                              kw.get("reduction", "sum"))
@@ -134,7 +208,7 @@ def test_refused_preference_options(kw):
 
 def test_refused_means_over_nothing():
     with pytest.raises(ValueError, match="not defined"):
-        O._preference_struct(_Stub(2, struct=B.Pairs(2, 0), total_weight=0.0), 1.0, 0.0, "logistic", "mean")
+        O._preference_struct(_Stub(2, struct=B.Pairs(n_rows=2), total_weight=0.0), 1.0, 0.0, "logistic", "mean")
     with pytest.raises(ValueError, match="not defined"):
         O._choice_struct(_Stub(0, struct=B.Groups(0, 0), n_groups=0), torch.zeros(0), "mean")
 
@@ -158,37 +232,50 @@ def test_library_refuses_bad_descriptors():
             B.check(lib.pb_objective_evaluate(C.byref(o), 1, 0, 1, None, None, None, None, 0, None))
         assert lib.pb_objective_workspace_bytes(C.byref(o)) < 0
 
-    ok = B.Pairs(4, 2, 1, 1, None, None)
+    def pairs(**kw):
+        return B.Pairs(**dict(dict(n_rows=4, n_items=1024, other=16, chunk_rows=16, chunk_heads=16, run_tiles=1), **kw))
+
+    def groups(**kw):
+        return B.Groups(**dict(dict(n_rows=3, n_groups=1, offsets=16, n_medium=1, listed=16), **kw))
+
+    ok, good = pairs(), groups()
     refused(B.Objective(kind=9), "unknown objective")
     refused(B.Objective(kind=0), "pairs are null")
     refused(B.Objective(kind=1), "groups are null")
-    for p, match in ((B.Pairs(-1, 0), "n_rows"), (B.Pairs(1 << 31, 0), "n_rows"), (B.Pairs(4, 1 << 31), "n_items"),
-                     (B.Pairs(4, 2, None, 1), "offsets"), (B.Pairs(4, 2, 1, None), "items"), (B.Pairs(1, 2, 1, 1), "items")):
-        refused(B.Objective(kind=0, pairs=C.pointer(p), beta=1.0), match)
+    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "n_rows"), (dict(n_items=1 << 31), "n_items"),
+                      (dict(n_items=1000), "tiles"), (dict(n_rows=0), "tiles"), (dict(other=None), "null"),
+                      (dict(chunk_rows=None), "null"), (dict(chunk_heads=None), "null"), (dict(run_tiles=0), "null"),
+                      (dict(n_cuts=2, cuts=16), "cuts"), (dict(n_cuts=1), "cuts"), (dict(offset=8), "aligned")):
+        refused(B.Objective(kind=0, pairs=C.pointer(pairs(**kw)), beta=1.0), match)
     for kw, match in ((dict(beta=0.0), "beta"), (dict(beta=1.0, smoothing=0.5), "smoothing"),
                       (dict(beta=1.0, scale=float("nan")), "scale")):
         refused(B.Objective(kind=0, pairs=C.pointer(ok), **kw), match)
-    for g, match in ((B.Groups(-1, 0), "n_rows"), (B.Groups(3, 4, 1), "n_groups"), (B.Groups(3, 0, 1), "without a group"),
-                     (B.Groups(3, 1, None), "offsets")):
-        refused(B.Objective(kind=1, groups=C.pointer(g)), match)
-    good = B.Groups(3, 1, 1)
+    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_groups=4), "n_groups"), (dict(n_groups=0), "without a group"),
+                      (dict(offsets=None), "offsets"), (dict(n_medium=0), "not laid out"), (dict(listed=None), "null"),
+                      (dict(n_windows=1), "null"), (dict(n_pieces=1), "null"), (dict(n_large=-1), "range")):
+        refused(B.Objective(kind=1, groups=C.pointer(groups(**kw))), match)
     refused(B.Objective(kind=1, groups=C.pointer(good)), "target")
-    rows = dict(groups=C.pointer(good), advantage=1, old=1)
-    refused(B.Objective(kind=2, groups=C.pointer(good), advantage=1), "old")
+    rows = dict(groups=C.pointer(good), advantage=16, old=16)
+    refused(B.Objective(kind=2, groups=C.pointer(good), advantage=16), "old")
     for kw, match in ((dict(clip_low=1.5), "clip_low"), (dict(clip_high=-1.0), "clip_high"), (dict(kl_coef=0.1), "reference")):
         refused(B.Objective(kind=2, **rows, **kw), match)
     # scores, types and scratch
     o = B.Objective(kind=0, pairs=C.pointer(ok), beta=1.0, scale=1.0)
-    for scores, typ, grad, loss, match in ((None, 0, 1, None, "null"), (1, 0, None, None, "null"), (1, 7, 1, None, "type"),
-                                           (1, 0, 1, 1, "workspace is null")):
+    for scores, typ, grad, scratch, match in ((None, 0, 16, 16, "null"), (16, 0, None, 16, "null"), (16, 7, 16, 16, "type"),
+                                              (16, 0, 16, None, "workspace is null")):
         with pytest.raises(ValueError, match=match):
-            B.check(lib.pb_objective_evaluate(C.byref(o), scores, typ, grad, loss, None, None, None, 0, None))
+            B.check(lib.pb_objective_evaluate(C.byref(o), scores, typ, grad, 16, None, None, scratch, 1 << 20, None))
     with pytest.raises(RuntimeError, match="bytes given"):
-        B.check(lib.pb_objective_evaluate(C.byref(o), 1, 0, 1, 1, None, None, 8, 8, None))
+        B.check(lib.pb_objective_evaluate(C.byref(o), 16, 0, 16, 16, None, None, 16, 8, None))
     with pytest.raises(ValueError, match="null"):
-        B.check(lib.pb_group_log_probs(C.byref(good), None, 0, 1, None))
+        B.check(lib.pb_group_log_probs(C.byref(good), None, 0, 16, None, 0, None))
     with pytest.raises(ValueError, match="type"):
-        B.check(lib.pb_group_log_probs(C.byref(good), 1, 5, 1, None))
+        B.check(lib.pb_group_log_probs(C.byref(good), 16, 5, 16, None, 0, None))
+    long = groups(n_medium=0, n_pieces=1, pieces=16)
+    with pytest.raises(ValueError, match="workspace"):
+        B.check(lib.pb_group_log_probs(C.byref(long), 16, 0, 16, None, 0, None))
+    with pytest.raises(RuntimeError, match="bytes given"):
+        B.check(lib.pb_group_log_probs(C.byref(long), 16, 0, 16, 16, 8, None))
     with pytest.raises(ValueError):
         B.check(lib.pb_round_begin_objective(C.byref(B.TrainState()), C.byref(o), 0, None, 0, None))
     with pytest.raises(ValueError):
