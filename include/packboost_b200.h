@@ -430,32 +430,30 @@ typedef struct pb_pairs {
     const int32_t* cuts;          /* [n_cuts][3] */
 } pb_pairs;
 
-/* Groups of rows: those that have any, `rows` lists their rows (NULL: the rows in order).  By length:
- * up to PB_SHORT_ROWS rows in windows of PB_WINDOW_ROWS places that start PB_WINDOW_STEP apart, a group
- * belonging to the window k that its first place is in, k * PB_WINDOW_STEP <= place < (k + 1) *
- * PB_WINDOW_STEP, with a word for every four places (bits 0-3: first places of groups of the window, 4-7:
- * places of its groups, 8-11: last ones, from 12: its groups that begin before the four); up to
- * PB_MEDIUM_ROWS and up to PB_LARGE_ROWS rows, by the group's number; longer ones in pieces of up to
- * PB_PIECE_ROWS: first place, places, number of the group's first piece, how many it has. */
-#define PB_SHORT_ROWS 128
-#define PB_WINDOW_ROWS 1024
-#define PB_WINDOW_STEP 896
+/* Groups of rows: those that have any; `rows` lists their rows (NULL: the rows in order), and a group is
+ * its first place in that list and its number of rows.  By length:
+ *  - up to 4 << c rows for c = 0 .. 5, 256 for c = 6: one of 32 >> min(c, 5) groups of a warp.  `teams`
+ *    holds the classes one after the other, each filled up with groups of no rows to whole warps;
+ *  - up to PB_MEDIUM_ROWS, then up to PB_LARGE_ROWS (`medium_rows` and `large_rows` are the longest of
+ *    either): a CTA's, in `held`;
+ *  - longer: pieces of up to PB_PIECE_ROWS: first place, rows, number of the group's first piece, number
+ *    of its pieces. */
 #define PB_MEDIUM_ROWS 1024
 #define PB_LARGE_ROWS 8192
 #define PB_PIECE_ROWS 4096
 typedef struct pb_groups {
     int64_t n_rows;
     int64_t n_groups;
-    const int32_t* offsets;       /* [n_groups + 1] */
     const int32_t* rows;          /* [n_rows], or NULL */
-    int64_t n_windows;
-    const int32_t* windows;       /* [n_windows] k */
-    const uint32_t* window_words; /* [n_windows][PB_WINDOW_ROWS / 4] */
+    int64_t team_warps[7];
+    const int32_t* teams;         /* [sum of team_warps[c] * (32 >> min(c, 5))][2], 8-byte aligned */
     int64_t n_medium;
     int64_t n_large;
-    const int32_t* listed;        /* [n_medium + n_large] */
+    int64_t medium_rows;
+    int64_t large_rows;
+    const int32_t* held;          /* [n_medium + n_large][2], 8-byte aligned */
     int64_t n_pieces;
-    const int32_t* pieces;        /* [n_pieces][4] */
+    const int32_t* pieces;        /* [n_pieces][4], 16-byte aligned */
 } pb_groups;
 
 typedef struct pb_objective {

@@ -87,8 +87,8 @@ class Groups(C.Structure):
     """Mirror of ``pb_groups``."""
 
     _fields_ = [
-        ("n_rows", i64), ("n_groups", i64), ("offsets", vp), ("rows", vp), ("n_windows", i64), ("windows", vp),
-        ("window_words", vp), ("n_medium", i64), ("n_large", i64), ("listed", vp), ("n_pieces", i64), ("pieces", vp),
+        ("n_rows", i64), ("n_groups", i64), ("rows", vp), ("team_warps", i64 * 7), ("teams", vp), ("n_medium", i64),
+        ("n_large", i64), ("medium_rows", i64), ("large_rows", i64), ("held", vp), ("n_pieces", i64), ("pieces", vp),
     ]
 
 

@@ -260,18 +260,19 @@ __global__ void __launch_bounds__(kPairFinishThreads) pair_finish_kernel(PairArg
     if (lane == 0) grad[row] = from_f32<T>((float)t * a.scale);
 }
 
-// A launch that may begin before the one in front of it on the stream has ended, and waits for it itself.
+// A launch; `early`: it may begin before the one in front of it on the stream has ended, and waits for that itself.
 template <typename... P, typename... A>
-cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, cudaStream_t stream, A... args) {
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, bool early, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, (P)args...);
 }
 
@@ -292,7 +293,7 @@ int launch_pairs(const PairArgs& a, double scale, const T* scores, T* grad, floa
     count_launch(1);
     if (!one && (loss || a.p.n_cuts)) {
         const int64_t grid = (a.p.n_cuts + kPairFinishThreads / 32 - 1) / (kPairFinishThreads / 32) + 1;
-        PB_CUDA_TRY(launch_after(pair_finish_kernel<T>, (unsigned)grid, kPairFinishThreads, stream, a, pieces, n_runs, scale,
+        PB_CUDA_TRY(launch_after(pair_finish_kernel<T>, (unsigned)grid, kPairFinishThreads, 0, true, stream, a, pieces, n_runs, scale,
                                  grad, loss));
         count_launch(1);
     }
@@ -300,106 +301,94 @@ int launch_pairs(const PairArgs& a, double scale, const T* scores, T* grad, floa
 }
 
 // ---- groups ---------------------------------------------------------------------------------------
+//
+// A group needs three sums in turn: the largest score and the sum of exponentials, then what its rows add to
+// one another's gradients, then nothing: the gradients.  The sum of exponentials is taken in 64 bits; from its log
+// on, numbers are pairs of floats (value and rounding error), which the 32-bit units add faster than the
+// few 64-bit ones would convert them.
 
 enum GroupOp { kChoice, kPolicy, kLogProbs };
+
+struct Pair32 {  // hi + lo
+    float hi, lo;
+};
+
+// a - b without rounding, plus a small `lo`
+__device__ __forceinline__ Pair32 difference(float a, float b, float lo) {
+    const float t = a - b, v = t - a;
+    const float err = (a - (t - v)) - (b + v);
+    return Pair32{t, fabsf(t) <= 3.402823466e38f ? err + lo : 0.f};  // (nothing to correct at infinity)
+}
+
+__host__ __device__ __forceinline__ Pair32 split(double x) {
+    const float hi = (float)x, lo = (float)(x - (double)hi);
+    return Pair32{hi, lo - lo == 0.f ? lo : 0.f};
+}
+
+__device__ __forceinline__ float exp_of(Pair32 x) {
+    const float e = expf(x.hi);
+    return fmaf(e, x.lo, e);
+}
 
 struct GroupArgs {
     pb_groups g;
     const float *target, *advantage, *old, *reference;
-    double log_high, log_low;  // borders of the log of the ratio
+    Pair32 log_high, log_low;  // borders of the log of the ratio
     float bound_high, bound_low;
-    double kl_coef;
+    float kl_coef;
     float scale;
 };
 
-// exp of a 64-bit value that 32 bits would round by more than exp forgives
-__device__ __forceinline__ float exp_of(double x) {
-    const float hi = (float)x;
-    const float lo = (float)(x - (double)hi);
-    const float e = expf(hi);
-    return isfinite(lo) ? fmaf(e, lo, e) : e;
-}
-
-// A taken row: its term of the loss, and that term's derivative with respect to its log-probability.
-struct Taken {
-    float loss, slope;
-    bool beyond;
-};
-__device__ __forceinline__ Taken taken_row(const GroupArgs& a, double adv_x, float adv) {
-    Taken t;
-    t.beyond = adv > 0.f ? adv_x > a.log_high : adv_x < a.log_low;
-    const float q = t.beyond ? (adv > 0.f ? a.bound_high : a.bound_low) : exp_of(adv_x);
-    t.loss = -adv * q;
-    t.slope = t.beyond ? 0.f : t.loss;
-    return t;
-}
-
-// Sums and divergence of one group, and what its rows get: a slope plus p times a number of the group.
-struct RowTerm {
-    float slope;  // of the row's own term (policy), or minus its target (choice)
-    float p;
-    float gap;    // p (l - reference), times kl_coef in the gradient
-};
-
-// What one row contributes.  `s` is its score, l its log-probability; the row's other inputs are read here.
-template <int OP>
-struct RowSums {
-    double sum = 0.0;   // targets, or slopes of taken rows
-    double kl = 0.0;
-    double loss = 0.0;
-    int clipped = 0;
-};
 struct RowInputs {
-    float target_or_advantage, old, reference;
+    float main, old, reference;  // main: target, or advantage
+};
+
+// What a row has and gives: its gradient is (fixed + p * share) * scale, the share being the group's sum.
+struct RowTerm {
+    float fixed, p;
+    float share;  // what the row adds to the group's
+    float loss, kl;
+    int clipped;
 };
 
 template <int OP>
-__device__ __forceinline__ RowInputs row_inputs(const GroupArgs& a, int r, bool in) {
-    RowInputs v{0.f, 0.f, 0.f};
-    if (in) {
-        v.target_or_advantage = OP == kChoice ? a.target[r] : a.advantage[r];
-        if (OP == kPolicy) v.old = a.old[r];
-        if (OP == kPolicy && a.reference) v.reference = a.reference[r];
-    }
-    return v;
-}
-
-template <int OP>
-__device__ __forceinline__ RowTerm row_term(const GroupArgs& a, float s, double l, const RowInputs& in, RowSums<OP>& sums) {
-    RowTerm t{0.f, 0.f, 0.f};
+__device__ __forceinline__ RowTerm row_term(const GroupArgs& a, float s, Pair32 lse, const RowInputs& in) {
+    RowTerm t{0.f, 0.f, 0.f, 0.f, 0.f, 0};
     const bool live = s != -INFINITY;
+    const Pair32 l = difference(s, lse.hi, -lse.lo);
     if (live) t.p = exp_of(l);
     if (OP == kChoice) {
-        t.slope = -in.target_or_advantage;
-        sums.sum += (double)in.target_or_advantage;
-        if (in.target_or_advantage != 0.f) sums.loss -= (double)in.target_or_advantage * l;
+        t.fixed = -in.main;
+        t.share = in.main;
     } else if (live) {
-        const float adv = in.target_or_advantage;
+        const float adv = in.main;
         if (adv != 0.f) {
-            const Taken k = taken_row(a, l - (double)in.old, adv);
-            t.slope = k.slope;
-            sums.sum += (double)k.slope;
-            sums.loss += (double)k.loss;
-            sums.clipped += k.beyond ? 1 : 0;
+            const Pair32 x = difference(l.hi, in.old, l.lo);
+            const Pair32 edge = adv > 0.f ? a.log_high : a.log_low;
+            const float past = (x.hi - edge.hi) + (x.lo - edge.lo);
+            const bool beyond = adv > 0.f ? past > 0.f : past < 0.f;
+            t.loss = -adv * (beyond ? (adv > 0.f ? a.bound_high : a.bound_low) : exp_of(x));
+            t.fixed = beyond ? 0.f : t.loss;
+            t.clipped = beyond ? 1 : 0;
         }
+        t.share = -t.fixed;
         if (a.reference) {
-            t.gap = t.p * (float)(l - (double)in.reference);
-            sums.kl += (double)t.gap;
+            const Pair32 gap = difference(l.hi, in.reference, l.lo);
+            t.kl = t.p * (gap.hi + gap.lo);
+            t.fixed = fmaf(a.kl_coef, t.kl, t.fixed);
+            t.share = fmaf(-a.kl_coef, t.kl, t.share);
         }
     }
     return t;
 }
 
-// The gradient of a row: with H the sum of the slopes (or T of the targets) and D the divergence,
-// slope + p (k (l - reference - D) - H), or p T - target.
-template <int OP>
-__device__ __forceinline__ float row_gradient(const GroupArgs& a, const RowTerm& t, float share) {
-    const float fixed = OP == kChoice ? t.slope : fmaf((float)a.kl_coef, t.gap, t.slope);
-    return (t.p == 0.f ? fixed : fmaf(t.p, share, fixed)) * a.scale;  // (the share may be infinite)
+__device__ __forceinline__ float row_gradient(const GroupArgs& a, float fixed, float p, float share) {
+    return (p == 0.f ? fixed : fmaf(p, share, fixed)) * a.scale;  // (the share may be infinite)
 }
-template <int OP>
-__device__ __forceinline__ float group_share(const GroupArgs& a, double sum, double kl) {
-    return OP == kChoice ? (float)sum : (float)(-a.kl_coef * kl - sum);
+
+// What the loss of a choice gets from a row, in 64 bits: the terms of a group may be of very different size.
+__device__ __forceinline__ double choice_loss(float s, double lse, float target) {
+    return target != 0.f ? (double)target * (lse - (double)s) : 0.0;
 }
 
 __device__ __forceinline__ double log_sum(float m, double z) {
@@ -409,15 +398,17 @@ __device__ __forceinline__ double log_sum(float m, double z) {
 // exp(s - m), 0 for a masked row
 __device__ __forceinline__ double mass_of(float s, float m) { return s == -INFINITY ? 0.0 : exp((double)s - (double)m); }
 
-// Writes the totals of a CTA, or, where it is the only one, the outputs.
+// Where a CTA puts its totals; the only CTA of an evaluation puts the outputs.
 struct Totals {
-    Part* parts;           // null: not wanted
+    Part* parts;  // null: not wanted
     double scale;
     float *loss, *kl;
     int64_t* clipped;
-    int only;              // this launch's one CTA is all there is
+    int only;
+    float kl_coef;
 };
 __device__ __forceinline__ void put_totals(const Totals& out, int slot, double loss, double kl, double clipped) {
+    loss += (double)out.kl_coef * kl;
     if (out.only) {
         if (out.loss) *out.loss = (float)(loss * out.scale);
         if (out.kl) *out.kl = (float)(kl * out.scale);
@@ -426,199 +417,142 @@ __device__ __forceinline__ void put_totals(const Totals& out, int slot, double l
         out.parts[slot] = Part{loss, kl, clipped};
     }
 }
-__device__ __forceinline__ bool wants_totals(const Totals& out) { return out.only ? (out.loss || out.kl || out.clipped) : out.parts != nullptr; }
+// (all threads of the CTA)
+template <int OP>
+__device__ __forceinline__ void put_cta_totals(const Totals& out, int slot, double loss, double kl, int clipped, double* scratch) {
+    if (!out.parts && !out.only) return;
+    loss = block_sum(loss, scratch);
+    if (OP == kPolicy) {
+        kl = block_sum(kl, scratch);
+        const double c = block_sum((double)clipped, scratch);
+        if (threadIdx.x == 0) put_totals(out, slot, loss, kl, c);
+    } else if (threadIdx.x == 0) {
+        put_totals(out, slot, loss, 0.0, 0.0);
+    }
+}
 
-// ---- short groups: a window of rows per CTA ----
+template <int OP>
+__device__ __forceinline__ RowInputs row_inputs(const GroupArgs& a, int r) {
+    RowInputs v;
+    v.main = OP == kChoice ? a.target[r] : a.advantage[r];
+    v.old = OP == kPolicy ? a.old[r] : 0.f;
+    v.reference = OP == kPolicy && a.reference ? a.reference[r] : 0.f;
+    return v;
+}
+
+// The kernels of one evaluation write different rows, so the next may start while one runs (its CTAs fill SMs that the
+// last of this one's leave idle); each waits for the one before it at its end, so that the last one's end is
+// everyone's.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---- short groups: lanes of a warp ----
 //
-// A window is 1024 neighbouring places; every short group belongs to the window its first row is in, and
-// windows start 896 apart so that it ends there too.  A thread has four places; sums over groups are
-// segmented scans over the CTA's threads, so groups of one row and groups of 128 cost the same per row.
-constexpr int kWindowThreads = 256;
-static_assert(kWindowThreads * 4 == PB_WINDOW_ROWS, "layout of the windows");
+// 1, 2, 4 ... 32 neighbouring lanes have a group, ROWS rows each; a warp's groups are of one class (so many lanes), and
+// sums over a group are shuffles within its lanes.  Of up to 4 x lanes rows at least half are there; one launch
+// takes all classes.
+constexpr int kTeamThreads = 256;
 
-// Bits of a thread's word: first rows of groups 0-3, rows of this window 4-7, last rows 8-11, groups begun before the thread 12-.
-__device__ __forceinline__ bool word_head(uint32_t w, int u) { return (w >> u) & 1u; }
-__device__ __forceinline__ bool word_in(uint32_t w, int u) { return (w >> (4 + u)) & 1u; }
-__device__ __forceinline__ bool word_last(uint32_t w, int u) { return (w >> (8 + u)) & 1u; }
-__device__ __forceinline__ int word_group(uint32_t w, int u) { return (int)(w >> 12) + __popc(w & ((2u << u) - 1u)) - 1; }
-
-struct AddOp {
-    template <typename V> __device__ static V apply(V x, V y) { return x + y; }
-};
-struct MaxOp {
-    __device__ static float apply(float x, float y) { return fmaxf(x, y); }
-};
-
-// Totals of the groups of a window, by group, in `total`.  A group of at most 128 rows is open in one warp
-// before the one that ends it at most, since a warp has 128 places.
-template <typename V, typename Op>
-__device__ __forceinline__ void window_totals(const V x[4], uint32_t word, uint32_t mask, V none, V* warp_open, V* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    V v = none;
+template <typename T, int OP, int ROWS>
+__global__ void __launch_bounds__(kTeamThreads) team_kernel(GroupArgs a, const int2* __restrict__ teams, const int first_class,
+                                                            int64_t n_warps, int slot0, const T* __restrict__ scores,
+                                                            T* __restrict__ out, Totals totals) {
+    __shared__ double scratch[kTeamThreads / 32];
+    let_next_start();
+    const int lane = threadIdx.x & 31;
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0;
+    for (int64_t w = ((int64_t)blockIdx.x * kTeamThreads + threadIdx.x) >> 5; w < n_warps; w += (int64_t)gridDim.x * (kTeamThreads / 32)) {
+        // the class of this warp, and its first team
+        int c = first_class;
+        int64_t left = w, team = 0;
+        while (left >= a.g.team_warps[c]) {
+            left -= a.g.team_warps[c];
+            team += a.g.team_warps[c] * (32 >> min(c, 5));
+            ++c;
+        }
+        c = min(c, 5);
+        const int lanes = 1 << c, me = lane & (lanes - 1);
+        const int2 group = teams[team + left * (32 >> c) + (lane >> c)];
+        int r[ROWS];
+        float s[ROWS];
+        RowInputs in[ROWS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v = word_head(word, u) ? x[u] : Op::apply(v, x[u]);
-    const uint32_t below = mask & (0xFFFFFFFFu >> (31 - lane));
-    const int reach = below ? lane - (31 - __clz(below)) : lane;
-    for (int d = 1; d < 32; d <<= 1) {
-        const V o = __shfl_up_sync(0xFFFFFFFFu, v, d);
-        if (d <= reach) v = Op::apply(o, v);
-    }
-    if (lane == 31) warp_open[warp] = v;
-    V open = __shfl_up_sync(0xFFFFFFFFu, v, 1);
-    if (lane == 0) open = none;
-    __syncthreads();
-    if (!(mask & ((1u << lane) - 1u)) && warp > 0) open = Op::apply(warp_open[warp - 1], open);
-    v = open;
+        for (int u = 0; u < ROWS; ++u) {
+            const int i = u * lanes + me;
+            r[u] = i < group.y ? group.x + i : -1;
+            if (a.g.rows && r[u] >= 0) r[u] = a.g.rows[r[u]];
+        }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        v = word_head(word, u) ? x[u] : Op::apply(v, x[u]);
-        if (word_last(word, u)) total[word_group(word, u)] = v;
-    }
-    __syncthreads();
-}
-
-// Four neighbouring places of an array, or of the rows that an index lists.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, const int r[4], bool straight, uint32_t word, T v[4]) {
-    if (straight) {
-        if (sizeof(T) == 4)
-            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p + r[0]);
-        else
-            *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(p + r[0]);
-    } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (word_in(word, u)) v[u] = p[r[u]];
-    }
-}
-
-template <typename T, int OP>
-__global__ void __launch_bounds__(kWindowThreads) window_kernel(GroupArgs a, int vectors, const T* __restrict__ scores,
-                                                                T* __restrict__ out, Totals totals) {
-    __shared__ double s_z[PB_WINDOW_ROWS], s_open[3][kWindowThreads / 32];
-    __shared__ float s_m[PB_WINDOW_ROWS], s_open_m[kWindowThreads / 32];
-    __shared__ double s_kl[OP == kPolicy ? PB_WINDOW_ROWS : 1];
-    __shared__ double scratch[kWindowThreads / 32];
-    asm volatile("griddepcontrol.launch_dependents;");
-    const int64_t i0 = (int64_t)a.g.windows[blockIdx.x] * PB_WINDOW_STEP + threadIdx.x * 4;
-    const uint32_t word = a.g.window_words[(int64_t)blockIdx.x * kWindowThreads + threadIdx.x];
-    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, (word & 15u) != 0u);
-    int r[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = (int)(i0 + u);
-    if (a.g.rows) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (word_in(word, u)) r[u] = a.g.rows[i0 + u];
-    }
-    const bool straight = vectors && i0 + 3 < a.g.n_rows && (word & 0xF0u);
-    T raw[4];
-    RowInputs in[4];
-    load4(scores, r, straight, word, raw);
-    if (OP != kLogProbs) {
-        float v[4];
-        load4(OP == kChoice ? a.target : a.advantage, r, straight, word, v);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) in[u].target_or_advantage = v[u];
-        if (OP == kPolicy) {
-            load4(a.old, r, straight, word, v);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) in[u].old = v[u];
-            if (a.reference) {
-                load4(a.reference, r, straight, word, v);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) in[u].reference = v[u];
+        for (int u = 0; u < ROWS; ++u) {
+            s[u] = -INFINITY;
+            in[u] = RowInputs{0.f, 0.f, 0.f};
+            if (r[u] >= 0) {
+                s[u] = to_f32(scores[r[u]]);
+                if (OP != kLogProbs) in[u] = row_inputs<OP>(a, r[u]);
             }
         }
-    }
-    float s[4];
+        float m = s[0];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) s[u] = word_in(word, u) ? to_f32(raw[u]) : -INFINITY;
-    window_totals<float, MaxOp>(s, word, mask, -INFINITY, s_open_m, s_m);
-    double e[4];
+        for (int u = 1; u < ROWS; ++u) m = fmaxf(m, s[u]);
+        for (int d = lanes >> 1; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+        double z = 0.0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) e[u] = word_in(word, u) ? mass_of(s[u], s_m[word_group(word, u)]) : 0.0;
-    window_totals<double, AddOp>(e, word, mask, 0.0, s_open[0], s_z);
-    // (the log of each group's sum once, by the thread of its last row)
+        for (int u = 0; u < ROWS; ++u) z += mass_of(s[u], m);
+        for (int d = lanes >> 1; d > 0; d >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, d);
+        const double lse64 = log_sum(m, z);
+        const Pair32 lse = split(lse64);
+        if (OP == kLogProbs) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (word_last(word, u)) {
-            const int k = word_group(word, u);
-            s_z[k] = log_sum(s_m[k], s_z[k]);
+            for (int u = 0; u < ROWS; ++u)
+                if (r[u] >= 0) {
+                    const Pair32 l = difference(s[u], lse.hi, -lse.lo);
+                    out[r[u]] = from_f32<T>(l.hi + l.lo);
+                }
+            continue;
         }
-    __syncthreads();
-    double l[4];
+        float fixed[ROWS], part = 0.f, part_loss = 0.f, part_kl = 0.f;
+        double part64 = 0.0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) l[u] = word_in(word, u) ? (double)s[u] - s_z[word_group(word, u)] : 0.0;
-    float g[4];
-    if (OP == kLogProbs) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) g[u] = (float)l[u];
-    } else {
-        RowSums<OP> all;
-        RowTerm t[4];
-        double sum[4], kl[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            RowSums<OP> one;
-            t[u] = RowTerm{0.f, 0.f, 0.f};
-            if (word_in(word, u)) t[u] = row_term<OP>(a, s[u], l[u], in[u], one);
-            sum[u] = one.sum;
-            kl[u] = one.kl;
-            all.loss += one.loss;
-            all.kl += one.kl;
-            all.clipped += one.clipped;
-        }
-        window_totals<double, AddOp>(sum, word, mask, 0.0, s_open[1], s_z);
-        if (OP == kPolicy && a.reference) window_totals<double, AddOp>(kl, word, mask, 0.0, s_open[2], s_kl);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            g[u] = 0.f;
-            if (word_in(word, u)) {
-                const int k = word_group(word, u);
-                g[u] = row_gradient<OP>(a, t[u], group_share<OP>(a, s_z[k], OP == kPolicy && a.reference ? s_kl[k] : 0.0));
+        for (int u = 0; u < ROWS; ++u) {
+            if (r[u] >= 0) {
+                if (OP == kChoice) loss += choice_loss(s[u], lse64, in[u].main);
+                const RowTerm t = row_term<OP>(a, s[u], lse, in[u]);
+                s[u] = t.p;
+                fixed[u] = t.fixed;
+                part += t.share;
+                part_loss += t.loss;
+                part_kl += t.kl;
+                clipped += t.clipped;
+            }
+            if ((u & 3) == 3) {  // (four terms in 32 bits, the sums of fours in 64)
+                part64 += (double)part;
+                if (OP == kPolicy) {
+                    loss += (double)part_loss;
+                    kl += (double)part_kl;
+                }
+                part = part_loss = part_kl = 0.f;
             }
         }
-        if (wants_totals(totals)) {
-            const double loss = block_sum(all.loss, scratch);
-            double kl_all = 0.0, clipped = 0.0;
-            if (OP == kPolicy) {
-                kl_all = block_sum(all.kl, scratch);
-                clipped = block_sum((double)all.clipped, scratch);
-            }
-            if (threadIdx.x == 0) put_totals(totals, blockIdx.x, loss + a.kl_coef * kl_all, kl_all, clipped);
-        }
-    }
-    if (straight && (word & 0xF0u) == 0xF0u) {
-        T v[4] = {from_f32<T>(g[0]), from_f32<T>(g[1]), from_f32<T>(g[2]), from_f32<T>(g[3])};
-        if (sizeof(T) == 4)
-            *reinterpret_cast<uint4*>(out + r[0]) = *reinterpret_cast<const uint4*>(v);
-        else
-            *reinterpret_cast<uint2*>(out + r[0]) = *reinterpret_cast<const uint2*>(v);
-    } else {
+        for (int d = lanes >> 1; d > 0; d >>= 1) part64 += __shfl_xor_sync(0xFFFFFFFFu, part64, d);
+        const float share = (float)part64;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (word_in(word, u)) out[r[u]] = from_f32<T>(g[u]);
+        for (int u = 0; u < ROWS; ++u)
+            if (r[u] >= 0) out[r[u]] = from_f32<T>(row_gradient(a, fixed[u], s[u], share));
     }
+    if (OP != kLogProbs) put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
+    wait_for_previous();
 }
 
 // ---- groups that a CTA holds ----
 //
-// A group of up to THREADS x ROWS rows stays in the registers of one CTA: its scores are read once, and of the
-// rest of a row two numbers are kept between the sums and the gradient.
-template <int THREADS>
-__device__ __forceinline__ double cta_sum(double v, double* scratch) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double t = 0.0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) t += scratch[w];
-    return t;
+// The rows of a group stay in the shared memory of one CTA, each thread using the words it filled itself: the
+// inputs that the gradient needs are on their way there (cp.async) while the scores are summed.
+__device__ __forceinline__ void copy_word(float* to, const float* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from));
 }
 
-// Largest score and the log of the sum of exponentials over the CTA's threads, from the threads' own ones.
+// Largest score and log of the sum of exponentials over the CTA, from the threads' own ones.
 template <int THREADS>
 __device__ __forceinline__ double cta_log_sum(float m, double z, float* s_m, double* s_z) {
     float wm = warp_max(m);
@@ -638,70 +572,113 @@ __device__ __forceinline__ double cta_log_sum(float m, double z, float* s_m, dou
     return log_sum(all, warp_sum(z));
 }
 
-template <typename T, int OP, int THREADS, int ROWS>
-__global__ void __launch_bounds__(THREADS) held_kernel(GroupArgs a, const int32_t* __restrict__ list, int slot0,
+template <int THREADS>
+__device__ __forceinline__ double cta_sum(double v, double* scratch) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    const int k = threadIdx.x & 31;
+    return warp_sum(k < THREADS / 32 ? scratch[k] : 0.0);
+}
+
+template <typename T, int OP, int THREADS>
+__global__ void __launch_bounds__(THREADS) held_kernel(GroupArgs a, const int2* __restrict__ list, int most, int slot0,
                                                        const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
+    extern __shared__ float held[];  // scores (then p) | main (then fixed) | old | reference, `most` each
     __shared__ float s_m[THREADS / 32];
     __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
-    asm volatile("griddepcontrol.launch_dependents;");
-    const int group = list[blockIdx.x];
-    const int begin = a.g.offsets[group], n = a.g.offsets[group + 1] - begin;
+    let_next_start();
+    const int2 group = list[blockIdx.x];
+    const int begin = group.x, n = group.y;
+    float* const h_main = held + most;
+    float* const h_old = held + 2 * most;
+    float* const h_ref = held + 3 * most;
     auto row_of = [&](int i) { return a.g.rows ? a.g.rows[begin + i] : begin + i; };
-    float s[ROWS];
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        const int i = u * THREADS + threadIdx.x;
-        s[u] = i < n ? to_f32(scores[row_of(i)]) : -INFINITY;
-    }
-    float m = s[0];
-#pragma unroll
-    for (int u = 1; u < ROWS; ++u) m = fmaxf(m, s[u]);
-    double z = 0.0;
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u)
-        if (u * THREADS < n) z += mass_of(s[u], m);
-    const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
-    if (OP == kLogProbs) {
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            const int i = u * THREADS + threadIdx.x;
-            if (i < n) out[row_of(i)] = from_f32<T>((float)((double)s[u] - lse));
+    if (OP != kLogProbs) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const int r = row_of(i);
+            copy_word(h_main + i, (OP == kChoice ? a.target : a.advantage) + r);
+            if (OP == kPolicy) {
+                copy_word(h_old + i, a.old + r);
+                if (a.reference) copy_word(h_ref + i, a.reference + r);
+            }
         }
+        asm volatile("cp.async.commit_group;");
+    }
+    float m = -INFINITY;
+    {
+        constexpr int kAhead = 8;
+        for (int i0 = threadIdx.x; i0 < n; i0 += THREADS * kAhead) {
+            float v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * THREADS;
+                v[u] = i < n ? to_f32(scores[row_of(i)]) : -INFINITY;
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * THREADS;
+                m = fmaxf(m, v[u]);
+                if (i < n) held[i] = v[u];
+            }
+        }
+    }
+    double z = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += THREADS) z += mass_of(held[i], m);
+    const double lse64 = cta_log_sum<THREADS>(m, z, s_m, s_z);
+    const Pair32 lse = split(lse64);
+    if (OP == kLogProbs) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+            const Pair32 l = difference(held[i], lse.hi, -lse.lo);
+            out[row_of(i)] = from_f32<T>(l.hi + l.lo);
+        }
+        wait_for_previous();
         return;
     }
-    RowSums<OP> sums;
-    float fixed[ROWS];  // what does not hang on the group; s becomes p
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    double part = 0.0, loss = 0.0, kl = 0.0;
+    int clipped = 0;
+    for (int i0 = threadIdx.x; i0 < n; i0 += THREADS * 4) {
+        float p4 = 0.f, l4 = 0.f, k4 = 0.f;
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        const int i = u * THREADS + threadIdx.x;
-        if (i < n) {
-            const RowInputs in = row_inputs<OP>(a, row_of(i), true);
-            const RowTerm t = row_term<OP>(a, s[u], (double)s[u] - lse, in, sums);
-            s[u] = t.p;
-            fixed[u] = OP == kChoice ? t.slope : fmaf((float)a.kl_coef, t.gap, t.slope);
+        for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * THREADS;
+            if (i < n) {
+                const float s = held[i];
+                const RowInputs in{h_main[i], OP == kPolicy ? h_old[i] : 0.f, OP == kPolicy && a.reference ? h_ref[i] : 0.f};
+                if (OP == kChoice) loss += choice_loss(s, lse64, in.main);
+                const RowTerm t = row_term<OP>(a, s, lse, in);
+                held[i] = t.p;
+                h_main[i] = t.fixed;
+                p4 += t.share;
+                l4 += t.loss;
+                k4 += t.kl;
+                clipped += t.clipped;
+            }
+        }
+        part += (double)p4;
+        if (OP == kPolicy) {
+            loss += (double)l4;
+            kl += (double)k4;
         }
     }
-    const double sum = cta_sum<THREADS>(sums.sum, scratch);
-    const double kl = OP == kPolicy && a.reference ? cta_sum<THREADS>(sums.kl, scratch) : 0.0;
-    const float share = group_share<OP>(a, sum, kl);
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        const int i = u * THREADS + threadIdx.x;
-        if (i < n) out[row_of(i)] = from_f32<T>((s[u] == 0.f ? fixed[u] : fmaf(s[u], share, fixed[u])) * a.scale);
-    }
-    if (wants_totals(totals)) {
-        const double loss = cta_sum<THREADS>(sums.loss, scratch);
-        const double clipped = OP == kPolicy ? cta_sum<THREADS>((double)sums.clipped, scratch) : 0.0;
-        if (threadIdx.x == 0) put_totals(totals, slot0 + blockIdx.x, loss + a.kl_coef * kl, kl, clipped);
-    }
+    const float share = (float)cta_sum<THREADS>(part, scratch);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += THREADS) out[row_of(i)] = from_f32<T>(row_gradient(a, h_main[i], held[i], share));
+    put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
+    wait_for_previous();
 }
 
 // ---- long groups: many CTAs each ----
 //
 // Pieces of PB_PIECE_ROWS rows; the sums of a group's pieces go through memory from one launch to the next: sums of
-// exponentials, then slopes and divergence, then the gradient.  The rows are read again each time, from L2 mostly.
+// exponentials, then shares, then the gradient.  The rows are read again each time, from L2 mostly.
 struct PieceSums {
-    double z, sum, kl;
+    double z, share;
     float m, unused;
 };
 constexpr int kPieceThreads = 512;
@@ -714,14 +691,26 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     constexpr int THREADS = kPieceThreads, ROWS = kPieceRows;
     __shared__ float s_m[THREADS / 32];
     __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
-    const int begin = a.g.pieces[4 * blockIdx.x], n = a.g.pieces[4 * blockIdx.x + 1];
-    const int first = a.g.pieces[4 * blockIdx.x + 2], count = a.g.pieces[4 * blockIdx.x + 3];  // of the group's pieces
-    auto row_of = [&](int i) { return a.g.rows ? a.g.rows[begin + i] : begin + i; };
+    let_next_start();
+    if (STEP == kPieceMass) wait_for_previous();
+    const int4 piece = reinterpret_cast<const int4*>(a.g.pieces)[blockIdx.x];
+    const int begin = piece.x, n = piece.y, first = piece.z, count = piece.w;  // (first, count: the group's pieces)
+    int r[ROWS];
     float s[ROWS];
+    RowInputs in[ROWS];
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
         const int i = u * THREADS + threadIdx.x;
-        s[u] = i < n ? to_f32(scores[row_of(i)]) : -INFINITY;
+        r[u] = i < n ? begin + i : -1;
+        if (a.g.rows && r[u] >= 0) r[u] = a.g.rows[r[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+        s[u] = -INFINITY;
+        if (r[u] >= 0) {
+            s[u] = to_f32(scores[r[u]]);
+            if (OP != kLogProbs && STEP != kPieceMass) in[u] = row_inputs<OP>(a, r[u]);
+        }
     }
     float m = -INFINITY;
     double z = 0.0;
@@ -730,71 +719,78 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
         for (int u = 0; u < ROWS; ++u) m = fmaxf(m, s[u]);
 #pragma unroll
         for (int u = 0; u < ROWS; ++u) z += mass_of(s[u], m);
-        float wm = warp_max(m);
+        const float wm = warp_max(m);
         z = warp_sum(z == 0.0 ? 0.0 : z * exp((double)m - (double)wm));
         if ((threadIdx.x & 31) == 0) {
             s_m[threadIdx.x >> 5] = wm;
             s_z[threadIdx.x >> 5] = z;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 0; w < THREADS / 32; ++w) wm = fmaxf(wm, s_m[w]);
-            z = 0.0;
-            for (int w = 0; w < THREADS / 32; ++w)
-                if (s_z[w] != 0.0) z += s_z[w] * exp((double)s_m[w] - (double)wm);
-            pieces[blockIdx.x].m = wm;
-            pieces[blockIdx.x].z = z;
+        if (threadIdx.x < 32) {
+            const float k = threadIdx.x < THREADS / 32 ? s_m[threadIdx.x] : -INFINITY;
+            z = threadIdx.x < THREADS / 32 ? s_z[threadIdx.x] : 0.0;
+            m = warp_max(k);
+            z = warp_sum(z == 0.0 ? 0.0 : z * exp((double)k - (double)m));
+            if (threadIdx.x == 0) {
+                pieces[blockIdx.x].m = m;
+                pieces[blockIdx.x].z = z;
+            }
         }
         return;
     }
-    // the group's log of the sum, from all its pieces
+    wait_for_previous();   // (the rows' inputs do not come from the launch before, the sums do)
     for (int k = threadIdx.x; k < count; k += THREADS) m = fmaxf(m, pieces[first + k].m);
     for (int k = threadIdx.x; k < count; k += THREADS) {
         const double zk = pieces[first + k].z;
         if (zk != 0.0) z += zk * exp((double)pieces[first + k].m - (double)m);
     }
-    const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
+    const double lse64 = cta_log_sum<THREADS>(m, z, s_m, s_z);
+    const Pair32 lse = split(lse64);
     if (OP == kLogProbs) {
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            const int i = u * THREADS + threadIdx.x;
-            if (i < n) out[row_of(i)] = from_f32<T>((float)((double)s[u] - lse));
-        }
+        for (int u = 0; u < ROWS; ++u)
+            if (r[u] >= 0) {
+                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
+                out[r[u]] = from_f32<T>(l.hi + l.lo);
+            }
         return;
     }
-    double sum = 0.0, kl = 0.0;
+    float share = 0.f;
     if (STEP == kPieceOut) {
-        for (int k = threadIdx.x; k < count; k += THREADS) {
-            sum += pieces[first + k].sum;
-            kl += pieces[first + k].kl;
-        }
-        sum = cta_sum<THREADS>(sum, scratch);
-        kl = OP == kPolicy && a.reference ? cta_sum<THREADS>(kl, scratch) : 0.0;
+        double sum = 0.0;
+        for (int k = threadIdx.x; k < count; k += THREADS) sum += pieces[first + k].share;
+        share = (float)cta_sum<THREADS>(sum, scratch);
     }
-    const float share = group_share<OP>(a, sum, kl);
-    RowSums<OP> sums;
+    double part = 0.0, loss = 0.0, kl = 0.0;
+    int clipped = 0;
+    float p4 = 0.f, l4 = 0.f, k4 = 0.f;
 #pragma unroll
     for (int u = 0; u < ROWS; ++u) {
-        const int i = u * THREADS + threadIdx.x;
-        if (i < n) {
-            const int r = row_of(i);
-            const RowInputs in = row_inputs<OP>(a, r, true);
-            const RowTerm t = row_term<OP>(a, s[u], (double)s[u] - lse, in, sums);
-            if (STEP == kPieceOut) out[r] = from_f32<T>(row_gradient<OP>(a, t, share));
+        if (r[u] >= 0) {
+            const RowTerm t = row_term<OP>(a, s[u], lse, in[u]);
+            if (STEP == kPieceOut) {
+                out[r[u]] = from_f32<T>(row_gradient(a, t.fixed, t.p, share));
+            } else {
+                if (OP == kChoice) loss += choice_loss(s[u], lse64, in[u].main);
+                p4 += t.share;
+                l4 += t.loss;
+                k4 += t.kl;
+                clipped += t.clipped;
+            }
+        }
+        if (STEP == kPieceTerms && (u & 3) == 3) {
+            part += (double)p4;
+            if (OP == kPolicy) {
+                loss += (double)l4;
+                kl += (double)k4;
+            }
+            p4 = l4 = k4 = 0.f;
         }
     }
     if (STEP == kPieceTerms) {
-        sum = cta_sum<THREADS>(sums.sum, scratch);
-        kl = OP == kPolicy ? cta_sum<THREADS>(sums.kl, scratch) : 0.0;
-        if (threadIdx.x == 0) {
-            pieces[blockIdx.x].sum = sum;
-            pieces[blockIdx.x].kl = kl;
-        }
-        if (wants_totals(totals)) {
-            const double loss = cta_sum<THREADS>(sums.loss, scratch);
-            const double clipped = OP == kPolicy ? cta_sum<THREADS>((double)sums.clipped, scratch) : 0.0;
-            if (threadIdx.x == 0) put_totals(totals, slot0 + blockIdx.x, loss + a.kl_coef * kl, kl, clipped);
-        }
+        part = cta_sum<THREADS>(part, scratch);
+        if (threadIdx.x == 0) pieces[blockIdx.x].share = part;
+        put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
     }
 }
 
@@ -805,15 +801,21 @@ int check_groups(const pb_groups* g) {
     PB_REQUIRE(g->n_rows >= 0 && g->n_rows < (1ll << 31) - 1, "n_rows=%lld out of range", (long long)g->n_rows);
     PB_REQUIRE(g->n_groups >= 0 && g->n_groups <= g->n_rows, "n_groups=%lld out of range", (long long)g->n_groups);
     PB_REQUIRE((g->n_groups == 0) == (g->n_rows == 0), "rows without a group");
-    PB_REQUIRE(g->n_groups == 0 || g->offsets, "offsets of the groups are null");
     const int64_t most = (1ll << 31) - 1;
-    PB_REQUIRE(g->n_windows >= 0 && g->n_medium >= 0 && g->n_large >= 0 && g->n_pieces >= 0 && g->n_windows < most &&
-                   g->n_pieces < most && g->n_medium + g->n_large <= g->n_groups,
+    int64_t warps = 0;
+    for (int c = 0; c < 7; ++c) {
+        PB_REQUIRE(g->team_warps[c] >= 0 && g->team_warps[c] < most, "team_warps[%d] is out of range", c);
+        warps += g->team_warps[c];
+    }
+    PB_REQUIRE(g->n_medium >= 0 && g->n_large >= 0 && g->n_medium + g->n_large <= g->n_groups && g->n_pieces >= 0 && g->n_pieces < most,
                "counts of the groups' layout are out of range");
-    PB_REQUIRE((g->n_windows == 0 || (g->windows && g->window_words)) && (g->n_medium + g->n_large == 0 || g->listed) &&
-                   (g->n_pieces == 0 || g->pieces),
+    PB_REQUIRE(g->n_medium == 0 || (g->medium_rows > 0 && g->medium_rows <= PB_MEDIUM_ROWS), "medium_rows is out of range");
+    PB_REQUIRE(g->n_large == 0 || (g->large_rows > 0 && g->large_rows <= PB_LARGE_ROWS), "large_rows is out of range");
+    PB_REQUIRE((warps == 0 || g->teams) && (g->n_medium + g->n_large == 0 || g->held) && (g->n_pieces == 0 || g->pieces),
                "a table of the groups' layout is null");
-    PB_REQUIRE(g->n_groups == 0 || g->n_windows + g->n_medium + g->n_large + g->n_pieces > 0, "the groups are not laid out");
+    PB_REQUIRE((uintptr_t)g->teams % 8 == 0 && (uintptr_t)g->held % 8 == 0 && (uintptr_t)g->pieces % 16 == 0,
+               "tables of the groups' layout must be aligned");
+    PB_REQUIRE(g->n_groups == 0 || warps + g->n_medium + g->n_large + g->n_pieces > 0, "the groups are not laid out");
     return PB_OK;
 }
 
@@ -853,12 +855,26 @@ int64_t n_rows_of(const pb_objective* o) {
     return o->kind == PB_OBJECTIVE_PREFERENCE ? o->pairs->n_rows : o->groups->n_rows;
 }
 
-int64_t n_group_parts(const pb_groups* g) { return g->n_windows + g->n_medium + g->n_large + g->n_pieces; }
+// CTAs of the launch that takes all warps of short groups: what the SMs hold at once, or as many as there are warps.
+constexpr int64_t kTeamGrid = 148 * 6;
+int64_t team_grid(int64_t warps) { return warps == 0 ? 0 : warps / 8 + 1 < kTeamGrid ? (warps + 7) / 8 : kTeamGrid; }
+int64_t team_warps(const pb_groups* g, int from, int to) {
+    int64_t n = 0;
+    for (int c = from; c < to; ++c) n += g->team_warps[c];
+    return n;
+}
+
+int64_t n_group_parts(const pb_groups* g) {
+    return team_grid(team_warps(g, 0, 6)) + team_grid(g->team_warps[6]) + g->n_medium + g->n_large + g->n_pieces;
+}
 
 // Scratch: what the CTAs leave of the totals, then the sums of pieces.
+int64_t group_scratch_bytes(const pb_groups* g) {
+    return n_group_parts(g) * (int64_t)sizeof(Part) + g->n_pieces * (int64_t)sizeof(PieceSums);
+}
 int64_t scratch_bytes(const pb_objective* o) {
     if (o->kind == PB_OBJECTIVE_PREFERENCE) return 3 * n_runs_of(o->pairs) * (int64_t)sizeof(double);
-    return n_group_parts(o->groups) * (int64_t)sizeof(Part) + o->groups->n_pieces * (int64_t)sizeof(PieceSums);
+    return group_scratch_bytes(o->groups);
 }
 
 template <typename T, int OP>
@@ -869,38 +885,50 @@ int launch_groups(const GroupArgs& a, double scale, const void* scores_, void* o
     const pb_groups& g = a.g;
     const int64_t n_parts = n_group_parts(&g);
     const bool want = loss || kl || clipped;
-    Totals totals{want ? static_cast<Part*>(scratch) : nullptr, scale, loss, kl, clipped, n_parts == 1};
-    if (g.n_windows) {
-        const uintptr_t bits = (uintptr_t)scores | (uintptr_t)out | (uintptr_t)a.target | (uintptr_t)a.advantage | (uintptr_t)a.old | (uintptr_t)a.reference;
-        const int vectors = !g.rows && bits % 16 == 0;
-        window_kernel<T, OP><<<(unsigned)g.n_windows, kWindowThreads, 0, stream>>>(a, vectors, scores, out, totals);
-        count_launch(1);
+    const Totals totals{want ? static_cast<Part*>(scratch) : nullptr, scale, loss, kl, clipped, n_parts == 1, a.kl_coef};
+    const int2* teams = reinterpret_cast<const int2*>(g.teams);
+    int slot = 0, launches = 0;
+    // the first launch waits for what is before it on the stream, the others may overlap with the ones before
+    auto launch = [&](auto kernel, int64_t grid, int block, size_t smem, auto... args) -> int {
+        PB_TRY(allow_shared(kernel, smem));
+        PB_CUDA_TRY(launch_after(kernel, (unsigned)grid, (unsigned)block, smem, launches > 0, stream, args...));
+        ++launches;
+        return PB_OK;
+    };
+    const int64_t small = team_warps(&g, 0, 6);
+    if (small) {
+        PB_TRY(launch(team_kernel<T, OP, 4>, team_grid(small), kTeamThreads, 0, a, teams, 0, small, slot, scores, out, totals));
+        slot += (int)team_grid(small);
     }
+    if (g.team_warps[6]) {
+        int64_t before = 0;
+        for (int c = 0; c < 6; ++c) before += g.team_warps[c] * (32 >> c);
+        PB_TRY(launch(team_kernel<T, OP, 8>, team_grid(g.team_warps[6]), kTeamThreads, 0, a, teams + before, 6, g.team_warps[6], slot,
+                      scores, out, totals));
+        slot += (int)team_grid(g.team_warps[6]);
+    }
+    const int arrays = OP == kLogProbs ? 1 : OP == kChoice ? 2 : a.reference ? 4 : 3;
+    const int2* held = reinterpret_cast<const int2*>(g.held);
     if (g.n_medium) {
-        held_kernel<T, OP, 128, PB_MEDIUM_ROWS / 128><<<(unsigned)g.n_medium, 128, 0, stream>>>(
-            a, g.listed, (int)g.n_windows, scores, out, totals);
-        count_launch(1);
+        PB_TRY(launch(held_kernel<T, OP, 128>, g.n_medium, 128, (size_t)(g.medium_rows * arrays * 4), a, held, (int)g.medium_rows, slot,
+                      scores, out, totals));
+        slot += (int)g.n_medium;
     }
     if (g.n_large) {
-        held_kernel<T, OP, 512, PB_LARGE_ROWS / 512><<<(unsigned)g.n_large, 512, 0, stream>>>(
-            a, g.listed + g.n_medium, (int)(g.n_windows + g.n_medium), scores, out, totals);
-        count_launch(1);
+        PB_TRY(launch(held_kernel<T, OP, 512>, g.n_large, 512, (size_t)(g.large_rows * arrays * 4), a, held + g.n_medium,
+                      (int)g.large_rows, slot, scores, out, totals));
+        slot += (int)g.n_large;
     }
     if (g.n_pieces) {
         PieceSums* sums = reinterpret_cast<PieceSums*>(static_cast<Part*>(scratch) + n_parts);
-        const int slot0 = (int)(n_parts - g.n_pieces);
-        piece_kernel<T, OP, kPieceMass><<<(unsigned)g.n_pieces, kPieceThreads, 0, stream>>>(a, sums, slot0, scores, out, totals);
-        if (OP != kLogProbs) {
-            piece_kernel<T, OP, kPieceTerms><<<(unsigned)g.n_pieces, kPieceThreads, 0, stream>>>(a, sums, slot0, scores, out, totals);
-            count_launch(1);
-        }
-        piece_kernel<T, OP, kPieceOut><<<(unsigned)g.n_pieces, kPieceThreads, 0, stream>>>(a, sums, slot0, scores, out, totals);
-        count_launch(2);
+        PB_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
+        if (OP != kLogProbs)
+            PB_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
+        PB_TRY(launch(piece_kernel<T, OP, kPieceOut>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
     }
-    if (want && n_parts != 1) {
-        PB_CUDA_TRY(launch_after(finish_kernel, 1u, (unsigned)kFinishThreads, stream, (const Part*)totals.parts, n_parts, scale, loss, kl, clipped));
-        count_launch(1);
-    }
+    if (want && n_parts != 1)
+        PB_TRY(launch(finish_kernel, 1, kFinishThreads, 0, (const Part*)totals.parts, n_parts, scale, loss, kl, clipped));
+    count_launch(launches);
     return PB_OK;
 }
 
@@ -913,8 +941,8 @@ int launch_objective(const pb_objective* o, const void* scores, void* grad, floa
         if (clipped) PB_CUDA_TRY(cudaMemsetAsync(clipped, 0, sizeof(*clipped), stream));
         return launch_pairs<T>(a, o->scale, static_cast<const T*>(scores), static_cast<T*>(grad), loss, static_cast<double*>(scratch), stream);
     }
-    const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, log1p(o->clip_high), log1p(-o->clip_low),
-                      (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), o->kl_coef, (float)o->scale};
+    const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(o->clip_high)), split(log1p(-o->clip_low)),
+                      (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
     if (o->kind == PB_OBJECTIVE_CHOICE) return launch_groups<T, kChoice>(a, o->scale, scores, grad, loss, kl, clipped, scratch, stream);
     return launch_groups<T, kPolicy>(a, o->scale, scores, grad, loss, kl, clipped, scratch, stream);
 }
@@ -973,7 +1001,7 @@ extern "C" int pb_objective_evaluate(const pb_objective* o, const void* scores, 
 
 extern "C" int64_t pb_group_log_probs_bytes(const pb_groups* g) {
     if (check_groups(g)) return PB_ERR_ARG;
-    return n_group_parts(g) * (int64_t)sizeof(Part) + g->n_pieces * (int64_t)sizeof(PieceSums);
+    return group_scratch_bytes(g);
 }
 
 extern "C" int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* workspace,

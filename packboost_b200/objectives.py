@@ -187,15 +187,16 @@ def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
     return group, n_groups
 
 
-_SHORT, _WINDOW, _STEP, _MEDIUM, _LARGE, _PIECE = 128, 1024, 896, 1024, 8192, 4096
+_TEAM_ROWS = (4, 8, 16, 32, 64, 128, 256)
+_MEDIUM, _LARGE, _PIECE = 1024, 8192, 4096
 
 
 def _lay_out_groups(group: torch.Tensor) -> dict:
-    """Offsets of the groups that have rows, the rows by group where they are in another order, and the groups by
-    length: windows of short ones, lists of those a CTA holds, pieces of long ones."""
+    """The rows by group where they are in another order, and the groups by length: teams of lanes for short ones, a
+    list of those that a CTA holds, pieces of long ones."""
     n, dev = group.shape[0], group.device
     if n == 0:
-        return {"n_groups": 0, "n_windows": 0, "n_medium": 0, "n_large": 0, "n_pieces": 0}
+        return {"n_groups": 0}
     rows = None
     if not bool((group[1:] >= group[:-1]).all()):
         group, order = torch.sort(group, stable=True)
@@ -203,43 +204,32 @@ def _lay_out_groups(group: torch.Tensor) -> dict:
     heads = torch.ones(n, dtype=torch.bool, device=dev)
     heads[1:] = group[1:] != group[:-1]
     starts = torch.nonzero(heads)[:, 0]
-    offsets = torch.cat([starts, starts.new_full((1,), n)])
-    lengths = offsets[1:] - offsets[:-1]
-    out = {"rows": rows, "offsets": offsets.to(torch.int32), "n_groups": starts.shape[0], "windows": None,
-           "window_words": None}
-
-    short = lengths <= _SHORT
-    windows = torch.unique(starts[short] // _STEP)
-    out["n_windows"] = windows.shape[0]
-    if out["n_windows"]:
-        number = heads.cumsum(0) - 1                       # group of a place
-        home = torch.where(short, starts // _STEP, torch.full_like(starts, -1))[number]
-        place = windows[:, None] * _STEP + torch.arange(_WINDOW, device=dev)
-        inside = place < n
-        place = place.clamp_max(n - 1)
-        mine = inside & (home[place] == windows[:, None])
-        first = mine & heads[place]
-        last = mine & (place + 1 == offsets[1:][number[place]])
-        shape = (out["n_windows"], _WINDOW // 4, 4)
-        bit = torch.arange(4, device=dev)
-        word = ((first.view(shape) << bit) | (mine.view(shape) << (bit + 4)) | (last.view(shape) << (bit + 8))).sum(2)
-        begun = first.view(shape).sum(2)
-        out["window_words"] = (word | ((begun.cumsum(1) - begun) << 12)).to(torch.int32)
-        out["windows"] = windows.to(torch.int32)
-
-    medium = torch.nonzero(~short & (lengths <= _MEDIUM))[:, 0]
-    large = torch.nonzero((lengths > _MEDIUM) & (lengths <= _LARGE))[:, 0]
-    out["n_medium"], out["n_large"] = medium.shape[0], large.shape[0]
-    out["listed"] = torch.cat([medium, large]).to(torch.int32)
-    long = lengths > _LARGE
-    begin, length = starts[long].cpu().numpy(), lengths[long].cpu().numpy()
+    lengths = torch.diff(starts, append=starts.new_full((1,), n))
+    # class 0 .. 6: teams, 7 and 8: held, 9: pieces; groups of a class in the order of their rows
+    limits = torch.tensor(_TEAM_ROWS + (_MEDIUM, _LARGE), device=dev)
+    kind = torch.bucketize(lengths, limits)
+    table = torch.stack([starts, lengths], 1).to(torch.int32)[torch.sort(kind, stable=True).indices]
+    count = torch.bincount(kind, minlength=10).tolist()
+    parts = list(torch.split(table, count))
+    out = {"rows": rows, "n_groups": starts.shape[0]}
+    teams, warps = [], []
+    for c in range(7):
+        per_warp = 32 >> min(c, 5)
+        warps.append(-(-count[c] // per_warp))
+        teams += [parts[c], table.new_zeros((warps[c] * per_warp - count[c], 2))]
+    out["team_warps"] = tuple(warps)
+    out["teams"] = torch.cat(teams)
+    out["n_medium"], out["n_large"] = count[7], count[8]
+    out["medium_rows"], out["large_rows"] = (int(parts[c][:, 1].max()) if count[c] else 0 for c in (7, 8))
+    out["held"] = torch.cat(parts[7:9])
+    begin, length = parts[9].cpu().numpy().astype(np.int64).T
     count = -(-length // _PIECE)
     first = np.cumsum(count) - count
     which = np.repeat(np.arange(len(count)), count)
     step = (np.arange(len(which)) - first[which]) * _PIECE
-    table = np.stack([begin[which] + step, np.minimum(length[which] - step, _PIECE), first[which], count[which]], 1)
+    pieces = np.stack([begin[which] + step, np.minimum(length[which] - step, _PIECE), first[which], count[which]], 1)
     out["n_pieces"] = len(which)
-    out["pieces"] = torch.from_numpy(table.astype(np.int32)).to(dev)
+    out["pieces"] = torch.from_numpy(pieces.astype(np.int32)).to(dev)
     return out
 
 

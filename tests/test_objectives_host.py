@@ -103,7 +103,7 @@ def test_layout_of_pairs(rows, pairs, hubs, touched, n_sm):
     assert lay["n_cuts"] == len(cut) and run[-1] < n_sm * O._RUNS_PER_SM
 
 
-@pytest.mark.parametrize("lengths", [[], [1], [1] * 5000, [128] * 40, [129, 1, 128, 1024, 1025, 3, 8192, 8193, 5, 4096 * 3, 1],
+@pytest.mark.parametrize("lengths", [[], [1], [1] * 5000, [128] * 40, [256, 257, 129, 1, 128, 1024, 1025, 3, 8192, 8193, 5, 4096 * 3, 1],
                                      [7, 13, 127, 2] * 400, [20_000], [895, 1, 1, 128, 900, 128]])
 @pytest.mark.parametrize("mixed", [False, True])
 def test_layout_of_groups(lengths, mixed):
@@ -118,32 +118,36 @@ def test_layout_of_groups(lengths, mixed):
         return
     rows = np.arange(n) if lay["rows"] is None else lay["rows"].numpy()
     assert (lay["rows"] is None) == bool((np.diff(ids) >= 0).all())
-    off = lay["offsets"].numpy()
-    for g, (a, b) in enumerate(zip(off[:-1], off[1:])):
-        assert b - a == lengths[g] and (ids[rows[a:b]] == 3 * g).all()
-    assert off[0] == 0 and off[-1] == n
+    starts = np.cumsum([0] + lengths)[:-1]
+    length_of = dict(zip(starts.tolist(), lengths))
+    for a, size in length_of.items():
+        assert len(set(ids[rows[a: a + size]])) == 1
     done = np.zeros(n, int)                                     # every place is somebody's, once
-    if lay["n_windows"]:
-        words = lay["window_words"].numpy().view(np.uint32)
-        for k, word in zip(lay["windows"].numpy(), words):
-            bits = (word[:, None] >> np.arange(12, dtype=np.uint32)) & 1
-            head, mine, last = (bits[:, i: i + 4].reshape(-1).astype(bool) for i in (0, 4, 8))
-            place = k * O._STEP + np.arange(O._WINDOW)
-            assert place[mine].max() < n and mine.any()
-            done[place[mine]] += 1
-            np.testing.assert_array_equal(place[head], off[:-1][np.isin(off[:-1], place[mine])])
-            np.testing.assert_array_equal(place[last] + 1, off[1:][np.isin(off[1:] - 1, place[mine])])
-            np.testing.assert_array_equal(word >> 12, np.cumsum(head.reshape(-1, 4).sum(1)) - head.reshape(-1, 4).sum(1))
-            for a, b in zip(np.flatnonzero(head), np.flatnonzero(last)):
-                assert b - a < O._SHORT and mine[a: b + 1].all()
-    listed = lay["listed"].numpy()
-    for i, g in enumerate(listed):
-        low, high = (O._SHORT, O._MEDIUM) if i < lay["n_medium"] else (O._MEDIUM, O._LARGE)
-        assert low < lengths[g] <= high
-        done[off[g]: off[g + 1]] += 1
+
+    def take(table, low, high):
+        for begin, size in table:
+            assert length_of[begin] == size and low < size <= high
+            done[begin: begin + size] += 1
+
+    team, low = lay["teams"].numpy(), 0
+    for c, high in enumerate(O._TEAM_ROWS):
+        own = team[: lay["team_warps"][c] * (32 >> min(c, 5))]
+        team = team[len(own):]
+        real = own[own[:, 1] > 0]
+        assert (own[len(real):] == 0).all() and len(own) - len(real) < 32
+        take(real.tolist(), low, high)
+        low = high
+    assert len(team) == 0
+    held = lay["held"].numpy().tolist()
+    take(held[: lay["n_medium"]], 256, O._MEDIUM)
+    take(held[lay["n_medium"]:], O._MEDIUM, O._LARGE)
+    assert len(held) == lay["n_medium"] + lay["n_large"]
+    assert lay["medium_rows"] == max([s for _, s in held[: lay["n_medium"]]], default=0)
+    assert lay["large_rows"] == max([s for _, s in held[lay["n_medium"]:]], default=0)
     for i, (begin, size, first, count) in enumerate(lay["pieces"].numpy()):
-        assert 0 < size <= O._PIECE and first <= i < first + count
-        assert begin - (i - first) * O._PIECE in off and (i == first + count - 1) == (begin + size in off)
+        start = begin - (i - first) * O._PIECE
+        assert 0 < size <= O._PIECE and first <= i < first + count and length_of[start] > O._LARGE
+        assert (i == first + count - 1) == (begin + size == start + length_of[start])
         done[begin: begin + size] += 1
     assert (done == 1).all() and lay["n_pieces"] == len(lay["pieces"])
 
@@ -236,7 +240,7 @@ def test_library_refuses_bad_descriptors():
         return B.Pairs(**dict(dict(n_rows=4, n_items=1024, other=16, chunk_rows=16, chunk_heads=16, run_tiles=1), **kw))
 
     def groups(**kw):
-        return B.Groups(**dict(dict(n_rows=3, n_groups=1, offsets=16, n_medium=1, listed=16), **kw))
+        return B.Groups(**dict(dict(n_rows=3, n_groups=1, n_medium=1, medium_rows=3, held=16), **kw))
 
     ok, good = pairs(), groups()
     refused(B.Objective(kind=9), "unknown objective")
@@ -251,8 +255,10 @@ def test_library_refuses_bad_descriptors():
                       (dict(beta=1.0, scale=float("nan")), "scale")):
         refused(B.Objective(kind=0, pairs=C.pointer(ok), **kw), match)
     for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_groups=4), "n_groups"), (dict(n_groups=0), "without a group"),
-                      (dict(offsets=None), "offsets"), (dict(n_medium=0), "not laid out"), (dict(listed=None), "null"),
-                      (dict(n_windows=1), "null"), (dict(n_pieces=1), "null"), (dict(n_large=-1), "range")):
+                      (dict(n_medium=0), "not laid out"), (dict(held=None), "null"), (dict(held=20), "aligned"),
+                      (dict(team_warps=(0, 1, 0, 0, 0, 0, 0)), "null"), (dict(team_warps=(-1, 0, 0, 0, 0, 0, 0)), "range"),
+                      (dict(n_pieces=1), "null"), (dict(n_large=-1), "range"), (dict(medium_rows=0), "range"),
+                      (dict(medium_rows=1025), "range"), (dict(n_medium=0, n_large=1, large_rows=9000), "range")):
         refused(B.Objective(kind=1, groups=C.pointer(groups(**kw))), match)
     refused(B.Objective(kind=1, groups=C.pointer(good)), "target")
     rows = dict(groups=C.pointer(good), advantage=16, old=16)
