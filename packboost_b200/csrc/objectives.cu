@@ -80,23 +80,35 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Part* __re
 struct PairArgs {
     pb_pairs p;
     float beta, smoothing, half_tau;  // half_tau: 1 / (2 beta)
-    int squared;
-    float scale;
+    float factor;                     // of the sum of a row's terms: scale and what the terms leave out
 };
 
-// Loss and derivative with respect to d of a pair whose (reference-corrected) score difference is d.
-__device__ __forceinline__ float pair_slope(const PairArgs& a, float d, float* loss) {
-    if (a.squared) {
+// log(1 + e) for e in [0, 1]: with s = e / (2 + e), 2 atanh(s), s <= 1/3; the term after the last one kept is
+// s^14 / 15 of the sum, below 2^-26.
+__device__ __forceinline__ float log1p_of(float e) {
+    const float s = __fdividef(e, 2.f + e), q = s * s;
+    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+    p = fmaf(q, p, 1.f / 9.f);
+    p = fmaf(q, p, 1.f / 7.f);
+    p = fmaf(q, p, 1.f / 5.f);
+    p = fmaf(q, p, 1.f / 3.f);
+    return 2.f * fmaf(s * q, p, s);
+}
+
+// Derivative with respect to d, without the factor 2 (squared) or beta, of a pair whose (reference-corrected)
+// score difference is d; its loss, if wanted.
+template <bool SQUARED>
+__device__ __forceinline__ float pair_slope(const PairArgs& a, float d, bool want, float* loss) {
+    if (SQUARED) {
         const float off = d - a.half_tau;
         *loss = off * off;
-        return 2.f * off;
+        return off;
     }
     // softplus(-z) + e z has the derivative e - sigmoid(-z)
     const float z = a.beta * d;
     const float e = expf(-fabsf(z));
-    *loss = fmaxf(-z, 0.f) + log1pf(e) + (a.smoothing != 0.f ? a.smoothing * z : 0.f);
-    const float q = __fdividef(z > 0.f ? e : 1.f, 1.f + e);
-    return a.beta * (a.smoothing - q);
+    if (want) *loss = fmaxf(-z, 0.f) + log1p_of(e) + (a.smoothing != 0.f ? a.smoothing * z : 0.f);
+    return a.smoothing - __fdividef(z > 0.f ? e : 1.f, 1.f + e);
 }
 
 // A thread takes eight neighbouring items, a CTA a tile of them at a time and a run of tiles in all; a row's
@@ -112,7 +124,7 @@ struct PairPieces {
     double *lead, *tail, *loss;  // per run: sums before its first row starts and after its last one has
 };
 
-template <typename T>
+template <typename T, bool SQUARED>
 __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T* __restrict__ scores, T* __restrict__ grad,
                                                             PairPieces pieces, double scale, float* loss_out) {
     __shared__ double s_tail[2][kPairThreads / 32];
@@ -122,6 +134,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t tile0 = (int64_t)blockIdx.x * a.p.run_tiles;
     const int64_t tile1 = min(tile0 + a.p.run_tiles, a.p.n_items / kPairTile);
+    const bool want = pieces.loss || loss_out;
     double carry = 0.0, loss = 0.0;  // carry: of the row that is open where the tile begins
     bool seen = false;               // a row has started in this run
     int last_row = 0;
@@ -136,47 +149,60 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
         if (a.p.offset) {
             *reinterpret_cast<float4*>(off) = *reinterpret_cast<const float4*>(a.p.offset + i0);
             *reinterpret_cast<float4*>(off + 4) = *reinterpret_cast<const float4*>(a.p.offset + i0 + 4);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kPairItems; ++u) off[u] = 0.f;
         }
         if (a.p.weight) {
             *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(a.p.weight + i0);
             *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(a.p.weight + i0 + 4);
-        }
-        float other[kPairItems];
+        } else {
 #pragma unroll
-        for (int u = 0; u < kPairItems; ++u) other[u] = to_f32(scores[word[u] & 0x7FFFFFFFu]);
+            for (int u = 0; u < kPairItems; ++u) w[u] = 1.f;
+        }
+        float term[kPairItems];
+        {
+            T own[kPairItems], other[kPairItems];
+            int r = row;
+#pragma unroll
+            for (int u = 0; u < kPairItems; ++u) {
+                other[u] = scores[word[u] & 0x7FFFFFFFu];
+                if (u > 0) r += (int)((heads >> u) & 1u);
+                own[u] = scores[r];
+            }
+            r = row;
+            float chunk_loss = 0.f;
+#pragma unroll
+            for (int u = 0; u < kPairItems; ++u) {
+                if (u > 0) r += (int)((heads >> u) & 1u);
+                const uint32_t sign = word[u] & 0x80000000u;
+                const float d = (to_f32(own[u]) - to_f32(other[u])) - off[u];
+                float l;
+                float t = pair_slope<SQUARED>(a, __uint_as_float(__float_as_uint(d) ^ sign), want, &l);
+                t = __uint_as_float(__float_as_uint(t) ^ sign) * w[u];
+                // (an item of a row with itself fills a row without pairs, or the last tile)
+                term[u] = (int)(word[u] ^ sign) != r ? t : 0.f;
+                if (want && !sign && (int)word[u] != r) chunk_loss = fmaf(w[u], l, chunk_loss);
+            }
+            loss += (double)chunk_loss;
+        }
         const int row_open = row - (int)(heads & 1u);  // the row that is open where the chunk begins
-        float own = to_f32(scores[row]);
-        float acc = 0.f, lead = 0.f, chunk_loss = 0.f;
+        float acc = 0.f, lead = 0.f;
         bool any = false;                              // a row has started in this chunk
 #pragma unroll
         for (int u = 0; u < kPairItems; ++u) {
             if ((heads >> u) & 1u) {
                 if (any)
-                    grad[row] = from_f32<T>(acc * a.scale);
+                    grad[row] = from_f32<T>(acc * a.factor);
                 else
                     lead = acc;
-                if (u > 0) own = to_f32(scores[++row]);
+                if (u > 0) ++row;
                 any = true;
                 acc = 0.f;
             }
-            const uint32_t o = word[u] & 0x7FFFFFFFu;
-            const bool rejected = word[u] >> 31;
-            float d = own - other[u];
-            if (a.p.offset) d -= off[u];
-            if (rejected) d = -d;
-            float l;
-            float sl = pair_slope(a, d, &l);
-            if (a.p.weight) {
-                sl *= w[u];
-                l *= w[u];
-            }
-            if (o != (uint32_t)row) {                  // (else it fills a row without pairs, or the last tile)
-                acc += rejected ? -sl : sl;
-                if (!rejected) chunk_loss += l;
-            }
+            acc += term[u];
         }
         if (!any) lead = acc;
-        loss += (double)chunk_loss;
 
         // inclusive scan of what is open at the end of each chunk
         const uint32_t mask = __ballot_sync(0xFFFFFFFFu, any);
@@ -206,8 +232,8 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
         if (any) {
             const double sum = open + (double)lead;
             if (started || prior)
-                grad[row_open] = from_f32<T>((float)sum * a.scale);
-            else
+                grad[row_open] = from_f32<T>((float)sum * a.factor);
+            else if (pieces.lead)   // (there are several runs)
                 pieces.lead[blockIdx.x] = sum;
         }
         for (int k = 0; k < kPairThreads / 32; ++k) {
@@ -220,11 +246,13 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
         // the row that is open at the end: done, or continued in the next run
         const int64_t next = tile1 * kPairThreads;
         const bool ends = tile1 == a.p.n_items / kPairTile || (a.p.chunk_heads[next] & 1u);
-        if (seen && ends) grad[last_row] = from_f32<T>((float)carry * a.scale);
-        if (!seen) pieces.lead[blockIdx.x] = carry;
-        pieces.tail[blockIdx.x] = carry;
+        if (seen && ends) grad[last_row] = from_f32<T>((float)carry * a.factor);
+        if (pieces.lead) {
+            if (!seen) pieces.lead[blockIdx.x] = carry;
+            pieces.tail[blockIdx.x] = carry;
+        }
     }
-    if (pieces.loss || loss_out) {
+    if (want) {
         loss = block_sum(loss, scratch);
         if (threadIdx.x == 0) {
             if (loss_out)  // one run: nothing else to add
@@ -257,7 +285,7 @@ __global__ void __launch_bounds__(kPairFinishThreads) pair_finish_kernel(PairArg
     double t = 0.0;
     for (int r = first + 1 + lane; r <= last; r += 32) t += pieces.lead[r];
     t = warp_sum(t) + pieces.tail[first];
-    if (lane == 0) grad[row] = from_f32<T>((float)t * a.scale);
+    if (lane == 0) grad[row] = from_f32<T>((float)t * a.factor);
 }
 
 // A launch; `early`: it may begin before the one in front of it on the stream has ended, and waits for that itself.
@@ -281,15 +309,19 @@ int64_t n_runs_of(const pb_pairs* p) {
 }
 
 template <typename T>
-int launch_pairs(const PairArgs& a, double scale, const T* scores, T* grad, float* loss, double* scratch, cudaStream_t stream) {
+int launch_pairs(const PairArgs& a, bool squared, double scale, const T* scores, T* grad, float* loss, double* scratch, cudaStream_t stream) {
     const int64_t n_runs = n_runs_of(&a.p);
     if (n_runs == 0) {
         if (loss) PB_CUDA_TRY(cudaMemsetAsync(loss, 0, 4, stream));
         return PB_OK;
     }
     const bool one = n_runs == 1;
-    PairPieces pieces{scratch, scratch + n_runs, loss && !one ? scratch + 2 * n_runs : nullptr};
-    pair_kernel<T><<<(unsigned)n_runs, kPairThreads, 0, stream>>>(a, scores, grad, pieces, scale, one ? loss : nullptr);
+    PairPieces pieces{nullptr, nullptr, nullptr};
+    if (!one) pieces = PairPieces{scratch, scratch + n_runs, loss ? scratch + 2 * n_runs : nullptr};
+    if (squared)
+        pair_kernel<T, true><<<(unsigned)n_runs, kPairThreads, 0, stream>>>(a, scores, grad, pieces, scale, one ? loss : nullptr);
+    else
+        pair_kernel<T, false><<<(unsigned)n_runs, kPairThreads, 0, stream>>>(a, scores, grad, pieces, scale, one ? loss : nullptr);
     count_launch(1);
     if (!one && (loss || a.p.n_cuts)) {
         const int64_t grid = (a.p.n_cuts + kPairFinishThreads / 32 - 1) / (kPairFinishThreads / 32) + 1;
@@ -868,13 +900,14 @@ int64_t n_group_parts(const pb_groups* g) {
     return team_grid(team_warps(g, 0, 6)) + team_grid(g->team_warps[6]) + g->n_medium + g->n_large + g->n_pieces;
 }
 
-// Scratch: what the CTAs leave of the totals, then the sums of pieces.
-int64_t group_scratch_bytes(const pb_groups* g) {
-    return n_group_parts(g) * (int64_t)sizeof(Part) + g->n_pieces * (int64_t)sizeof(PieceSums);
+// Scratch: the sums of pieces, then what the CTAs leave of the totals, if there are several.
+int64_t group_scratch_bytes(const pb_groups* g, bool totals) {
+    const int64_t n = n_group_parts(g);
+    return (totals && n > 1 ? n * (int64_t)sizeof(Part) : 0) + g->n_pieces * (int64_t)sizeof(PieceSums);
 }
 int64_t scratch_bytes(const pb_objective* o) {
-    if (o->kind == PB_OBJECTIVE_PREFERENCE) return 3 * n_runs_of(o->pairs) * (int64_t)sizeof(double);
-    return group_scratch_bytes(o->groups);
+    if (o->kind == PB_OBJECTIVE_PREFERENCE) return n_runs_of(o->pairs) > 1 ? 3 * n_runs_of(o->pairs) * (int64_t)sizeof(double) : 0;
+    return group_scratch_bytes(o->groups, true);
 }
 
 template <typename T, int OP>
@@ -885,7 +918,8 @@ int launch_groups(const GroupArgs& a, double scale, const void* scores_, void* o
     const pb_groups& g = a.g;
     const int64_t n_parts = n_group_parts(&g);
     const bool want = loss || kl || clipped;
-    const Totals totals{want ? static_cast<Part*>(scratch) : nullptr, scale, loss, kl, clipped, n_parts == 1, a.kl_coef};
+    PieceSums* const sums = static_cast<PieceSums*>(scratch);
+    const Totals totals{want && n_parts > 1 ? reinterpret_cast<Part*>(sums + g.n_pieces) : nullptr, scale, loss, kl, clipped, want && n_parts == 1, a.kl_coef};
     const int2* teams = reinterpret_cast<const int2*>(g.teams);
     int slot = 0, launches = 0;
     // the first launch waits for what is before it on the stream, the others may overlap with the ones before
@@ -920,7 +954,6 @@ int launch_groups(const GroupArgs& a, double scale, const void* scores_, void* o
         slot += (int)g.n_large;
     }
     if (g.n_pieces) {
-        PieceSums* sums = reinterpret_cast<PieceSums*>(static_cast<Part*>(scratch) + n_parts);
         PB_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
         if (OP != kLogProbs)
             PB_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
@@ -936,10 +969,11 @@ template <typename T>
 int launch_objective(const pb_objective* o, const void* scores, void* grad, float* loss, float* kl, int64_t* clipped, void* scratch,
                      cudaStream_t stream) {
     if (o->kind == PB_OBJECTIVE_PREFERENCE) {
-        const PairArgs a{*o->pairs, (float)o->beta, (float)o->smoothing, (float)(0.5 / o->beta), o->squared != 0, (float)o->scale};
+        const PairArgs a{*o->pairs, (float)o->beta, (float)o->smoothing, (float)(0.5 / o->beta),
+                         (float)(o->scale * (o->squared ? 2.0 : o->beta))};
         if (kl) PB_CUDA_TRY(cudaMemsetAsync(kl, 0, sizeof(*kl), stream));
         if (clipped) PB_CUDA_TRY(cudaMemsetAsync(clipped, 0, sizeof(*clipped), stream));
-        return launch_pairs<T>(a, o->scale, static_cast<const T*>(scores), static_cast<T*>(grad), loss, static_cast<double*>(scratch), stream);
+        return launch_pairs<T>(a, o->squared != 0, o->scale, static_cast<const T*>(scores), static_cast<T*>(grad), loss, static_cast<double*>(scratch), stream);
     }
     const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(o->clip_high)), split(log1p(-o->clip_low)),
                       (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
@@ -1001,7 +1035,7 @@ extern "C" int pb_objective_evaluate(const pb_objective* o, const void* scores, 
 
 extern "C" int64_t pb_group_log_probs_bytes(const pb_groups* g) {
     if (check_groups(g)) return PB_ERR_ARG;
-    return group_scratch_bytes(g);
+    return group_scratch_bytes(g, false);
 }
 
 extern "C" int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* workspace,
@@ -1011,7 +1045,7 @@ extern "C" int pb_group_log_probs(const pb_groups* g, const void* scores, int64_
     PB_REQUIRE(g->n_rows == 0 || (scores && out), "scores or output is null");
     if (g->n_pieces) {
         PB_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 8 == 0, "workspace is null or not aligned");
-        if (workspace_bytes < pb_group_log_probs_bytes(g)) {
+        if (workspace_bytes < group_scratch_bytes(g, false)) {
             set_error("workspace of the log-probabilities: %lld bytes given, %lld needed", (long long)workspace_bytes,
                       (long long)pb_group_log_probs_bytes(g));
             return PB_ERR_WORKSPACE;

@@ -247,14 +247,19 @@ class _Layout:
     def _settle(self, device: torch.device, tensors: dict) -> None:
         self.device = device
         self._tensors = [t for t in tensors.values() if isinstance(t, torch.Tensor)]
+        self._structs: dict = {}   # descriptors of objectives on this layout, by their options
         stream = torch.cuda.current_stream(device)
         self._stream = stream.cuda_stream
         stream.synchronize()
 
-    def _used_on(self, stream: torch.cuda.Stream) -> None:
-        if stream.cuda_stream != self._stream:
+    def _used_now(self) -> int:
+        """The current stream of the layout's device, which must be the current one."""
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if stream != self._stream:
+            current = torch.cuda.current_stream()
             for t in self._tensors:
-                t.record_stream(stream)
+                t.record_stream(current)
+        return stream
 
 
 class RowPairs(_Layout):
@@ -299,19 +304,20 @@ class RowGroups(_Layout):
             self.n_rows, self.n_groups = int(g.shape[0]), n_groups
             self._settle(home, parts)
         self._struct = self._point(B.Groups, parts, n_rows=self.n_rows)
+        self._log_probs_bytes: int | None = None
 
 
 # ---- operators --------------------------------------------------------------------------------------
 
 
-def _check_scores(scores, layout, name: str = "scores") -> torch.Tensor:
+def _check_scores(scores, layout) -> torch.Tensor:
     if not isinstance(scores, torch.Tensor) or scores.dtype not in _SCORE_TYPES:
-        raise TypeError(f"{name} must be a float32, float16 or bfloat16 tensor")
+        raise TypeError("scores must be a float32, float16 or bfloat16 tensor")
     if scores.device != layout.device:
-        raise ValueError(f"{name} are on {scores.device}, the layout on {layout.device}")
+        raise ValueError(f"scores are on {scores.device}, the layout on {layout.device}")
     if scores.dim() != 1 or scores.shape[0] != layout.n_rows:
-        raise ValueError(f"{name} must be 1-D with {layout.n_rows} entries")
-    return scores.detach().contiguous()
+        raise ValueError(f"scores must be 1-D with {layout.n_rows} entries")
+    return scores.detach() if scores.is_contiguous() else scores.detach().contiguous()
 
 
 def _per_row(values, name: str, layout) -> torch.Tensor:
@@ -319,6 +325,8 @@ def _per_row(values, name: str, layout) -> torch.Tensor:
         raise TypeError(f"{name} must be a tensor")
     if values.device != layout.device:
         raise ValueError(f"{name} is on {values.device}, the layout on {layout.device}")
+    if values.dtype == torch.float32 and values.dim() == 1 and values.shape[0] == layout.n_rows and values.is_contiguous():
+        return values
     return _numbers(values, name, layout.n_rows, layout.device).to(torch.float32).contiguous()
 
 
@@ -334,6 +342,9 @@ def _scale(reduction: str, total: float, what: str) -> float:
 
 def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) -> B.Objective:
     beta, smoothing = float(beta), float(label_smoothing)
+    options = (beta, smoothing, kind, reduction)
+    if options in pairs._structs:
+        return pairs._structs[options]
     if not (beta > 0 and math.isfinite(beta)):
         raise ValueError("beta must be positive")
     if not 0 <= smoothing < 0.5:
@@ -342,46 +353,71 @@ def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) 
         raise ValueError(f"unknown kind {kind!r}")
     if kind == "squared" and smoothing:
         raise ValueError("the squared form has no label smoothing")
-    return B.Objective(kind=_PREFERENCE, pairs=C.pointer(pairs._struct), beta=beta, smoothing=smoothing,
-                       squared=int(kind == "squared"), scale=_scale(reduction, pairs.total_weight, "pairs"))
+    struct = B.Objective(kind=_PREFERENCE, pairs=C.pointer(pairs._struct), beta=beta, smoothing=smoothing,
+                         squared=int(kind == "squared"), scale=_scale(reduction, pairs.total_weight, "pairs"))
+    return _kept_struct(pairs, options, struct)
 
 
 def _choice_struct(groups: RowGroups, target: torch.Tensor, reduction) -> B.Objective:
-    return B.Objective(kind=_CHOICE, groups=C.pointer(groups._struct), target=B._ptr(target) or None,
-                       scale=_scale(reduction, groups.n_groups, "groups"))
+    options = (_CHOICE, reduction)
+    if options not in groups._structs:
+        _kept_struct(groups, options, B.Objective(kind=_CHOICE, groups=C.pointer(groups._struct), target=16,
+                                                  scale=_scale(reduction, groups.n_groups, "groups")))
+    struct = B.Objective.from_buffer_copy(groups._structs[options])
+    struct.target = target.data_ptr()
+    return struct
 
 
 def _policy_struct(groups: RowGroups, advantage, old, reference, clip, kl_coef, reduction) -> B.Objective:
-    low, high = (float(c) for c in clip)
-    if not (0 <= low <= 1 and high >= 0):
-        raise ValueError("clip must be (low, high) with low in [0, 1] and high not negative")
-    kl_coef = float(kl_coef)
-    if not math.isfinite(kl_coef):
-        raise ValueError("kl_coef must be finite")
-    if reference is None and kl_coef:
+    low, high = clip
+    low, high, kl = float(low), float(high), float(kl_coef)
+    options = (_POLICY, low, high, kl, reduction)
+    if options not in groups._structs:
+        if not (0 <= low <= 1 and high >= 0):
+            raise ValueError("clip must be (low, high) with low in [0, 1] and high not negative")
+        if not math.isfinite(kl):
+            raise ValueError("kl_coef must be finite")
+        _kept_struct(groups, options, B.Objective(
+            kind=_POLICY, groups=C.pointer(groups._struct), advantage=16, old=16, reference=16, clip_low=low, clip_high=high,
+            kl_coef=kl, scale=_scale(reduction, groups.n_groups, "groups")))
+    if reference is None and kl:
         raise ValueError("kl_coef needs reference_log_probs")
-    return B.Objective(kind=_POLICY, groups=C.pointer(groups._struct), advantage=B._ptr(advantage) or None,
-                       old=B._ptr(old) or None, reference=B._ptr(reference) or None, clip_low=low, clip_high=high,
-                       kl_coef=kl_coef, scale=_scale(reduction, groups.n_groups, "groups"))
+    struct = B.Objective.from_buffer_copy(groups._structs[options])
+    struct.advantage, struct.old = advantage.data_ptr(), old.data_ptr()
+    struct.reference = None if reference is None else reference.data_ptr()
+    return struct
+
+
+def _kept_struct(layout: _Layout, options: tuple, struct: B.Objective) -> B.Objective:
+    """Keeps a descriptor (with addresses of rows still to be put in) and the size of its scratch."""
+    nbytes = int(B.lib().pb_objective_workspace_bytes(C.byref(struct)))
+    if nbytes < 0:
+        B.check(nbytes)
+    layout._scratch_bytes = nbytes    # (the layout alone decides it)
+    if len(layout._structs) >= 64:    # (options that change from call to call: start again)
+        layout._structs = {}
+    layout._structs[options] = struct
+    return struct
 
 
 def _evaluate(struct: B.Objective, layout: _Layout, scores: torch.Tensor, policy: bool = False):
-    lib, dev = B.lib(), layout.device
-    nbytes = lib.pb_objective_workspace_bytes(C.byref(struct))
-    if nbytes < 0:
-        B.check(int(nbytes))
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev)
-        layout._used_on(stream)
-        grad = torch.empty_like(scores)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        kl = torch.empty((), dtype=torch.float32, device=dev) if policy else None
-        clipped = torch.empty((), dtype=torch.int64, device=dev) if policy else None
-        scratch = torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
-        B.check(lib.pb_objective_evaluate(C.byref(struct), scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(),
-                                          loss.data_ptr(), B._ptr(kl), B._ptr(clipped), scratch.data_ptr(), nbytes,
-                                          stream.cuda_stream))
-    return PolicyLoss(loss, grad, kl, clipped) if policy else LossAndGradient(loss, grad)
+    dev = layout.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _evaluate(struct, layout, scores, policy)
+    stream, nbytes = layout._used_now(), layout._scratch_bytes
+    grad = torch.empty_like(scores)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None   # (the allocator takes it back in the stream's order)
+    if not policy:
+        B.check(B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(),
+                                              loss.data_ptr(), None, None, scratch, nbytes, stream))
+        return LossAndGradient(loss, grad)
+    kl = torch.empty((), dtype=torch.float32, device=dev)
+    clipped = torch.empty((), dtype=torch.int64, device=dev)
+    B.check(B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
+                                          kl.data_ptr(), clipped.data_ptr(), scratch, nbytes, stream))
+    return PolicyLoss(loss, grad, kl, clipped)
 
 
 def preference_loss(scores: torch.Tensor, pairs: RowPairs, *, beta: float = 1.0, label_smoothing: float = 0.0,
@@ -435,15 +471,17 @@ def policy_loss(scores: torch.Tensor, groups: RowGroups, advantage: torch.Tensor
 def group_log_probs(scores: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """``s - log sum exp s`` over each row's group, in the scores' type; -inf where the score is."""
     scores = _check_scores(scores, groups)
-    with torch.cuda.device(groups.device):
-        stream = torch.cuda.current_stream(groups.device)
-        groups._used_on(stream)
-        out = torch.empty_like(scores)
-        lib, struct = B.lib(), C.byref(groups._struct)
-        nbytes = int(lib.pb_group_log_probs_bytes(struct))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=groups.device)
-        B.check(lib.pb_group_log_probs(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], out.data_ptr(),
-                                       scratch.data_ptr(), nbytes, stream.cuda_stream))
+    if torch.cuda.current_device() != groups.device.index:
+        with torch.cuda.device(groups.device):
+            return group_log_probs(scores, groups)
+    lib, stream = B.lib(), groups._used_now()
+    out = torch.empty_like(scores)
+    if groups._log_probs_bytes is None:
+        groups._log_probs_bytes = int(lib.pb_group_log_probs_bytes(groups._struct))
+    nbytes = groups._log_probs_bytes
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=groups.device).data_ptr() if nbytes else None
+    B.check(lib.pb_group_log_probs(groups._struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], out.data_ptr(), scratch,
+                                   nbytes, stream))
     return out
 
 
@@ -455,10 +493,7 @@ class _FitObjective:
 
     def __init__(self, struct: B.Objective, layout: _Layout, kept: tuple) -> None:
         self.struct, self.layout, self._kept = struct, layout, kept
-        nbytes = int(B.lib().pb_objective_workspace_bytes(C.byref(struct)))
-        if nbytes < 0:
-            B.check(nbytes)
-        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=layout.device)
+        self.workspace = torch.empty(layout._scratch_bytes, dtype=torch.uint8, device=layout.device)
 
     def loss(self, preds: torch.Tensor) -> float:
         return float(_evaluate(self.struct, self.layout, preds).loss)

@@ -180,7 +180,7 @@ class _Stub:
     """A layout as far as the checks look at it."""
 
     def __init__(self, n_rows, **kw):
-        self.n_rows, self.device, self._struct = n_rows, torch.device("cpu"), kw.pop("struct", None)
+        self.n_rows, self.device, self._struct, self._structs = n_rows, torch.device("cpu"), kw.pop("struct", None), {}
         self.__dict__.update(kw)
 
 
@@ -242,7 +242,7 @@ def test_library_refuses_bad_descriptors():
     def groups(**kw):
         return B.Groups(**dict(dict(n_rows=3, n_groups=1, n_medium=1, medium_rows=3, held=16), **kw))
 
-    ok, good = pairs(), groups()
+    ok, good = pairs(n_items=2048), groups()
     refused(B.Objective(kind=9), "unknown objective")
     refused(B.Objective(kind=0), "pairs are null")
     refused(B.Objective(kind=1), "groups are null")
