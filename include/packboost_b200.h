@@ -411,47 +411,51 @@ typedef struct pb_round_log_header {
 #define PB_SCORE_F16 1
 #define PB_SCORE_BF16 2
 
-/* Pairs by row.  A pair is one item of each of its two rows; a row without pairs has one item that names
- * the row itself, and so have the places that fill the last tile of PB_PAIR_TILE items.  Items are in the
- * order of their rows.  A run of `run_tiles` tiles is one CTA's; a cut is a row whose items lie in several
- * runs: row, first run, last run. */
-#define PB_PAIR_ITEMS 8
-#define PB_PAIR_TILE 1024
+/* Pairs by row: a pair is one item of each of its two rows.
+ *  - A row with at most PB_SLICE_ITEMS items of either side is one of 64 rows of a slice.  The items of
+ *    a slice are stored by columns of 64, those of rows that were chosen first: `slices` holds the first
+ *    column and the numbers of columns of either side (rejected << 16), `slice_rows` the row (-1: none) and
+ *    its own numbers of items.  Items that fill up a column name any row.
+ *  - Another row's items are neighbours, the chosen ones first, and in chunks of up to PB_CHUNK_ITEMS: row,
+ *    first item, items, how many of them chosen; among the rows of several chunks, the row's number; first
+ *    chunk of the row, its number of chunks, 0.
+ * Every row is in one slice or has chunks. */
+#define PB_SLICE_ITEMS 32
+#define PB_CHUNK_ITEMS 512
 typedef struct pb_pairs {
     int64_t n_rows;
-    int64_t n_items;              /* a multiple of PB_PAIR_TILE */
-    const uint32_t* other;        /* [n_items] the other row; bit 31: the item's own row is the rejected one; 16-byte aligned */
-    const float* offset;          /* [n_items] reference score of the own row minus the other's, or NULL; aligned alike */
-    const float* weight;          /* [n_items], or NULL: 1; aligned alike */
-    const int32_t* chunk_rows;    /* [n_items / 8] row of the first of eight items */
-    const uint8_t* chunk_heads;   /* [n_items / 8] which of the eight are the first of their row */
-    int64_t run_tiles;
-    int64_t n_cuts;
-    const int32_t* cuts;          /* [n_cuts][3] */
+    int64_t n_slices;
+    const int32_t* slices;        /* [n_slices][2], 8-byte aligned */
+    const int32_t* slice_rows;    /* [n_slices][64][2], 16-byte aligned */
+    int64_t n_chunks;
+    const int32_t* chunks;        /* [n_chunks][8], 16-byte aligned */
+    int64_t n_split;              /* rows of several chunks */
+    const int32_t* other;         /* the other row of every item; 8-byte aligned like the next two */
+    const float* offset;          /* reference score of the own row minus the other's, or NULL */
+    const float* weight;          /* or NULL: 1 */
 } pb_pairs;
 
 /* Groups of rows: those that have any; `rows` lists their rows (NULL: the rows in order), and a group is
  * its first place in that list and its number of rows.  By length:
- *  - up to 4 << c rows for c = 0 .. 5, 256 for c = 6: one of 32 >> min(c, 5) groups of a warp.  `teams`
- *    holds the classes one after the other, each filled up with groups of no rows to whole warps;
- *  - up to PB_MEDIUM_ROWS, then up to PB_LARGE_ROWS (`medium_rows` and `large_rows` are the longest of
- *    either): a CTA's, in `held`;
+ *  - up to PB_TEAM_ROWS: 1, 2, 4 ... 32 lanes of a warp, the fewest that have at most eight rows each.
+ *    `team_warps` holds for every warp its first entry of `teams` and log2 of the lanes (bits 0-7) with the most
+ *    rows that a lane has (from bit 8); of `teams` a warp takes 32 >> log2(lanes) entries, of no rows some;
+ *  - up to PB_BLOCK_ROWS: a CTA's, in `blocks` (`block_rows`: rows of the longest);
  *  - longer: pieces of up to PB_PIECE_ROWS: first place, rows, number of the group's first piece, number
  *    of its pieces. */
-#define PB_MEDIUM_ROWS 1024
-#define PB_LARGE_ROWS 8192
-#define PB_PIECE_ROWS 4096
+#define PB_TEAM_ROWS 256
+#define PB_BLOCK_ROWS 8192
+#define PB_PIECE_ROWS 2048
 typedef struct pb_groups {
     int64_t n_rows;
     int64_t n_groups;
     const int32_t* rows;          /* [n_rows], or NULL */
-    int64_t team_warps[7];
-    const int32_t* teams;         /* [sum of team_warps[c] * (32 >> min(c, 5))][2], 8-byte aligned */
-    int64_t n_medium;
-    int64_t n_large;
-    int64_t medium_rows;
-    int64_t large_rows;
-    const int32_t* held;          /* [n_medium + n_large][2], 8-byte aligned */
+    int64_t n_team_warps;
+    const int32_t* team_warps;    /* [n_team_warps][2], 8-byte aligned */
+    const int32_t* teams;         /* [][2], 8-byte aligned */
+    int64_t n_blocks;
+    int64_t block_rows;
+    const int32_t* blocks;        /* [n_blocks][2], 8-byte aligned */
     int64_t n_pieces;
     const int32_t* pieces;        /* [n_pieces][4], 16-byte aligned */
 } pb_groups;
@@ -476,7 +480,8 @@ typedef struct pb_objective {
 /* sizeof of the three, so that a binding can verify its mirrors: 0 pairs, 1 groups, 2 objective. */
 int64_t pb_objective_struct_bytes(int64_t which);
 
-/* Scratch of one evaluation. */
+/* Scratch of an evaluation, 16-byte aligned.  It has to be zero when it is first used; what a call needs to be
+ * zero it leaves so.  Evaluations that may run at the same time need one each. */
 int64_t pb_objective_workspace_bytes(const pb_objective* o);
 
 /* Gradient with respect to the scores [n_rows] (of the scores' type), the loss and, for a policy, the

@@ -78,8 +78,8 @@ class Pairs(C.Structure):
     """Mirror of ``pb_pairs``."""
 
     _fields_ = [
-        ("n_rows", i64), ("n_items", i64), ("other", vp), ("offset", vp), ("weight", vp), ("chunk_rows", vp),
-        ("chunk_heads", vp), ("run_tiles", i64), ("n_cuts", i64), ("cuts", vp),
+        ("n_rows", i64), ("n_slices", i64), ("slices", vp), ("slice_rows", vp), ("n_chunks", i64), ("chunks", vp),
+        ("n_split", i64), ("other", vp), ("offset", vp), ("weight", vp),
     ]
 
 
@@ -87,8 +87,8 @@ class Groups(C.Structure):
     """Mirror of ``pb_groups``."""
 
     _fields_ = [
-        ("n_rows", i64), ("n_groups", i64), ("rows", vp), ("team_warps", i64 * 7), ("teams", vp), ("n_medium", i64),
-        ("n_large", i64), ("medium_rows", i64), ("large_rows", i64), ("held", vp), ("n_pieces", i64), ("pieces", vp),
+        ("n_rows", i64), ("n_groups", i64), ("rows", vp), ("n_team_warps", i64), ("team_warps", vp), ("teams", vp),
+        ("n_blocks", i64), ("block_rows", i64), ("blocks", vp), ("n_pieces", i64), ("pieces", vp),
     ]
 
 

@@ -2,10 +2,12 @@
 // rows of a group, and a clipped policy over groups (include/packboost_b200.h has the formulas).
 //
 // Sums over a row's pairs, over a group and over the whole table are taken in a fixed order, so a
-// result does not change from run to run.  Within a group, the log of the sum of exponentials and the
-// differences of log-probabilities are held in 64 bits: whether a policy's ratio is beyond its border
-// must not hang on the rounding of a sum over a whole era, and with a reference near the policy the
-// difference of the two log-probabilities is all there is.
+// result does not change from run to run.  The log of a group's sum of exponentials comes from 64 bits:
+// whether a policy's ratio is beyond its border must not hang on the rounding of a sum over a whole era, and
+// with a reference near the policy the difference of the two log-probabilities is all there is.
+//
+// All of it is bound by the instructions that the SMs issue, not by memory, until it is written tightly: a
+// row of a policy is 20 bytes and about a hundred instructions.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -16,7 +18,7 @@ namespace pb {
 
 namespace {
 
-// ---- scores of either type ---------------------------------------------------------------------
+// ---- scores of any type ---------------------------------------------------------------------------
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
@@ -27,51 +29,85 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// What a CTA leaves of the three totals; finish_kernel adds them up.
-struct Part {
-    double loss, kl, clipped;
-};
-
 __device__ __forceinline__ double warp_sum(double v) {
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
     return v;
 }
-
 __device__ __forceinline__ float warp_max(float v) {
     for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
     return v;
 }
 
 // The sum over the CTA, the same in every thread.  `scratch` holds a value per warp.
-__device__ __forceinline__ double block_sum(double v, double* scratch) {
+template <int THREADS>
+__device__ __forceinline__ double cta_sum(double v, double* scratch) {
     v = warp_sum(v);
     __syncthreads();  // (the scratch may still be read from the call before)
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
     __syncthreads();
-    double t = 0.0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += scratch[w];
-    return t;
+    const int k = threadIdx.x & 31;
+    return warp_sum(k < THREADS / 32 ? scratch[k] : 0.0);
 }
 
-constexpr int kFinishThreads = 512;
+// ---- launches that overlap, and the totals of an evaluation ------------------------------------------
+//
+// The kernels of one evaluation write different rows, so the next may start while one runs (its CTAs fill SMs that the
+// last of this one's leave idle); each waits for the one before it at its end, so that the last one's end is
+// everyone's.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Part* __restrict__ parts, int64_t n, double scale,
-                                                                float* loss, float* kl, int64_t* clipped) {
-    __shared__ double scratch[kFinishThreads / 32];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    Part t{0.0, 0.0, 0.0};
-    for (int64_t i = threadIdx.x; i < n; i += kFinishThreads) {
-        t.loss += parts[i].loss;
-        t.kl += parts[i].kl;
-        t.clipped += parts[i].clipped;
+// What a CTA leaves of the totals.  The CTA that leaves the last of them adds them up, in the order of their slots, and
+// resets the count: a launch only for that would take longer than the sums.
+struct Part {
+    double loss, kl, clipped;
+};
+struct Totals {
+    unsigned* ticket;  // null: not wanted
+    Part* parts;
+    int n_parts;
+    double scale;
+    float *loss, *kl;
+    int64_t* clipped;
+};
+
+template <int THREADS>
+__device__ __forceinline__ void put_totals(const Totals& out, int slot, double loss, double kl, int clipped, bool policy, double* scratch) {
+    if (!out.ticket) return;
+    __shared__ int s_last;
+    Part mine{cta_sum<THREADS>(loss, scratch), 0.0, 0.0};
+    if (policy) {
+        mine.kl = cta_sum<THREADS>(kl, scratch);
+        mine.clipped = cta_sum<THREADS>((double)clipped, scratch);
     }
-    t.loss = block_sum(t.loss, scratch);
-    t.kl = block_sum(t.kl, scratch);
-    t.clipped = block_sum(t.clipped, scratch);
+    if (out.n_parts > 1) {
+        if (threadIdx.x == 0) {
+            out.parts[slot] = mine;
+            __threadfence();  // the part is visible before the ticket is
+            s_last = atomicAdd(out.ticket, 1u) == (unsigned)out.n_parts - 1u;
+        }
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        Part t{0.0, 0.0, 0.0};
+        for (int i = threadIdx.x; i < out.n_parts; i += THREADS) {
+            t.loss += __ldcg(&out.parts[i].loss);
+            if (policy) {
+                t.kl += __ldcg(&out.parts[i].kl);
+                t.clipped += __ldcg(&out.parts[i].clipped);
+            }
+        }
+        mine.loss = cta_sum<THREADS>(t.loss, scratch);
+        if (policy) {
+            mine.kl = cta_sum<THREADS>(t.kl, scratch);
+            mine.clipped = cta_sum<THREADS>(t.clipped, scratch);
+        }
+    }
     if (threadIdx.x == 0) {
-        if (loss) *loss = (float)(t.loss * scale);
-        if (kl) *kl = (float)(t.kl * scale);
-        if (clipped) *clipped = (int64_t)t.clipped;
+        if (out.n_parts > 1) *out.ticket = 0u;
+        if (out.loss) *out.loss = (float)(mine.loss * out.scale);
+        if (out.kl) *out.kl = (float)(mine.kl * out.scale);
+        if (out.clipped) *out.clipped = (int64_t)mine.clipped;
     }
 }
 
@@ -79,257 +115,214 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const Part* __re
 
 struct PairArgs {
     pb_pairs p;
-    float beta, smoothing, half_tau;  // half_tau: 1 / (2 beta)
-    float factor;                     // of the sum of a row's terms: scale and what the terms leave out
+    float beta, beta_log2e, smoothing, half_tau;  // half_tau: 1 / (2 beta)
+    float factor;                                 // of the sum of a row's terms: scale and what the terms leave out
+    double* sums;                                 // [n_chunks]
+    unsigned* counts;                             // [n_split], 0 before and after
 };
 
-// log(1 + e) for e in [0, 1]: with s = e / (2 + e), 2 atanh(s), s <= 1/3; the term after the last one kept is
-// s^14 / 15 of the sum, below 2^-26.
-__device__ __forceinline__ float log1p_of(float e) {
-    const float s = __fdividef(e, 2.f + e), q = s * s;
-    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-    p = fmaf(q, p, 1.f / 9.f);
-    p = fmaf(q, p, 1.f / 7.f);
-    p = fmaf(q, p, 1.f / 5.f);
-    p = fmaf(q, p, 1.f / 3.f);
-    return 2.f * fmaf(s * q, p, s);
+__device__ __forceinline__ float exp2_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // Derivative with respect to d, without the factor 2 (squared) or beta, of a pair whose (reference-corrected)
-// score difference is d; its loss, if wanted.
+// score difference is d.  Of softplus(-z) + e z it is e - sigmoid(-z); the units' 2^x and 1 / x (2 and 1 ulp) are off
+// by less than 4 roundings of the slope's range.
 template <bool SQUARED>
-__device__ __forceinline__ float pair_slope(const PairArgs& a, float d, bool want, float* loss) {
-    if (SQUARED) {
-        const float off = d - a.half_tau;
-        *loss = off * off;
-        return off;
-    }
-    // softplus(-z) + e z has the derivative e - sigmoid(-z)
-    const float z = a.beta * d;
-    const float e = expf(-fabsf(z));
-    if (want) *loss = fmaxf(-z, 0.f) + log1p_of(e) + (a.smoothing != 0.f ? a.smoothing * z : 0.f);
-    return a.smoothing - __fdividef(z > 0.f ? e : 1.f, 1.f + e);
+__device__ __forceinline__ float pair_slope(const PairArgs& a, float d) {
+    if (SQUARED) return d - a.half_tau;
+    return a.smoothing - reciprocal(1.f + exp2_of(d * a.beta_log2e));
 }
 
-// A thread takes eight neighbouring items, a CTA a tile of them at a time and a run of tiles in all; a row's
-// items are neighbours, so a segmented scan over the threads gives every row its sum however many items it
-// has: rows of one pair and a row that all pairs share cost the same per item.  Rows cut by the border of
-// two runs leave a piece on either side, which pair_finish_kernel adds up in order.
-constexpr int kPairThreads = 128;
-constexpr int kPairItems = 8;
-constexpr int kPairTile = kPairThreads * kPairItems;
-static_assert(kPairTile == PB_PAIR_TILE && kPairItems == PB_PAIR_ITEMS, "layout of the items");
+// The same pair's loss, from its slope.  With h the smaller of q = sigmoid(-z) and 1 - q, softplus(-z) is max(-z, 0) -
+// log(1 - h), and -log(1 - h) = 2 atanh(h / (2 - h)), an argument of at most 1/3; the term after the last one kept is
+// s^14 / 15 of the sum, below 2^-26.
+template <bool SQUARED>
+__device__ __forceinline__ float pair_loss(const PairArgs& a, float d, float slope) {
+    if (SQUARED) return slope * slope;
+    const float z = a.beta * d, q = reciprocal(1.f + exp2_of(d * a.beta_log2e)), h = fminf(q, 1.f - q);
+    const float s = h * reciprocal(2.f - h), s2 = s * s;
+    float p = fmaf(s2, 1.f / 13.f, 1.f / 11.f);
+    p = fmaf(s2, p, 1.f / 9.f);
+    p = fmaf(s2, p, 1.f / 7.f);
+    p = fmaf(s2, p, 1.f / 5.f);
+    p = fmaf(s2, p, 1.f / 3.f);
+    p = fmaf(s2 * s, p, s);
+    const float loss = fmaf(2.f, p, fmaxf(-z, 0.f));
+    return a.smoothing != 0.f ? fmaf(a.smoothing, z, loss) : loss;
+}
 
-struct PairPieces {
-    double *lead, *tail, *loss;  // per run: sums before its first row starts and after its last one has
+// Every pair is an item of both of its rows and is evaluated for each: a row then adds up its own items, with no
+// atomics, and 4 to 12 bytes of an item are read in order; only the other row's score is looked up, mostly in L1, since rows
+// that are compared lie together.  Two rows of few items are one lane of a slice of 64 rows whose items are stored by
+// columns; rows of a slice have equal numbers of chosen and of rejected items, or nearly, because the layout
+// sorts the rows of a window by them.  So few lanes idle, and which side a column is on is the same for the whole
+// warp.  A row of many items has warps of its own, PB_CHUNK_ITEMS items each.
+constexpr int kPairThreads = 512;
+constexpr int kPairWarps = kPairThreads / 32;
+constexpr int kAhead = 4;  // columns, or 32 items of a chunk, that are asked for at once
+
+// What a lane has of a slice: two rows, their scores, their numbers of items.
+struct LaneRows {
+    float own0, own1;
+    int chosen0, end0, chosen1, end1;  // columns of the chosen side, of the rejected side from the slice's `chosen` on
+    double sum0, sum1, loss;
 };
 
+// N columns from the c0-th on.
+template <int N, typename T, bool SQUARED>
+__device__ __forceinline__ void slice_columns(const PairArgs& a, const T* __restrict__ scores, int64_t item, int c0, int chosen, bool want,
+                                              LaneRows& r) {
+    int2 o[N];
+    float2 off[N], w[N];
+    T s0[N], s1[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        // (read once: L1 is for the scores)
+        o[u] = __ldcs(reinterpret_cast<const int2*>(a.p.other + item + (c0 + u) * 64));
+        off[u] = a.p.offset ? __ldcs(reinterpret_cast<const float2*>(a.p.offset + item + (c0 + u) * 64)) : make_float2(0.f, 0.f);
+        w[u] = a.p.weight ? __ldcs(reinterpret_cast<const float2*>(a.p.weight + item + (c0 + u) * 64)) : make_float2(1.f, 1.f);
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        s0[u] = scores[o[u].x];
+        s1[u] = scores[o[u].y];
+    }
+    float p0 = 0.f, p1 = 0.f, cost = 0.f;  // (eight terms at most in 32 bits)
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int c = c0 + u;
+        const float d0 = (r.own0 - to_f32(s0[u])) - off[u].x, d1 = (r.own1 - to_f32(s1[u])) - off[u].y;
+        if (c < chosen) {
+            const float t0 = pair_slope<SQUARED>(a, d0), t1 = pair_slope<SQUARED>(a, d1);
+            if (c < r.chosen0) p0 = fmaf(w[u].x, t0, p0);
+            if (c < r.chosen1) p1 = fmaf(w[u].y, t1, p1);
+            if (want) {
+                const float l0 = pair_loss<SQUARED>(a, d0, t0), l1 = pair_loss<SQUARED>(a, d1, t1);
+                if (c < r.chosen0) cost = fmaf(w[u].x, l0, cost);
+                if (c < r.chosen1) cost = fmaf(w[u].y, l1, cost);
+            }
+        } else {
+            const float t0 = pair_slope<SQUARED>(a, -d0), t1 = pair_slope<SQUARED>(a, -d1);
+            if (c < r.end0) p0 = fmaf(-w[u].x, t0, p0);
+            if (c < r.end1) p1 = fmaf(-w[u].y, t1, p1);
+        }
+    }
+    r.sum0 += (double)p0;
+    r.sum1 += (double)p1;
+    r.loss += (double)cost;
+}
+
 template <typename T, bool SQUARED>
-__global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T* __restrict__ scores, T* __restrict__ grad,
-                                                            PairPieces pieces, double scale, float* loss_out) {
-    __shared__ double s_tail[2][kPairThreads / 32];
-    __shared__ int s_seen[2][kPairThreads / 32];
-    __shared__ double scratch[kPairThreads / 32];
-    asm volatile("griddepcontrol.launch_dependents;");
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T* __restrict__ scores, T* __restrict__ grad, Totals totals) {
+    __shared__ double scratch[kPairWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t tile0 = (int64_t)blockIdx.x * a.p.run_tiles;
-    const int64_t tile1 = min(tile0 + a.p.run_tiles, a.p.n_items / kPairTile);
-    const bool want = pieces.loss || loss_out;
-    double carry = 0.0, loss = 0.0;  // carry: of the row that is open where the tile begins
-    bool seen = false;               // a row has started in this run
-    int last_row = 0;
-    for (int64_t tile = tile0; tile < tile1; ++tile) {
-        const int64_t chunk = tile * kPairThreads + threadIdx.x, i0 = chunk * kPairItems;
-        uint32_t word[kPairItems];
-        float off[kPairItems], w[kPairItems];
-        *reinterpret_cast<uint4*>(word) = *reinterpret_cast<const uint4*>(a.p.other + i0);
-        *reinterpret_cast<uint4*>(word + 4) = *reinterpret_cast<const uint4*>(a.p.other + i0 + 4);
-        int row = a.p.chunk_rows[chunk];
-        const uint32_t heads = a.p.chunk_heads[chunk];
-        if (a.p.offset) {
-            *reinterpret_cast<float4*>(off) = *reinterpret_cast<const float4*>(a.p.offset + i0);
-            *reinterpret_cast<float4*>(off + 4) = *reinterpret_cast<const float4*>(a.p.offset + i0 + 4);
-        } else {
+    const bool want = totals.ticket != nullptr;
+    double loss = 0.0;
+    // rows of many items first: the last of a row's chunks adds up all of them while the others go on
+    const int h0 = (int)(a.p.n_chunks * blockIdx.x / gridDim.x), h1 = (int)(a.p.n_chunks * (blockIdx.x + 1) / gridDim.x);
+    for (int k = h0 + warp; k < h1; k += kPairWarps) {
+        const int4 chunk = reinterpret_cast<const int4*>(a.p.chunks)[2 * k], of = reinterpret_cast<const int4*>(a.p.chunks)[2 * k + 1];
+        const int row = chunk.x, count = chunk.z, chosen = chunk.w;
+        const int64_t begin = chunk.y;
+        const float own = to_f32(scores[row]);
+        double sum = 0.0;
+        for (int i0 = lane; i0 < count; i0 += 32 * kAhead) {
+            int o[kAhead];
+            float off[kAhead], w[kAhead];
+            T s[kAhead];
 #pragma unroll
-            for (int u = 0; u < kPairItems; ++u) off[u] = 0.f;
-        }
-        if (a.p.weight) {
-            *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(a.p.weight + i0);
-            *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(a.p.weight + i0 + 4);
-        } else {
-#pragma unroll
-            for (int u = 0; u < kPairItems; ++u) w[u] = 1.f;
-        }
-        float term[kPairItems];
-        {
-            T own[kPairItems], other[kPairItems];
-            int r = row;
-#pragma unroll
-            for (int u = 0; u < kPairItems; ++u) {
-                other[u] = scores[word[u] & 0x7FFFFFFFu];
-                if (u > 0) r += (int)((heads >> u) & 1u);
-                own[u] = scores[r];
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t i = begin + min(i0 + u * 32, count - 1);
+                o[u] = a.p.other[i];
+                off[u] = a.p.offset ? a.p.offset[i] : 0.f;
+                w[u] = a.p.weight ? a.p.weight[i] : 1.f;
             }
-            r = row;
-            float chunk_loss = 0.f;
 #pragma unroll
-            for (int u = 0; u < kPairItems; ++u) {
-                if (u > 0) r += (int)((heads >> u) & 1u);
-                const uint32_t sign = word[u] & 0x80000000u;
-                const float d = (to_f32(own[u]) - to_f32(other[u])) - off[u];
-                float l;
-                float t = pair_slope<SQUARED>(a, __uint_as_float(__float_as_uint(d) ^ sign), want, &l);
-                t = __uint_as_float(__float_as_uint(t) ^ sign) * w[u];
-                // (an item of a row with itself fills a row without pairs, or the last tile)
-                term[u] = (int)(word[u] ^ sign) != r ? t : 0.f;
-                if (want && !sign && (int)word[u] != r) chunk_loss = fmaf(w[u], l, chunk_loss);
-            }
-            loss += (double)chunk_loss;
-        }
-        const int row_open = row - (int)(heads & 1u);  // the row that is open where the chunk begins
-        float acc = 0.f, lead = 0.f;
-        bool any = false;                              // a row has started in this chunk
+            for (int u = 0; u < kAhead; ++u) s[u] = scores[o[u]];
+            float four = 0.f, four_loss = 0.f;
 #pragma unroll
-        for (int u = 0; u < kPairItems; ++u) {
-            if ((heads >> u) & 1u) {
-                if (any)
-                    grad[row] = from_f32<T>(acc * a.factor);
-                else
-                    lead = acc;
-                if (u > 0) ++row;
-                any = true;
-                acc = 0.f;
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * 32;
+                const bool better = i < chosen;
+                const float d = (own - to_f32(s[u])) - off[u], t = pair_slope<SQUARED>(a, better ? d : -d);
+                if (i < count) four = fmaf(better ? w[u] : -w[u], t, four);
+                if (want) {
+                    const float l = pair_loss<SQUARED>(a, d, t);
+                    if (better) four_loss = fmaf(w[u], l, four_loss);
+                }
             }
-            acc += term[u];
+            sum += (double)four;
+            loss += (double)four_loss;
         }
-        if (!any) lead = acc;
-
-        // inclusive scan of what is open at the end of each chunk
-        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, any);
-        const uint32_t below = mask & (0xFFFFFFFFu >> (31 - lane));
-        const int reach = below ? lane - (31 - __clz(below)) : lane;
-        double v = (double)(any ? acc : lead);
-        for (int d = 1; d < 32; d <<= 1) {
-            const double o = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            if (d <= reach) v += o;
+        sum = warp_sum(sum);
+        if (of.z == 1) {
+            if (lane == 0) grad[row] = from_f32<T>((float)sum * a.factor);
+            continue;
         }
-        const int b = (int)(tile - tile0) & 1;
-        if (lane == 31) {
-            s_tail[b][warp] = v;
-            s_seen[b][warp] = mask != 0u;
+        // one of several chunks: whoever is the last adds them up
+        int last = 0;
+        if (lane == 0) {
+            a.sums[k] = sum;
+            __threadfence();
+            last = atomicAdd(a.counts + of.x, 1u) == (unsigned)of.z - 1u;
         }
-        __syncthreads();  // (two buffers: the other one was last read before this barrier's predecessor)
-        double before = carry;  // open where this warp begins
-        bool started = seen;
-        for (int k = 0; k < warp; ++k) {
-            before = s_seen[b][k] ? s_tail[b][k] : before + s_tail[b][k];
-            started |= s_seen[b][k] != 0;
-        }
-        double open = __shfl_up_sync(0xFFFFFFFFu, v, 1);
-        if (lane == 0) open = 0.0;
-        const uint32_t prior = mask & ((1u << lane) - 1u);
-        if (!prior) open += before;
-        if (any) {
-            const double sum = open + (double)lead;
-            if (started || prior)
-                grad[row_open] = from_f32<T>((float)sum * a.factor);
-            else if (pieces.lead)   // (there are several runs)
-                pieces.lead[blockIdx.x] = sum;
-        }
-        for (int k = 0; k < kPairThreads / 32; ++k) {
-            carry = s_seen[b][k] ? s_tail[b][k] : carry + s_tail[b][k];
-            seen |= s_seen[b][k] != 0;
-        }
-        last_row = row;
-    }
-    if (threadIdx.x == kPairThreads - 1) {
-        // the row that is open at the end: done, or continued in the next run
-        const int64_t next = tile1 * kPairThreads;
-        const bool ends = tile1 == a.p.n_items / kPairTile || (a.p.chunk_heads[next] & 1u);
-        if (seen && ends) grad[last_row] = from_f32<T>((float)carry * a.factor);
-        if (pieces.lead) {
-            if (!seen) pieces.lead[blockIdx.x] = carry;
-            pieces.tail[blockIdx.x] = carry;
+        if (!__shfl_sync(0xFFFFFFFFu, last, 0)) continue;
+        __threadfence();
+        sum = 0.0;
+#pragma unroll 8
+        for (int i = lane; i < of.z; i += 32) sum += __ldcg(a.sums + of.y + i);
+        sum = warp_sum(sum);
+        if (lane == 0) {
+            grad[row] = from_f32<T>((float)sum * a.factor);
+            a.counts[of.x] = 0u;
         }
     }
-    if (want) {
-        loss = block_sum(loss, scratch);
-        if (threadIdx.x == 0) {
-            if (loss_out)  // one run: nothing else to add
-                *loss_out = (float)(loss * scale);
-            else
-                pieces.loss[blockIdx.x] = loss;
-        }
+    // neighbouring slices to one CTA: their rows are compared with the same ones
+    const int s0 = (int)(a.p.n_slices * blockIdx.x / gridDim.x), s1 = (int)(a.p.n_slices * (blockIdx.x + 1) / gridDim.x);
+    // (a slice's description is read one slice ahead)
+    const int2* slices = reinterpret_cast<const int2*>(a.p.slices);
+    const int4* slice_rows = reinterpret_cast<const int4*>(a.p.slice_rows);
+    auto describe = [&](int k) { return k < s1 ? slices[k] : make_int2(0, 0); };
+    auto rows_of = [&](int k) { return k < s1 ? slice_rows[(int64_t)k * 32 + lane] : make_int4(-1, 0, -1, 0); };
+    int2 slice = describe(s0 + warp);
+    int4 mine = rows_of(s0 + warp);
+    for (int k = s0 + warp; k < s1; k += kPairWarps) {
+        const int2 next_slice = describe(k + kPairWarps);
+        const int4 next_mine = rows_of(k + kPairWarps);
+        const int chosen = slice.y & 0xFFFF, columns = chosen + (slice.y >> 16);
+        LaneRows r;
+        r.own0 = mine.x >= 0 ? to_f32(scores[mine.x]) : 0.f;
+        r.own1 = mine.z >= 0 ? to_f32(scores[mine.z]) : 0.f;
+        r.chosen0 = mine.y & 0xFFFF;
+        r.end0 = chosen + (mine.y >> 16);
+        r.chosen1 = mine.w & 0xFFFF;
+        r.end1 = chosen + (mine.w >> 16);
+        r.sum0 = r.sum1 = 0.0;
+        r.loss = loss;
+        const int64_t item = (int64_t)slice.x * 64 + 2 * lane;
+        int c = 0;
+        for (; c + 4 <= columns; c += 4) slice_columns<4, T, SQUARED>(a, scores, item, c, chosen, want, r);
+        if (columns - c == 3)
+            slice_columns<3, T, SQUARED>(a, scores, item, c, chosen, want, r);
+        else if (columns - c == 2)
+            slice_columns<2, T, SQUARED>(a, scores, item, c, chosen, want, r);
+        else if (columns - c == 1)
+            slice_columns<1, T, SQUARED>(a, scores, item, c, chosen, want, r);
+        loss = r.loss;
+        if (mine.x >= 0) grad[mine.x] = from_f32<T>((float)r.sum0 * a.factor);
+        if (mine.z >= 0) grad[mine.z] = from_f32<T>((float)r.sum1 * a.factor);
+        slice = next_slice;
+        mine = next_mine;
     }
-}
-
-// Rows cut by borders of runs: a warp each; the loss: the last CTA.
-constexpr int kPairFinishThreads = 256;
-template <typename T>
-__global__ void __launch_bounds__(kPairFinishThreads) pair_finish_kernel(PairArgs a, PairPieces pieces, int64_t n_runs,
-                                                                         double scale, T* __restrict__ grad, float* loss_out) {
-    __shared__ double scratch[kPairFinishThreads / 32];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (blockIdx.x == gridDim.x - 1) {
-        if (!loss_out) return;
-        double t = 0.0;
-        for (int64_t i = threadIdx.x; i < n_runs; i += kPairFinishThreads) t += pieces.loss[i];
-        t = block_sum(t, scratch);
-        if (threadIdx.x == 0) *loss_out = (float)(t * scale);
-        return;
-    }
-    const int64_t k = (int64_t)blockIdx.x * (kPairFinishThreads / 32) + (threadIdx.x >> 5);
-    if (k >= a.p.n_cuts) return;
-    const int lane = threadIdx.x & 31;
-    const int row = a.p.cuts[3 * k], first = a.p.cuts[3 * k + 1], last = a.p.cuts[3 * k + 2];
-    double t = 0.0;
-    for (int r = first + 1 + lane; r <= last; r += 32) t += pieces.lead[r];
-    t = warp_sum(t) + pieces.tail[first];
-    if (lane == 0) grad[row] = from_f32<T>((float)t * a.factor);
-}
-
-// A launch; `early`: it may begin before the one in front of it on the stream has ended, and waits for that itself.
-template <typename... P, typename... A>
-cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, bool early, cudaStream_t stream, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, (P)args...);
-}
-
-int64_t n_runs_of(const pb_pairs* p) {
-    return p->n_items ? (p->n_items / kPairTile + p->run_tiles - 1) / p->run_tiles : 0;
-}
-
-template <typename T>
-int launch_pairs(const PairArgs& a, bool squared, double scale, const T* scores, T* grad, float* loss, double* scratch, cudaStream_t stream) {
-    const int64_t n_runs = n_runs_of(&a.p);
-    if (n_runs == 0) {
-        if (loss) PB_CUDA_TRY(cudaMemsetAsync(loss, 0, 4, stream));
-        return PB_OK;
-    }
-    const bool one = n_runs == 1;
-    PairPieces pieces{nullptr, nullptr, nullptr};
-    if (!one) pieces = PairPieces{scratch, scratch + n_runs, loss ? scratch + 2 * n_runs : nullptr};
-    if (squared)
-        pair_kernel<T, true><<<(unsigned)n_runs, kPairThreads, 0, stream>>>(a, scores, grad, pieces, scale, one ? loss : nullptr);
-    else
-        pair_kernel<T, false><<<(unsigned)n_runs, kPairThreads, 0, stream>>>(a, scores, grad, pieces, scale, one ? loss : nullptr);
-    count_launch(1);
-    if (!one && (loss || a.p.n_cuts)) {
-        const int64_t grid = (a.p.n_cuts + kPairFinishThreads / 32 - 1) / (kPairFinishThreads / 32) + 1;
-        PB_CUDA_TRY(launch_after(pair_finish_kernel<T>, (unsigned)grid, kPairFinishThreads, 0, true, stream, a, pieces, n_runs, scale,
-                                 grad, loss));
-        count_launch(1);
-    }
-    return PB_OK;
+    put_totals<kPairThreads>(totals, blockIdx.x, loss, 0.0, 0, false, scratch);
 }
 
 // ---- groups ---------------------------------------------------------------------------------------
@@ -345,11 +338,12 @@ struct Pair32 {  // hi + lo
     float hi, lo;
 };
 
-// a - b without rounding, plus a small `lo`
+// a - b without rounding, plus a small `lo`.  (Where hi is infinite, lo comes out as NaN and is made 1, with which
+// exp and sums still come out right; where it is above 1 by itself, hi is beyond 2^24.)
 __device__ __forceinline__ Pair32 difference(float a, float b, float lo) {
     const float t = a - b, v = t - a;
     const float err = (a - (t - v)) - (b + v);
-    return Pair32{t, fabsf(t) <= 3.402823466e38f ? err + lo : 0.f};  // (nothing to correct at infinity)
+    return Pair32{t, fminf(err + lo, 1.f)};
 }
 
 __host__ __device__ __forceinline__ Pair32 split(double x) {
@@ -362,6 +356,39 @@ __device__ __forceinline__ float exp_of(Pair32 x) {
     return fmaf(e, x.lo, e);
 }
 
+// exp(x) for x <= 0, to 7e-15 of the value and exactly 1 at 0: with n = rint(x / ln 2), 2^n times the Taylor
+// polynomial of degree 11 at |f| <= ln 2 / 2.  Below -700: 0.  (The log of the sum has to be exact to some 1e-13: a
+// divergence of nearly equal policies is a mean of differences of that size.)
+__device__ __forceinline__ double exp_negative(double x) {
+    const double shift = 6755399441055744.0;  // 1.5 * 2^52: the low word of x + shift is x as an integer
+    const double t = fma(x, 1.4426950408889634, shift);
+    const double f = fma(t - shift, -0.6931471805599453, x);
+    double p = fma(f, 1.0 / 39916800.0, 1.0 / 3628800.0);
+    p = fma(f, p, 1.0 / 362880.0);
+    p = fma(f, p, 1.0 / 40320.0);
+    p = fma(f, p, 1.0 / 5040.0);
+    p = fma(f, p, 1.0 / 720.0);
+    p = fma(f, p, 1.0 / 120.0);
+    p = fma(f, p, 1.0 / 24.0);
+    p = fma(f, p, 1.0 / 6.0);
+    p = fma(f, p, 0.5);
+    p = fma(f, p, 1.0);
+    p = fma(f, p, 1.0);
+    p *= __hiloint2double((__double2loint(t) + 1023) << 20, 0);
+    return x < -700.0 ? 0.0 : p;
+}
+
+// m + log(z), z a sum of exponentials whose largest is 1 (or 0: nothing left in the group, every p is 0; or NaN).  With y
+// the units' log2(z) times ln 2, log z = y + log(1 + w), w = z exp(-y) - 1 of some 1e-6, where four terms are exact.
+__device__ __forceinline__ double log_sum(float m, double z) {
+    float y2;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y2) : "f"((float)z));
+    const double y = (double)y2 * 0.6931471805599453;
+    const double w = fma(z, exp_negative(-y), -1.0);
+    const double l = y + w * fma(w, fma(w, fma(w, -0.25, 1.0 / 3.0), -0.5), 1.0);
+    return z == 0.0 ? 0.0 : (double)m + l;
+}
+
 struct GroupArgs {
     pb_groups g;
     const float *target, *advantage, *old, *reference;
@@ -371,483 +398,390 @@ struct GroupArgs {
     float scale;
 };
 
-struct RowInputs {
-    float main, old, reference;  // main: target, or advantage
-};
-
-// What a row has and gives: its gradient is (fixed + p * share) * scale, the share being the group's sum.
-struct RowTerm {
-    float fixed, p;
-    float share;  // what the row adds to the group's
-    float loss, kl;
-    int clipped;
-};
-
-template <int OP>
-__device__ __forceinline__ RowTerm row_term(const GroupArgs& a, float s, Pair32 lse, const RowInputs& in) {
-    RowTerm t{0.f, 0.f, 0.f, 0.f, 0.f, 0};
-    const bool live = s != -INFINITY;
-    const Pair32 l = difference(s, lse.hi, -lse.lo);
-    if (live) t.p = exp_of(l);
-    if (OP == kChoice) {
-        t.fixed = -in.main;
-        t.share = in.main;
-    } else if (live) {
-        const float adv = in.main;
-        if (adv != 0.f) {
-            const Pair32 x = difference(l.hi, in.old, l.lo);
-            const Pair32 edge = adv > 0.f ? a.log_high : a.log_low;
-            const float past = (x.hi - edge.hi) + (x.lo - edge.lo);
-            const bool beyond = adv > 0.f ? past > 0.f : past < 0.f;
-            t.loss = -adv * (beyond ? (adv > 0.f ? a.bound_high : a.bound_low) : exp_of(x));
-            t.fixed = beyond ? 0.f : t.loss;
-            t.clipped = beyond ? 1 : 0;
-        }
-        t.share = -t.fixed;
-        if (a.reference) {
-            const Pair32 gap = difference(l.hi, in.reference, l.lo);
-            t.kl = t.p * (gap.hi + gap.lo);
-            t.fixed = fmaf(a.kl_coef, t.kl, t.fixed);
-            t.share = fmaf(-a.kl_coef, t.kl, t.share);
-        }
-    }
-    return t;
+__device__ __forceinline__ float gradient_of(const GroupArgs& a, float p, float fixed, float total) {
+    return (p == 0.f ? fixed : fmaf(p, total, fixed)) * a.scale;  // (the total may be infinite)
 }
 
-__device__ __forceinline__ float row_gradient(const GroupArgs& a, float fixed, float p, float share) {
-    return (p == 0.f ? fixed : fmaf(p, share, fixed)) * a.scale;  // (the share may be infinite)
-}
-
-// What the loss of a choice gets from a row, in 64 bits: the terms of a group may be of very different size.
-__device__ __forceinline__ double choice_loss(float s, double lse, float target) {
-    return target != 0.f ? (double)target * (lse - (double)s) : 0.0;
-}
-
-__device__ __forceinline__ double log_sum(float m, double z) {
-    return z == 0.0 ? 0.0 : (double)m + log(z);  // (nothing left in the group: every p is 0)
-}
-
-// exp(s - m), 0 for a masked row
-__device__ __forceinline__ double mass_of(float s, float m) { return s == -INFINITY ? 0.0 : exp((double)s - (double)m); }
-
-// Where a CTA puts its totals; the only CTA of an evaluation puts the outputs.
-struct Totals {
-    Part* parts;  // null: not wanted
-    double scale;
-    float *loss, *kl;
-    int64_t* clipped;
-    int only;
-    float kl_coef;
-};
-__device__ __forceinline__ void put_totals(const Totals& out, int slot, double loss, double kl, double clipped) {
-    loss += (double)out.kl_coef * kl;
-    if (out.only) {
-        if (out.loss) *out.loss = (float)(loss * out.scale);
-        if (out.kl) *out.kl = (float)(kl * out.scale);
-        if (out.clipped) *out.clipped = (int64_t)clipped;
-    } else {
-        out.parts[slot] = Part{loss, kl, clipped};
-    }
-}
-// (all threads of the CTA)
-template <int OP>
-__device__ __forceinline__ void put_cta_totals(const Totals& out, int slot, double loss, double kl, int clipped, double* scratch) {
-    if (!out.parts && !out.only) return;
-    loss = block_sum(loss, scratch);
-    if (OP == kPolicy) {
-        kl = block_sum(kl, scratch);
-        const double c = block_sum((double)clipped, scratch);
-        if (threadIdx.x == 0) put_totals(out, slot, loss, kl, c);
-    } else if (threadIdx.x == 0) {
-        put_totals(out, slot, loss, 0.0, 0.0);
-    }
-}
-
-template <int OP>
-__device__ __forceinline__ RowInputs row_inputs(const GroupArgs& a, int r) {
-    RowInputs v;
-    v.main = OP == kChoice ? a.target[r] : a.advantage[r];
-    v.old = OP == kPolicy ? a.old[r] : 0.f;
-    v.reference = OP == kPolicy && a.reference ? a.reference[r] : 0.f;
-    return v;
-}
-
-// The kernels of one evaluation write different rows, so the next may start while one runs (its CTAs fill SMs that the
-// last of this one's leave idle); each waits for the one before it at its end, so that the last one's end is
-// everyone's.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// ---- short groups: lanes of a warp ----
-//
-// 1, 2, 4 ... 32 neighbouring lanes have a group, ROWS rows each; a warp's groups are of one class (so many lanes), and
-// sums over a group are shuffles within its lanes.  Of up to 4 x lanes rows at least half are there; one launch
-// takes all classes.
-constexpr int kTeamThreads = 256;
-
-template <typename T, int OP, int ROWS>
-__global__ void __launch_bounds__(kTeamThreads) team_kernel(GroupArgs a, const int2* __restrict__ teams, const int first_class,
-                                                            int64_t n_warps, int slot0, const T* __restrict__ scores,
-                                                            T* __restrict__ out, Totals totals) {
-    __shared__ double scratch[kTeamThreads / 32];
-    let_next_start();
-    const int lane = threadIdx.x & 31;
-    double loss = 0.0, kl = 0.0;
+// Up to N rows of one group that a thread has: places first, first + stride ... below end.
+template <typename T, int OP, int N>
+struct Rows {
+    const GroupArgs& a;
+    int first, stride, end;  // places
+    int used;                // rows that any thread of the warp has
+    int row[N];              // only with a list of rows
+    float s[N], main[N], old[N], reference[N];  // s becomes p, main (target or advantage) the fixed part
+    double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
-    for (int64_t w = ((int64_t)blockIdx.x * kTeamThreads + threadIdx.x) >> 5; w < n_warps; w += (int64_t)gridDim.x * (kTeamThreads / 32)) {
-        // the class of this warp, and its first team
-        int c = first_class;
-        int64_t left = w, team = 0;
-        while (left >= a.g.team_warps[c]) {
-            left -= a.g.team_warps[c];
-            team += a.g.team_warps[c] * (32 >> min(c, 5));
-            ++c;
-        }
-        c = min(c, 5);
-        const int lanes = 1 << c, me = lane & (lanes - 1);
-        const int2 group = teams[team + left * (32 >> c) + (lane >> c)];
-        int r[ROWS];
-        float s[ROWS];
-        RowInputs in[ROWS];
+
+    __device__ __forceinline__ Rows(const GroupArgs& args) : a(args) {}
+
+    __device__ __forceinline__ bool has(int u) const { return first + u * stride < end; }
+    __device__ __forceinline__ int row_of(int u) const { return a.g.rows ? row[u] : first + u * stride; }
+    // (half of the rows are there more often than not: only the others are worth a branch)
+    __device__ __forceinline__ bool on(int u) const { return u < N / 2 || u < used; }
+
+    // Everything is asked for before anything is used.
+    __device__ __forceinline__ void load(const T* scores, bool inputs) {
+        T raw[N];
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            const int i = u * lanes + me;
-            r[u] = i < group.y ? group.x + i : -1;
-            if (a.g.rows && r[u] >= 0) r[u] = a.g.rows[r[u]];
-        }
+        for (int u = 0; u < N; ++u)
+            if (on(u) && a.g.rows && has(u)) row[u] = a.g.rows[first + u * stride];
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            s[u] = -INFINITY;
-            in[u] = RowInputs{0.f, 0.f, 0.f};
-            if (r[u] >= 0) {
-                s[u] = to_f32(scores[r[u]]);
-                if (OP != kLogProbs) in[u] = row_inputs<OP>(a, r[u]);
+        for (int u = 0; u < N; ++u)
+            if (on(u) && has(u)) raw[u] = scores[row_of(u)];
+        if (OP != kLogProbs && inputs) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                main[u] = old[u] = reference[u] = 0.f;
+                if (on(u) && has(u)) {
+                    const int r = row_of(u);
+                    main[u] = OP == kChoice ? a.target[r] : a.advantage[r];
+                    if (OP == kPolicy) {
+                        old[u] = a.old[r];
+                        if (a.reference) reference[u] = a.reference[r];
+                    }
+                }
             }
         }
+#pragma unroll
+        for (int u = 0; u < N; ++u) s[u] = on(u) && has(u) ? to_f32(raw[u]) : -INFINITY;
+    }
+
+    __device__ __forceinline__ float largest() const {
         float m = s[0];
 #pragma unroll
-        for (int u = 1; u < ROWS; ++u) m = fmaxf(m, s[u]);
-        for (int d = lanes >> 1; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+        for (int u = 1; u < N; ++u) m = fmaxf(m, s[u]);
+        return m;
+    }
+
+    // Sum of exp(s - m).  (m = -inf: no row is left, all of them add exp(-inf) to 0.)
+    __device__ __forceinline__ double mass(float m) const {
+        const double top = m == -INFINITY ? 0.0 : (double)m;
         double z = 0.0;
 #pragma unroll
-        for (int u = 0; u < ROWS; ++u) z += mass_of(s[u], m);
-        for (int d = lanes >> 1; d > 0; d >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, d);
-        const double lse64 = log_sum(m, z);
+        for (int u = 0; u < N; ++u)
+            if (on(u)) z += exp_negative((double)s[u] - top);
+        return z;
+    }
+
+    // With the log of the group's sum: p, the part of the gradient that does not hang on the rest of the group, and what
+    // goes into the sums.  A row's gradient is (fixed + p * share) * scale: of a choice -t + p * sum t, of a policy, with h
+    // the slopes of the taken rows and D the divergence, h + p (k (l - reference - D) - sum h).
+    __device__ __forceinline__ void terms(double lse64) {
         const Pair32 lse = split(lse64);
-        if (OP == kLogProbs) {
+        float part = 0.f, part_loss = 0.f, part_kl = 0.f;
 #pragma unroll
-            for (int u = 0; u < ROWS; ++u)
-                if (r[u] >= 0) {
-                    const Pair32 l = difference(s[u], lse.hi, -lse.lo);
-                    out[r[u]] = from_f32<T>(l.hi + l.lo);
+        for (int u = 0; u < N; ++u) {
+            if (on(u)) {
+                const bool live = s[u] != -INFINITY;
+                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
+                const float p = live ? exp_of(l) : 0.f;
+                float fixed, own;
+                if (OP == kChoice) {
+                    const float t = main[u];
+                    if (t != 0.f) loss += (double)t * (lse64 - (double)s[u]);  // (in 64 bits: terms may be of very different size)
+                    fixed = -t;
+                    own = t;
+                } else {
+                    const float adv = live ? main[u] : 0.f;
+                    const bool up = adv > 0.f, taken = adv != 0.f;
+                    const Pair32 x = difference(l.hi, old[u], l.lo);
+                    const float past = (x.hi - (up ? a.log_high.hi : a.log_low.hi)) + (x.lo - (up ? a.log_high.lo : a.log_low.lo));
+                    const bool beyond = taken && (up ? past > 0.f : past < 0.f);
+                    const float cost = -adv * (beyond ? (up ? a.bound_high : a.bound_low) : exp_of(x));
+                    fixed = taken && !beyond ? cost : 0.f;
+                    part_loss += taken ? cost : 0.f;
+                    clipped += beyond ? 1 : 0;
+                    own = -fixed;
+                    if (a.reference) {
+                        const Pair32 gap = difference(l.hi, reference[u], l.lo);
+                        const float k = live ? p * (gap.hi + gap.lo) : 0.f;
+                        fixed = fmaf(a.kl_coef, k, fixed);
+                        own = fmaf(-a.kl_coef, k, own);
+                        part_kl += k;
+                    }
                 }
-            continue;
-        }
-        float fixed[ROWS], part = 0.f, part_loss = 0.f, part_kl = 0.f;
-        double part64 = 0.0;
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) {
-            if (r[u] >= 0) {
-                if (OP == kChoice) loss += choice_loss(s[u], lse64, in[u].main);
-                const RowTerm t = row_term<OP>(a, s[u], lse, in[u]);
-                s[u] = t.p;
-                fixed[u] = t.fixed;
-                part += t.share;
-                part_loss += t.loss;
-                part_kl += t.kl;
-                clipped += t.clipped;
+                part += own;
+                s[u] = p;
+                main[u] = fixed;
             }
-            if ((u & 3) == 3) {  // (four terms in 32 bits, the sums of fours in 64)
-                part64 += (double)part;
+            if ((u & 3) == 3 && on(u - 3)) {  // (four terms in 32 bits, the sums of fours in 64)
+                share += (double)part;
                 if (OP == kPolicy) {
-                    loss += (double)part_loss;
+                    loss += (double)part_loss + (double)a.kl_coef * (double)part_kl;
                     kl += (double)part_kl;
                 }
                 part = part_loss = part_kl = 0.f;
             }
         }
-        for (int d = lanes >> 1; d > 0; d >>= 1) part64 += __shfl_xor_sync(0xFFFFFFFFu, part64, d);
-        const float share = (float)part64;
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-            if (r[u] >= 0) out[r[u]] = from_f32<T>(row_gradient(a, fixed[u], s[u], share));
     }
-    if (OP != kLogProbs) put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
+
+    __device__ __forceinline__ void gradient(float total, T* out) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (on(u) && has(u))
+                out[row_of(u)] = from_f32<T>(gradient_of(a, s[u], main[u], total));
+    }
+
+    __device__ __forceinline__ void log_probs(double lse64, T* out) const {
+        const Pair32 lse = split(lse64);
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (on(u) && has(u)) {
+                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
+                out[row_of(u)] = from_f32<T>(l.hi + l.lo);
+            }
+    }
+};
+
+// The sums of several threads into one: z is relative to m.
+__device__ __forceinline__ double rescaled(double z, float m, float top) {
+    return z == 0.0 ? 0.0 : z * exp_negative((double)m - (double)top);
+}
+
+// ---- short groups: lanes of a warp ----
+//
+// 1, 2, 4 ... 32 neighbouring lanes have a group, up to eight rows each; the groups of a warp have equal lengths, or nearly,
+// because the layout sorts them by length; sums over a group are shuffles within its lanes.
+constexpr int kTeamThreads = 256;
+constexpr int kTeamRows = PB_TEAM_ROWS / 32;
+
+template <typename T, int OP>
+__global__ void __launch_bounds__(kTeamThreads) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
+                                                            Totals totals) {
+    __shared__ double scratch[kTeamThreads / 32];
+    let_next_start();
+    const int lane = threadIdx.x & 31;
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0;
+    for (int w = (blockIdx.x * kTeamThreads + threadIdx.x) >> 5; w < (int)a.g.n_team_warps; w += gridDim.x * (kTeamThreads / 32)) {
+        const int2 what = reinterpret_cast<const int2*>(a.g.team_warps)[w];  // first team; class and rows of a lane
+        const int shift = what.y & 0xFF, lanes = 1 << shift;
+        const int2 group = reinterpret_cast<const int2*>(a.g.teams)[what.x + (lane >> shift)];
+        Rows<T, OP, kTeamRows> rows(a);
+        rows.first = group.x + (lane & (lanes - 1));
+        rows.stride = lanes;
+        rows.end = group.x + group.y;
+        rows.used = what.y >> 8;
+        rows.load(scores, true);
+        float m = rows.largest();
+        for (int d = lanes >> 1; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+        double z = rows.mass(m);
+        for (int d = lanes >> 1; d > 0; d >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, d);
+        const double lse = log_sum(m, z);
+        if (OP == kLogProbs) {
+            rows.log_probs(lse, out);
+            continue;
+        }
+        rows.terms(lse);
+        double share = rows.share;
+        for (int d = lanes >> 1; d > 0; d >>= 1) share += __shfl_xor_sync(0xFFFFFFFFu, share, d);
+        rows.gradient((float)share, out);
+        loss += rows.loss;
+        kl += rows.kl;
+        clipped += rows.clipped;
+    }
+    if (OP != kLogProbs) put_totals<kTeamThreads>(totals, slot0 + blockIdx.x, loss, kl, clipped, OP == kPolicy, scratch);
     wait_for_previous();
 }
 
-// ---- groups that a CTA holds ----
+// ---- longer groups: a CTA ----
 //
-// The rows of a group stay in the shared memory of one CTA, each thread using the words it filled itself: the
-// inputs that the gradient needs are on their way there (cp.async) while the scores are summed.
-__device__ __forceinline__ void copy_word(float* to, const float* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from));
-}
-
-// Largest score and log of the sum of exponentials over the CTA, from the threads' own ones.
+// The scores are gone through twice, the second time from L1; p and the fixed part of the gradient stay in shared memory for
+// the third step, so that the other inputs are read once.  Few threads with many rows each: what a warp does per group (sums
+// over its lanes, the log) is as much as five rows.
 template <int THREADS>
 __device__ __forceinline__ double cta_log_sum(float m, double z, float* s_m, double* s_z) {
-    float wm = warp_max(m);
-    z = z == 0.0 ? 0.0 : z * exp((double)m - (double)wm);
-    z = warp_sum(z);
-    if ((threadIdx.x & 31) == 0) {
+    const int lane = threadIdx.x & 31;
+    const float wm = warp_max(m);
+    z = warp_sum(rescaled(z, m, wm));
+    if (lane == 0) {
         s_m[threadIdx.x >> 5] = wm;
         s_z[threadIdx.x >> 5] = z;
     }
     __syncthreads();
-    constexpr int kWarps = THREADS / 32;
-    const int k = threadIdx.x & 31;
-    wm = k < kWarps ? s_m[k] : -INFINITY;
-    z = k < kWarps ? s_z[k] : 0.0;
-    const float all = warp_max(wm);
-    z = z == 0.0 ? 0.0 : z * exp((double)wm - (double)all);
-    return log_sum(all, warp_sum(z));
+    m = lane < THREADS / 32 ? s_m[lane] : -INFINITY;
+    z = lane < THREADS / 32 ? s_z[lane] : 0.0;
+    const float top = warp_max(m);
+    return log_sum(top, warp_sum(rescaled(z, m, top)));
 }
 
-template <int THREADS>
-__device__ __forceinline__ double cta_sum(double v, double* scratch) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    const int k = threadIdx.x & 31;
-    return warp_sum(k < THREADS / 32 ? scratch[k] : 0.0);
-}
+constexpr int kBlockRows = 4;  // of a thread at a time
 
 template <typename T, int OP, int THREADS>
-__global__ void __launch_bounds__(THREADS) held_kernel(GroupArgs a, const int2* __restrict__ list, int most, int slot0,
-                                                       const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
-    extern __shared__ float held[];  // scores (then p) | main (then fixed) | old | reference, `most` each
+__global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2* __restrict__ list, int slot0,
+                                                        const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
+    extern __shared__ float2 kept[];
     __shared__ float s_m[THREADS / 32];
     __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
     let_next_start();
     const int2 group = list[blockIdx.x];
-    const int begin = group.x, n = group.y;
-    float* const h_main = held + most;
-    float* const h_old = held + 2 * most;
-    float* const h_ref = held + 3 * most;
-    auto row_of = [&](int i) { return a.g.rows ? a.g.rows[begin + i] : begin + i; };
-    if (OP != kLogProbs) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const int r = row_of(i);
-            copy_word(h_main + i, (OP == kChoice ? a.target : a.advantage) + r);
-            if (OP == kPolicy) {
-                copy_word(h_old + i, a.old + r);
-                if (a.reference) copy_word(h_ref + i, a.reference + r);
-            }
-        }
-        asm volatile("cp.async.commit_group;");
-    }
+    constexpr int kStep = THREADS * kBlockRows;
+    auto rows_at = [&](auto& rows, int i0) {
+        rows.first = group.x + i0 + (int)threadIdx.x;
+        rows.stride = THREADS;
+        rows.end = group.x + group.y;
+        rows.used = (group.y - i0 + THREADS - 1) / THREADS;
+    };
     float m = -INFINITY;
-    {
-        constexpr int kAhead = 8;
-        for (int i0 = threadIdx.x; i0 < n; i0 += THREADS * kAhead) {
-            float v[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int i = i0 + u * THREADS;
-                v[u] = i < n ? to_f32(scores[row_of(i)]) : -INFINITY;
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int i = i0 + u * THREADS;
-                m = fmaxf(m, v[u]);
-                if (i < n) held[i] = v[u];
-            }
-        }
-    }
     double z = 0.0;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += THREADS) z += mass_of(held[i], m);
-    const double lse64 = cta_log_sum<THREADS>(m, z, s_m, s_z);
-    const Pair32 lse = split(lse64);
+    for (int i0 = 0; i0 < group.y; i0 += kStep) {
+        Rows<T, OP, kBlockRows> rows(a);
+        rows_at(rows, i0);
+        rows.load(scores, false);
+        const float top = fmaxf(m, rows.largest());
+        z = rescaled(z, m, top) + rows.mass(top);
+        m = top;
+    }
+    const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
     if (OP == kLogProbs) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const Pair32 l = difference(held[i], lse.hi, -lse.lo);
-            out[row_of(i)] = from_f32<T>(l.hi + l.lo);
+        for (int i0 = 0; i0 < group.y; i0 += kStep) {
+            Rows<T, OP, kBlockRows> rows(a);
+            rows_at(rows, i0);
+            rows.load(scores, false);
+            rows.log_probs(lse, out);
         }
         wait_for_previous();
         return;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    double part = 0.0, loss = 0.0, kl = 0.0;
+    double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
-    for (int i0 = threadIdx.x; i0 < n; i0 += THREADS * 4) {
-        float p4 = 0.f, l4 = 0.f, k4 = 0.f;
+    for (int i0 = 0; i0 < group.y; i0 += kStep) {
+        Rows<T, OP, kBlockRows> rows(a);
+        rows_at(rows, i0);
+        rows.load(scores, true);
+        rows.terms(lse);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * THREADS;
-            if (i < n) {
-                const float s = held[i];
-                const RowInputs in{h_main[i], OP == kPolicy ? h_old[i] : 0.f, OP == kPolicy && a.reference ? h_ref[i] : 0.f};
-                if (OP == kChoice) loss += choice_loss(s, lse64, in.main);
-                const RowTerm t = row_term<OP>(a, s, lse, in);
-                held[i] = t.p;
-                h_main[i] = t.fixed;
-                p4 += t.share;
-                l4 += t.loss;
-                k4 += t.kl;
-                clipped += t.clipped;
-            }
+        for (int u = 0; u < kBlockRows; ++u) {
+            const int i = i0 + u * THREADS + threadIdx.x;
+            if (i < group.y) kept[i] = make_float2(rows.s[u], rows.main[u]);
         }
-        part += (double)p4;
-        if (OP == kPolicy) {
-            loss += (double)l4;
-            kl += (double)k4;
-        }
+        loss += rows.loss;
+        kl += rows.kl;
+        share += rows.share;
+        clipped += rows.clipped;
     }
-    const float share = (float)cta_sum<THREADS>(part, scratch);
+    const float total = (float)cta_sum<THREADS>(share, scratch);
 #pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += THREADS) out[row_of(i)] = from_f32<T>(row_gradient(a, h_main[i], held[i], share));
-    put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
+    for (int i = threadIdx.x; i < group.y; i += THREADS) {
+        const float2 v = kept[i];
+        const int r = a.g.rows ? a.g.rows[group.x + i] : group.x + i;
+        out[r] = from_f32<T>(gradient_of(a, v.x, v.y, total));
+    }
+    put_totals<THREADS>(totals, slot0 + blockIdx.x, loss, kl, clipped, OP == kPolicy, scratch);
     wait_for_previous();
 }
 
 // ---- long groups: many CTAs each ----
 //
-// Pieces of PB_PIECE_ROWS rows; the sums of a group's pieces go through memory from one launch to the next: sums of
-// exponentials, then shares, then the gradient.  The rows are read again each time, from L2 mostly.
+// Pieces of up to 2048 rows; the sums of a group's pieces go through memory from one launch to the next: sums of
+// exponentials, then shares, then the gradient.  The rows are read again each time, from L2 mostly, while the launch
+// before still runs.
 struct PieceSums {
     double z, share;
     float m, unused;
 };
-constexpr int kPieceThreads = 512;
-constexpr int kPieceRows = PB_PIECE_ROWS / kPieceThreads;
 enum PieceStep { kPieceMass, kPieceTerms, kPieceOut };
+constexpr int kPieceThreads = 256;
+constexpr int kPieceRows = PB_PIECE_ROWS / kPieceThreads;
 
 template <typename T, int OP, int STEP>
 __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, PieceSums* __restrict__ pieces, int slot0,
                                                               const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
-    constexpr int THREADS = kPieceThreads, ROWS = kPieceRows;
-    __shared__ float s_m[THREADS / 32];
-    __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
+    constexpr int kWarps = kPieceThreads / 32;
+    __shared__ float s_m[kWarps];
+    __shared__ double s_z[kWarps], scratch[kWarps];
     let_next_start();
-    if (STEP == kPieceMass) wait_for_previous();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 piece = reinterpret_cast<const int4*>(a.g.pieces)[blockIdx.x];
-    const int begin = piece.x, n = piece.y, first = piece.z, count = piece.w;  // (first, count: the group's pieces)
-    int r[ROWS];
-    float s[ROWS];
-    RowInputs in[ROWS];
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        const int i = u * THREADS + threadIdx.x;
-        r[u] = i < n ? begin + i : -1;
-        if (a.g.rows && r[u] >= 0) r[u] = a.g.rows[r[u]];
-    }
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        s[u] = -INFINITY;
-        if (r[u] >= 0) {
-            s[u] = to_f32(scores[r[u]]);
-            if (OP != kLogProbs && STEP != kPieceMass) in[u] = row_inputs<OP>(a, r[u]);
-        }
-    }
-    float m = -INFINITY;
-    double z = 0.0;
+    const int first = piece.z, count = piece.w;  // the group's pieces
+    Rows<T, OP, kPieceRows> rows(a);
+    rows.first = piece.x + threadIdx.x;
+    rows.stride = kPieceThreads;
+    rows.end = piece.x + piece.y;
+    rows.used = (piece.y + kPieceThreads - 1) / kPieceThreads;
+    rows.load(scores, STEP != kPieceMass);
     if (STEP == kPieceMass) {
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) m = fmaxf(m, s[u]);
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u) z += mass_of(s[u], m);
+        float m = rows.largest();
         const float wm = warp_max(m);
-        z = warp_sum(z == 0.0 ? 0.0 : z * exp((double)m - (double)wm));
-        if ((threadIdx.x & 31) == 0) {
-            s_m[threadIdx.x >> 5] = wm;
-            s_z[threadIdx.x >> 5] = z;
+        double z = warp_sum(rows.mass(wm));
+        if (lane == 0) {
+            s_m[warp] = wm;
+            s_z[warp] = z;
         }
         __syncthreads();
-        if (threadIdx.x < 32) {
-            const float k = threadIdx.x < THREADS / 32 ? s_m[threadIdx.x] : -INFINITY;
-            z = threadIdx.x < THREADS / 32 ? s_z[threadIdx.x] : 0.0;
-            m = warp_max(k);
-            z = warp_sum(z == 0.0 ? 0.0 : z * exp((double)k - (double)m));
-            if (threadIdx.x == 0) {
-                pieces[blockIdx.x].m = m;
+        if (warp == 0) {
+            m = lane < kWarps ? s_m[lane] : -INFINITY;
+            z = lane < kWarps ? s_z[lane] : 0.0;
+            const float top = warp_max(m);
+            z = warp_sum(rescaled(z, m, top));
+            if (lane == 0) {
+                pieces[blockIdx.x].m = top;
                 pieces[blockIdx.x].z = z;
             }
         }
+        wait_for_previous();
         return;
     }
-    wait_for_previous();   // (the rows' inputs do not come from the launch before, the sums do)
-    for (int k = threadIdx.x; k < count; k += THREADS) m = fmaxf(m, pieces[first + k].m);
-    for (int k = threadIdx.x; k < count; k += THREADS) {
-        const double zk = pieces[first + k].z;
-        if (zk != 0.0) z += zk * exp((double)pieces[first + k].m - (double)m);
+    wait_for_previous();  // (the rows do not come from the launch before, the sums do)
+    float m = -INFINITY;
+    double z = 0.0;
+    for (int k = threadIdx.x; k < count; k += kPieceThreads) {
+        const float mk = pieces[first + k].m, top = fmaxf(m, mk);
+        z = rescaled(z, m, top) + rescaled(pieces[first + k].z, mk, top);
+        m = top;
     }
-    const double lse64 = cta_log_sum<THREADS>(m, z, s_m, s_z);
-    const Pair32 lse = split(lse64);
+    const double lse = cta_log_sum<kPieceThreads>(m, z, s_m, s_z);
     if (OP == kLogProbs) {
-#pragma unroll
-        for (int u = 0; u < ROWS; ++u)
-            if (r[u] >= 0) {
-                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
-                out[r[u]] = from_f32<T>(l.hi + l.lo);
-            }
+        rows.log_probs(lse, out);
         return;
     }
-    float share = 0.f;
-    if (STEP == kPieceOut) {
-        double sum = 0.0;
-        for (int k = threadIdx.x; k < count; k += THREADS) sum += pieces[first + k].share;
-        share = (float)cta_sum<THREADS>(sum, scratch);
-    }
-    double part = 0.0, loss = 0.0, kl = 0.0;
-    int clipped = 0;
-    float p4 = 0.f, l4 = 0.f, k4 = 0.f;
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-        if (r[u] >= 0) {
-            const RowTerm t = row_term<OP>(a, s[u], lse, in[u]);
-            if (STEP == kPieceOut) {
-                out[r[u]] = from_f32<T>(row_gradient(a, t.fixed, t.p, share));
-            } else {
-                if (OP == kChoice) loss += choice_loss(s[u], lse64, in[u].main);
-                p4 += t.share;
-                l4 += t.loss;
-                k4 += t.kl;
-                clipped += t.clipped;
-            }
-        }
-        if (STEP == kPieceTerms && (u & 3) == 3) {
-            part += (double)p4;
-            if (OP == kPolicy) {
-                loss += (double)l4;
-                kl += (double)k4;
-            }
-            p4 = l4 = k4 = 0.f;
-        }
-    }
+    rows.terms(lse);
     if (STEP == kPieceTerms) {
-        part = cta_sum<THREADS>(part, scratch);
-        if (threadIdx.x == 0) pieces[blockIdx.x].share = part;
-        put_cta_totals<OP>(totals, slot0 + blockIdx.x, loss, kl, clipped, scratch);
+        const double share = cta_sum<kPieceThreads>(rows.share, scratch);
+        if (threadIdx.x == 0) pieces[blockIdx.x].share = share;
+        put_totals<kPieceThreads>(totals, slot0 + blockIdx.x, rows.loss, rows.kl, rows.clipped, OP == kPolicy, scratch);
+        return;
     }
+    double share = 0.0;
+    for (int k = threadIdx.x; k < count; k += kPieceThreads) share += pieces[first + k].share;
+    rows.gradient((float)cta_sum<kPieceThreads>(share, scratch), out);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
 
+constexpr int64_t kMost = (1ll << 31) - 1;
+
 int check_groups(const pb_groups* g) {
     PB_REQUIRE(g != nullptr, "groups are null");
-    PB_REQUIRE(g->n_rows >= 0 && g->n_rows < (1ll << 31) - 1, "n_rows=%lld out of range", (long long)g->n_rows);
+    PB_REQUIRE(g->n_rows >= 0 && g->n_rows < kMost, "n_rows=%lld out of range", (long long)g->n_rows);
     PB_REQUIRE(g->n_groups >= 0 && g->n_groups <= g->n_rows, "n_groups=%lld out of range", (long long)g->n_groups);
     PB_REQUIRE((g->n_groups == 0) == (g->n_rows == 0), "rows without a group");
-    const int64_t most = (1ll << 31) - 1;
-    int64_t warps = 0;
-    for (int c = 0; c < 7; ++c) {
-        PB_REQUIRE(g->team_warps[c] >= 0 && g->team_warps[c] < most, "team_warps[%d] is out of range", c);
-        warps += g->team_warps[c];
-    }
-    PB_REQUIRE(g->n_medium >= 0 && g->n_large >= 0 && g->n_medium + g->n_large <= g->n_groups && g->n_pieces >= 0 && g->n_pieces < most,
+    PB_REQUIRE(g->n_team_warps >= 0 && g->n_team_warps < kMost / 32 && g->n_pieces >= 0 && g->n_pieces < kMost && g->n_blocks >= 0 &&
+                   g->n_blocks <= g->n_groups,
                "counts of the groups' layout are out of range");
-    PB_REQUIRE(g->n_medium == 0 || (g->medium_rows > 0 && g->medium_rows <= PB_MEDIUM_ROWS), "medium_rows is out of range");
-    PB_REQUIRE(g->n_large == 0 || (g->large_rows > 0 && g->large_rows <= PB_LARGE_ROWS), "large_rows is out of range");
-    PB_REQUIRE((warps == 0 || g->teams) && (g->n_medium + g->n_large == 0 || g->held) && (g->n_pieces == 0 || g->pieces),
+    PB_REQUIRE(g->n_blocks == 0 || (g->block_rows > 0 && g->block_rows <= PB_BLOCK_ROWS), "block_rows is out of range");
+    PB_REQUIRE((g->n_team_warps == 0 || (g->team_warps && g->teams)) && (g->n_blocks == 0 || g->blocks) && (g->n_pieces == 0 || g->pieces),
                "a table of the groups' layout is null");
-    PB_REQUIRE((uintptr_t)g->teams % 8 == 0 && (uintptr_t)g->held % 8 == 0 && (uintptr_t)g->pieces % 16 == 0,
+    PB_REQUIRE((uintptr_t)g->team_warps % 8 == 0 && (uintptr_t)g->teams % 8 == 0 && (uintptr_t)g->blocks % 8 == 0 && (uintptr_t)g->pieces % 16 == 0,
                "tables of the groups' layout must be aligned");
-    PB_REQUIRE(g->n_groups == 0 || warps + g->n_medium + g->n_large + g->n_pieces > 0, "the groups are not laid out");
+    PB_REQUIRE(g->n_groups == 0 || g->n_team_warps + g->n_blocks + g->n_pieces > 0, "the groups are not laid out");
+    return PB_OK;
+}
+
+int check_pairs(const pb_pairs* p) {
+    PB_REQUIRE(p != nullptr, "pairs are null");
+    PB_REQUIRE(p->n_rows >= 0 && p->n_rows < kMost, "n_rows=%lld out of range", (long long)p->n_rows);
+    PB_REQUIRE(p->n_slices >= 0 && p->n_slices < kMost / 64 && p->n_chunks >= 0 && p->n_chunks < kMost && p->n_split >= 0 &&
+                   2 * p->n_split <= p->n_chunks,
+               "counts of the pairs' layout are out of range");
+    PB_REQUIRE(p->n_rows == 0 || p->n_slices + p->n_chunks > 0, "the pairs are not laid out");
+    PB_REQUIRE((p->n_slices == 0 || (p->slices && p->slice_rows)) && (p->n_chunks == 0 || p->chunks) && (p->n_rows == 0 || p->other),
+               "a table of the pairs' layout is null");
+    PB_REQUIRE((uintptr_t)p->slices % 8 == 0 && (uintptr_t)p->slice_rows % 16 == 0 && (uintptr_t)p->chunks % 16 == 0,
+               "tables of the pairs' layout must be aligned");
+    PB_REQUIRE((uintptr_t)p->other % 8 == 0 && (uintptr_t)p->offset % 8 == 0 && (uintptr_t)p->weight % 8 == 0,
+               "items must be 8-byte aligned");
     return PB_OK;
 }
 
@@ -855,16 +789,7 @@ int check_objective(const pb_objective* o) {
     PB_REQUIRE(o != nullptr, "objective is null");
     PB_REQUIRE(isfinite(o->scale), "scale is not finite");
     if (o->kind == PB_OBJECTIVE_PREFERENCE) {
-        const pb_pairs* p = o->pairs;
-        PB_REQUIRE(p != nullptr, "pairs are null");
-        PB_REQUIRE(p->n_rows >= 0 && p->n_rows < (1ll << 31) - 1, "n_rows=%lld out of range", (long long)p->n_rows);
-        PB_REQUIRE(p->n_items >= 0 && p->n_items < (1ll << 31) - 1, "n_items=%lld out of range", (long long)p->n_items);
-        PB_REQUIRE(p->n_items % kPairTile == 0 && (p->n_items == 0) == (p->n_rows == 0), "items are not laid out in tiles");
-        PB_REQUIRE(p->n_items == 0 || (p->other && p->chunk_rows && p->chunk_heads && p->run_tiles >= 1),
-                   "a table of the pairs' layout is null");
-        PB_REQUIRE(p->n_cuts >= 0 && p->n_cuts <= p->n_items / kPairTile && (p->n_cuts == 0 || p->cuts), "cuts of the pairs' layout");
-        PB_REQUIRE((uintptr_t)p->other % 16 == 0 && (uintptr_t)p->offset % 16 == 0 && (uintptr_t)p->weight % 16 == 0,
-                   "items must be 16-byte aligned");
+        PB_TRY(check_pairs(o->pairs));
         PB_REQUIRE(o->beta > 0.0 && isfinite(o->beta), "beta must be positive");
         PB_REQUIRE(o->smoothing >= 0.0 && o->smoothing < 0.5, "smoothing outside [0, 0.5)");
         return PB_OK;
@@ -887,123 +812,149 @@ int64_t n_rows_of(const pb_objective* o) {
     return o->kind == PB_OBJECTIVE_PREFERENCE ? o->pairs->n_rows : o->groups->n_rows;
 }
 
-// CTAs of the launch that takes all warps of short groups: what the SMs hold at once, or as many as there are warps.
-constexpr int64_t kTeamGrid = 148 * 6;
-int64_t team_grid(int64_t warps) { return warps == 0 ? 0 : warps / 8 + 1 < kTeamGrid ? (warps + 7) / 8 : kTeamGrid; }
-int64_t team_warps(const pb_groups* g, int from, int to) {
-    int64_t n = 0;
-    for (int c = from; c < to; ++c) n += g->team_warps[c];
-    return n;
+// CTAs of a launch whose warps take one task after the other: what the SMs hold at once, or as many as there are tasks.
+constexpr int64_t kWarpGrid = 148 * 4;
+int64_t warp_grid(int64_t warps) { return warps / 8 < kWarpGrid ? (warps + 7) / 8 : kWarpGrid; }
+
+// (two CTAs per SM: with more, of which each looks up scores in another window of rows, L1 holds too little of each)
+int64_t n_parts_of(const pb_pairs* p) {
+    const int64_t tasks = p->n_slices > p->n_chunks ? p->n_slices : p->n_chunks;
+    return tasks < 148 * 2 * kPairWarps ? (tasks + kPairWarps - 1) / kPairWarps : 148 * 2;
+}
+int64_t n_parts_of(const pb_groups* g) {
+    return warp_grid(g->n_team_warps) + g->n_blocks + g->n_pieces;
 }
 
-int64_t n_group_parts(const pb_groups* g) {
-    return team_grid(team_warps(g, 0, 6)) + team_grid(g->team_warps[6]) + g->n_medium + g->n_large + g->n_pieces;
-}
-
-// Scratch: the sums of pieces, then what the CTAs leave of the totals, if there are several.
-int64_t group_scratch_bytes(const pb_groups* g, bool totals) {
-    const int64_t n = n_group_parts(g);
-    return (totals && n > 1 ? n * (int64_t)sizeof(Part) : 0) + g->n_pieces * (int64_t)sizeof(PieceSums);
+// Scratch: the ticket; of pairs, counts and sums of the rows in several chunks; of groups, the sums of pieces; the totals.
+constexpr int64_t kTicketBytes = 16;
+int64_t sums_bytes(const pb_pairs* p) { return (int64_t)align_up((size_t)p->n_split * 4, 8) + (p->n_split ? p->n_chunks * 8 : 0); }
+int64_t sums_bytes(const pb_groups* g) { return g->n_pieces * (int64_t)sizeof(PieceSums); }
+template <typename L>
+int64_t scratch_bytes(const L* layout) {
+    return kTicketBytes + sums_bytes(layout) + n_parts_of(layout) * (int64_t)sizeof(Part);
 }
 int64_t scratch_bytes(const pb_objective* o) {
-    if (o->kind == PB_OBJECTIVE_PREFERENCE) return n_runs_of(o->pairs) > 1 ? 3 * n_runs_of(o->pairs) * (int64_t)sizeof(double) : 0;
-    return group_scratch_bytes(o->groups, true);
+    return o->kind == PB_OBJECTIVE_PREFERENCE ? scratch_bytes(o->pairs) : scratch_bytes(o->groups);
+}
+template <typename L>
+Totals totals_of(const L* layout, double scale, float* loss, float* kl, int64_t* clipped, char* scratch) {
+    const bool want = loss || kl || clipped;
+    return Totals{want ? reinterpret_cast<unsigned*>(scratch) : nullptr, reinterpret_cast<Part*>(scratch + kTicketBytes + sums_bytes(layout)),
+                  (int)n_parts_of(layout), scale, loss, kl, clipped};
 }
 
-template <typename T, int OP>
-int launch_groups(const GroupArgs& a, double scale, const void* scores_, void* out_, float* loss, float* kl, int64_t* clipped,
-                  void* scratch, cudaStream_t stream) {
-    const T* scores = static_cast<const T*>(scores_);
-    T* out = static_cast<T*>(out_);
-    const pb_groups& g = a.g;
-    const int64_t n_parts = n_group_parts(&g);
-    const bool want = loss || kl || clipped;
-    PieceSums* const sums = static_cast<PieceSums*>(scratch);
-    const Totals totals{want && n_parts > 1 ? reinterpret_cast<Part*>(sums + g.n_pieces) : nullptr, scale, loss, kl, clipped, want && n_parts == 1, a.kl_coef};
-    const int2* teams = reinterpret_cast<const int2*>(g.teams);
-    int slot = 0, launches = 0;
-    // the first launch waits for what is before it on the stream, the others may overlap with the ones before
-    auto launch = [&](auto kernel, int64_t grid, int block, size_t smem, auto... args) -> int {
-        PB_TRY(allow_shared(kernel, smem));
-        PB_CUDA_TRY(launch_after(kernel, (unsigned)grid, (unsigned)block, smem, launches > 0, stream, args...));
-        ++launches;
-        return PB_OK;
-    };
-    const int64_t small = team_warps(&g, 0, 6);
-    if (small) {
-        PB_TRY(launch(team_kernel<T, OP, 4>, team_grid(small), kTeamThreads, 0, a, teams, 0, small, slot, scores, out, totals));
-        slot += (int)team_grid(small);
-    }
-    if (g.team_warps[6]) {
-        int64_t before = 0;
-        for (int c = 0; c < 6; ++c) before += g.team_warps[c] * (32 >> c);
-        PB_TRY(launch(team_kernel<T, OP, 8>, team_grid(g.team_warps[6]), kTeamThreads, 0, a, teams + before, 6, g.team_warps[6], slot,
-                      scores, out, totals));
-        slot += (int)team_grid(g.team_warps[6]);
-    }
-    const int arrays = OP == kLogProbs ? 1 : OP == kChoice ? 2 : a.reference ? 4 : 3;
-    const int2* held = reinterpret_cast<const int2*>(g.held);
-    if (g.n_medium) {
-        PB_TRY(launch(held_kernel<T, OP, 128>, g.n_medium, 128, (size_t)(g.medium_rows * arrays * 4), a, held, (int)g.medium_rows, slot,
-                      scores, out, totals));
-        slot += (int)g.n_medium;
-    }
-    if (g.n_large) {
-        PB_TRY(launch(held_kernel<T, OP, 512>, g.n_large, 512, (size_t)(g.large_rows * arrays * 4), a, held + g.n_medium,
-                      (int)g.large_rows, slot, scores, out, totals));
-        slot += (int)g.n_large;
-    }
-    if (g.n_pieces) {
-        PB_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
-        if (OP != kLogProbs)
-            PB_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
-        PB_TRY(launch(piece_kernel<T, OP, kPieceOut>, g.n_pieces, kPieceThreads, 0, a, sums, slot, scores, out, totals));
-    }
-    if (want && n_parts != 1)
-        PB_TRY(launch(finish_kernel, 1, kFinishThreads, 0, (const Part*)totals.parts, n_parts, scale, loss, kl, clipped));
-    count_launch(launches);
+// A launch; `early`: it may begin before the one in front of it on the stream has ended, and waits for that itself.
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), int64_t grid, int block, size_t smem, bool early, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = early ? 1 : 0;
+    count_launch(1);
+    return cudaLaunchKernelEx(&cfg, kernel, (P)args...);
+}
+
+// No rows: nothing to launch, all totals 0.
+int no_totals(float* loss, float* kl, int64_t* clipped, cudaStream_t stream) {
+    if (loss) PB_CUDA_TRY(cudaMemsetAsync(loss, 0, sizeof(*loss), stream));
+    if (kl) PB_CUDA_TRY(cudaMemsetAsync(kl, 0, sizeof(*kl), stream));
+    if (clipped) PB_CUDA_TRY(cudaMemsetAsync(clipped, 0, sizeof(*clipped), stream));
     return PB_OK;
 }
 
 template <typename T>
-int launch_objective(const pb_objective* o, const void* scores, void* grad, float* loss, float* kl, int64_t* clipped, void* scratch,
-                     cudaStream_t stream) {
-    if (o->kind == PB_OBJECTIVE_PREFERENCE) {
-        const PairArgs a{*o->pairs, (float)o->beta, (float)o->smoothing, (float)(0.5 / o->beta),
-                         (float)(o->scale * (o->squared ? 2.0 : o->beta))};
-        if (kl) PB_CUDA_TRY(cudaMemsetAsync(kl, 0, sizeof(*kl), stream));
-        if (clipped) PB_CUDA_TRY(cudaMemsetAsync(clipped, 0, sizeof(*clipped), stream));
-        return launch_pairs<T>(a, o->squared != 0, o->scale, static_cast<const T*>(scores), static_cast<T*>(grad), loss, static_cast<double*>(scratch), stream);
+int launch_pairs(const pb_objective* o, const T* scores, T* grad, const Totals& totals, char* scratch, cudaStream_t stream) {
+    const pb_pairs& p = *o->pairs;
+    unsigned* counts = reinterpret_cast<unsigned*>(scratch + kTicketBytes);
+    double* sums = reinterpret_cast<double*>(scratch + kTicketBytes + align_up((size_t)p.n_split * 4, 8));
+    const PairArgs a{p, (float)o->beta, (float)(o->beta * 1.4426950408889634), (float)o->smoothing, (float)(0.5 / o->beta), (float)(o->scale * (o->squared ? 2.0 : o->beta)), sums, counts};
+    if (o->squared)
+        PB_CUDA_TRY(launch(pair_kernel<T, true>, n_parts_of(&p), kPairThreads, 0, false, stream, a, scores, grad, totals));
+    else
+        PB_CUDA_TRY(launch(pair_kernel<T, false>, n_parts_of(&p), kPairThreads, 0, false, stream, a, scores, grad, totals));
+    return PB_OK;
+}
+
+template <typename T, int OP>
+int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& totals, char* scratch, cudaStream_t stream) {
+    const pb_groups& g = a.g;
+    int slot = 0;
+    bool early = false;  // the first launch waits for what is before it on the stream, the others may overlap with it
+    if (g.n_team_warps) {
+        const int64_t grid = warp_grid(g.n_team_warps);
+        PB_CUDA_TRY(launch(team_kernel<T, OP>, grid, kTeamThreads, 0, early, stream, a, slot, scores, out, totals));
+        slot += (int)grid;
+        early = true;
     }
+    if (g.n_blocks) {
+        // threads of a group: as few as still fill the SMs (see block_kernel)
+        const size_t smem = OP == kLogProbs ? 0 : (size_t)g.block_rows * sizeof(float2);
+        const int2* list = reinterpret_cast<const int2*>(g.blocks);
+        auto block = [&](auto kernel, int threads) -> int {
+            PB_TRY(allow_shared(kernel, smem));
+            PB_CUDA_TRY(launch(kernel, g.n_blocks, threads, smem, early, stream, a, list, slot, scores, out, totals));
+            return PB_OK;
+        };
+        if (g.n_blocks >= 148 * 3)
+            PB_TRY(block(block_kernel<T, OP, 256>, 256));
+        else if (g.n_blocks >= 148 * 3 / 2)
+            PB_TRY(block(block_kernel<T, OP, 512>, 512));
+        else
+            PB_TRY(block(block_kernel<T, OP, 1024>, 1024));
+        slot += (int)g.n_blocks;
+        early = true;
+    }
+    if (g.n_pieces) {
+        PieceSums* sums = reinterpret_cast<PieceSums*>(scratch + kTicketBytes);
+        PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, early, stream, a, sums, slot, scores, out, totals));
+        if (OP != kLogProbs)
+            PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
+        PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceOut>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
+    }
+    return PB_OK;
+}
+
+template <typename T>
+int launch_objective(const pb_objective* o, const void* scores_, void* grad_, float* loss, float* kl, int64_t* clipped, void* scratch_,
+                     cudaStream_t stream) {
+    const T* scores = static_cast<const T*>(scores_);
+    T* grad = static_cast<T*>(grad_);
+    char* scratch = static_cast<char*>(scratch_);
+    if (o->kind == PB_OBJECTIVE_PREFERENCE)
+        return launch_pairs<T>(o, scores, grad, totals_of(o->pairs, o->scale, loss, kl, clipped, scratch), scratch, stream);
     const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(o->clip_high)), split(log1p(-o->clip_low)),
                       (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
-    if (o->kind == PB_OBJECTIVE_CHOICE) return launch_groups<T, kChoice>(a, o->scale, scores, grad, loss, kl, clipped, scratch, stream);
-    return launch_groups<T, kPolicy>(a, o->scale, scores, grad, loss, kl, clipped, scratch, stream);
+    const Totals totals = totals_of(o->groups, o->scale, loss, kl, clipped, scratch);
+    if (o->kind == PB_OBJECTIVE_CHOICE) return launch_groups<T, kChoice>(a, scores, grad, totals, scratch, stream);
+    return launch_groups<T, kPolicy>(a, scores, grad, totals, scratch, stream);
+}
+
+int check_scratch(const void* workspace, int64_t given, int64_t need) {
+    PB_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 16 == 0, "workspace is null or not aligned");
+    if (given < need) {
+        set_error("objective workspace: %lld bytes given, %lld needed", (long long)given, (long long)need);
+        return PB_ERR_WORKSPACE;
+    }
+    return PB_OK;
 }
 
 }  // namespace
 
 int objective_gradient(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss, float* kl,
                        int64_t* clipped, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
-    PB_REQUIRE(n_rows_of(o) == 0 || (scores && grad), "scores or gradient is null");
-    const int64_t need = scratch_bytes(o);
-    if (need > 0) {
-        PB_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 8 == 0, "workspace is null or not aligned");
-        if (workspace_bytes < need) {
-            set_error("objective workspace: %lld bytes given, %lld needed", (long long)workspace_bytes, (long long)need);
-            return PB_ERR_WORKSPACE;
-        }
-    }
-    int rc;
-    switch (score_type) {
-        case PB_SCORE_F32: rc = launch_objective<float>(o, scores, grad, loss, kl, clipped, workspace, stream); break;
-        case PB_SCORE_F16: rc = launch_objective<__half>(o, scores, grad, loss, kl, clipped, workspace, stream); break;
-        case PB_SCORE_BF16: rc = launch_objective<__nv_bfloat16>(o, scores, grad, loss, kl, clipped, workspace, stream); break;
-        default: return fail_arg("unknown type of scores %lld", (long long)score_type);
-    }
-    if (rc) return rc;
-    PB_LAUNCH_CHECK("objective");
-    return PB_OK;
+    PB_REQUIRE(score_type >= PB_SCORE_F32 && score_type <= PB_SCORE_BF16, "unknown type of scores %lld", (long long)score_type);
+    if (n_rows_of(o) == 0) return no_totals(loss, kl, clipped, stream);
+    PB_REQUIRE(scores && grad, "scores or gradient is null");
+    PB_TRY(check_scratch(workspace, workspace_bytes, scratch_bytes(o)));
+    if (score_type == PB_SCORE_F32) return launch_objective<float>(o, scores, grad, loss, kl, clipped, workspace, stream);
+    if (score_type == PB_SCORE_F16) return launch_objective<__half>(o, scores, grad, loss, kl, clipped, workspace, stream);
+    return launch_objective<__nv_bfloat16>(o, scores, grad, loss, kl, clipped, workspace, stream);
 }
 
 int objective_check(const pb_objective* o, int64_t n_rows) {
@@ -1035,33 +986,25 @@ extern "C" int pb_objective_evaluate(const pb_objective* o, const void* scores, 
 
 extern "C" int64_t pb_group_log_probs_bytes(const pb_groups* g) {
     if (check_groups(g)) return PB_ERR_ARG;
-    return group_scratch_bytes(g, false);
+    return g->n_pieces ? kTicketBytes + sums_bytes(g) : 0;
 }
 
 extern "C" int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* workspace,
                                   int64_t workspace_bytes, void* stream_) {
     NvtxRange nvtx("pb.group_log_probs n=%lld", g ? (long long)g->n_rows : -1);
     PB_TRY(check_groups(g));
-    PB_REQUIRE(g->n_rows == 0 || (scores && out), "scores or output is null");
-    if (g->n_pieces) {
-        PB_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 8 == 0, "workspace is null or not aligned");
-        if (workspace_bytes < group_scratch_bytes(g, false)) {
-            set_error("workspace of the log-probabilities: %lld bytes given, %lld needed", (long long)workspace_bytes,
-                      (long long)pb_group_log_probs_bytes(g));
-            return PB_ERR_WORKSPACE;
-        }
-    }
+    PB_REQUIRE(score_type >= PB_SCORE_F32 && score_type <= PB_SCORE_BF16, "unknown type of scores %lld", (long long)score_type);
+    if (g->n_rows == 0) return PB_OK;
+    PB_REQUIRE(scores && out, "scores or output is null");
+    if (g->n_pieces) PB_TRY(check_scratch(workspace, workspace_bytes, kTicketBytes + sums_bytes(g)));
     cudaStream_t stream = (cudaStream_t)stream_;
     GroupArgs a{};
     a.g = *g;
-    int rc;
-    switch (score_type) {
-        case PB_SCORE_F32: rc = launch_groups<float, kLogProbs>(a, 1.0, scores, out, nullptr, nullptr, nullptr, workspace, stream); break;
-        case PB_SCORE_F16: rc = launch_groups<__half, kLogProbs>(a, 1.0, scores, out, nullptr, nullptr, nullptr, workspace, stream); break;
-        case PB_SCORE_BF16: rc = launch_groups<__nv_bfloat16, kLogProbs>(a, 1.0, scores, out, nullptr, nullptr, nullptr, workspace, stream); break;
-        default: return fail_arg("unknown type of scores %lld", (long long)score_type);
-    }
-    if (rc) return rc;
-    PB_LAUNCH_CHECK("group_log_probs");
-    return PB_OK;
+    const Totals none{};
+    char* scratch = static_cast<char*>(workspace);
+    if (score_type == PB_SCORE_F32)
+        return launch_groups<float, kLogProbs>(a, static_cast<const float*>(scores), static_cast<float*>(out), none, scratch, stream);
+    if (score_type == PB_SCORE_F16)
+        return launch_groups<__half, kLogProbs>(a, static_cast<const __half*>(scores), static_cast<__half*>(out), none, scratch, stream);
+    return launch_groups<__nv_bfloat16, kLogProbs>(a, static_cast<const __nv_bfloat16*>(scores), static_cast<__nv_bfloat16*>(out), none, scratch, stream);
 }

@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 from typing import NamedTuple
 
 import numpy as np
@@ -106,8 +107,8 @@ def _check_pairs(chosen, rejected, n_rows: int) -> tuple[torch.Tensor, torch.Ten
     chosen, rejected = _indices(chosen, "chosen"), _indices(rejected, "rejected")
     if chosen.shape[0] != rejected.shape[0]:
         raise ValueError("chosen and rejected differ in length")
-    if 2 * chosen.shape[0] + n_rows + _PAIR_TILE > _MOST:
-        raise ValueError("more rows and sides of pairs than 32-bit numbers count")
+    if 2 * chosen.shape[0] > _MOST:
+        raise ValueError(f"more than {_MOST // 2} pairs")
     rejected = rejected.to(chosen.device)
     if chosen.shape[0]:
         low = min(int(chosen.min()), int(rejected.min()))
@@ -127,50 +128,79 @@ def _check_weight(weight, n_pairs: int, device) -> torch.Tensor:
 
 
 # (the layouts below are the ones of include/packboost_b200.h; they are made by torch, on any device)
-_PAIR_ITEMS, _PAIR_TILE = 8, 1024
-_RUNS_PER_SM = 8
+_SLICE_ROWS, _SLICE_ITEMS, _CHUNK_ITEMS = 64, 32, 512
+_WINDOW = 8192   # rows whose order a slice may change: its rows stay near the ones they are compared with
 
 
-def _lay_out_pairs(chosen, rejected, n_rows, weight, reference, n_sm: int = 148) -> dict:
-    """Items by row, in the order in which the pairs were given (chosen side first)."""
+def _rank_in_row(rows: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+    """For each entry, how many entries of the same row come before it."""
+    order = torch.sort(rows.to(torch.int32), stable=True).indices
+    rank = torch.empty_like(rows)
+    rank[order] = torch.arange(rows.shape[0], device=rows.device) - (counts.cumsum(0) - counts)[rows[order]]
+    return rank
+
+
+def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict:
+    """The items of every row: by columns of 64 rows with equally many, in chunks where there are many."""
     dev = chosen.device
     if n_rows == 0:
-        return {"n_items": 0, "run_tiles": 1, "n_cuts": 0}
-    touched = torch.zeros(n_rows, dtype=torch.bool, device=dev)
-    touched[chosen] = True
-    touched[rejected] = True
-    alone = torch.nonzero(~touched)[:, 0]
-    n_pairs = chosen.shape[0]
-    n_real = 2 * n_pairs + alone.shape[0]
-    fill = torch.full((-n_real % _PAIR_TILE,), n_rows - 1, dtype=torch.int64, device=dev)
-    own, order = torch.sort(torch.cat([chosen, rejected, alone, fill]).to(torch.int32), stable=True)
-    other = torch.cat([rejected, chosen, alone, fill])
-    other[n_pairs: 2 * n_pairs] |= 1 << 31
-    other = torch.where(other >= 1 << 31, other - (1 << 32), other).to(torch.int32)[order]   # bits of an unsigned word
-    out = {"n_items": own.shape[0], "other": other, "offset": None, "weight": None}
+        return {}
+    n_chosen = torch.bincount(chosen, minlength=n_rows)
+    n_rejected = torch.bincount(rejected, minlength=n_rows)
+    few = (n_chosen <= _SLICE_ITEMS) & (n_rejected <= _SLICE_ITEMS)
+    row = torch.nonzero(few)[:, 0]
+    # (by turns up and down: rows on either side of a step differ by one item)
+    turn = torch.where(n_chosen[row] % 2 == 0, n_rejected[row], _SLICE_ITEMS - n_rejected[row])
+    key = ((row // _WINDOW) * (_SLICE_ITEMS + 1) + n_chosen[row]) * (_SLICE_ITEMS + 1) + turn
+    row = row[torch.sort(key, stable=True).indices]
+    n_slices = -(-row.shape[0] // _SLICE_ROWS)
+    lanes = torch.full((_SLICE_ROWS * n_slices,), -1, dtype=torch.int64, device=dev)
+    lanes[: row.shape[0]] = row
+    have = torch.stack([torch.where(lanes >= 0, c[lanes.clamp_min(0)], torch.zeros_like(lanes)) for c in (n_chosen, n_rejected)], 1)
+    tall = have.view(n_slices, _SLICE_ROWS, 2).amax(1) if n_slices else have.new_zeros((0, 2))
+    column = tall.sum(1).cumsum(0) - tall.sum(1)
+    out = {"n_slices": n_slices,
+           "slices": torch.stack([column, tall[:, 0] | (tall[:, 1] << 16)], 1).to(torch.int32),
+           "slice_rows": torch.stack([lanes, have[:, 0] | (have[:, 1] << 16)], 1).to(torch.int32)}
+    first_many = _SLICE_ROWS * int(tall.sum())
+    if first_many > _MOST:
+        raise ValueError("more items than 32-bit numbers count")
+
+    many = torch.nonzero(~few)[:, 0]
+    size = n_chosen[many] + n_rejected[many]
+    begin = first_many + size.cumsum(0) - size
+    n_items = first_many + int(size.sum())
+    # where an item goes: base + stride * its rank among its row's items of its side
+    base = torch.empty((n_rows, 2), dtype=torch.int64, device=dev)
+    stride = torch.ones(n_rows, dtype=torch.int64, device=dev)
+    at = torch.arange(row.shape[0], device=dev)
+    base[row, 0] = column[at // _SLICE_ROWS] * _SLICE_ROWS + at % _SLICE_ROWS
+    base[row, 1] = base[row, 0] + tall[at // _SLICE_ROWS, 0] * _SLICE_ROWS
+    stride[row] = _SLICE_ROWS
+    base[many, 0], base[many, 1] = begin, begin + n_chosen[many]
+    place = [base[own, k] + stride[own] * _rank_in_row(own, count)
+             for k, (own, count) in enumerate(((chosen, n_chosen), (rejected, n_rejected)))]
+    out["other"] = torch.zeros(max(n_items, 1), dtype=torch.int32, device=dev)
+    out["other"][place[0]], out["other"][place[1]] = rejected.to(torch.int32), chosen.to(torch.int32)
     if reference is not None:
         r = reference.to(torch.float64)
-        away = r[chosen] - r[rejected]
-        none = away.new_zeros(own.shape[0] - 2 * n_pairs)
-        out["offset"] = torch.cat([away, -away, none]).to(torch.float32)[order]
+        away = (r[chosen] - r[rejected]).to(torch.float32)
+        out["offset"] = torch.zeros(max(n_items, 1), dtype=torch.float32, device=dev)
+        out["offset"][place[0]], out["offset"][place[1]] = away, -away
     if weight is not None:
-        out["weight"] = torch.cat([weight, weight, weight.new_zeros(own.shape[0] - 2 * n_pairs)])[order]
-    heads = torch.ones_like(own, dtype=torch.bool)
-    heads[1:] = own[1:] != own[:-1]
-    out["chunk_rows"] = own[::_PAIR_ITEMS].contiguous()
-    bits = heads.view(-1, _PAIR_ITEMS).to(torch.uint8) << torch.arange(_PAIR_ITEMS, dtype=torch.uint8, device=dev)
-    out["chunk_heads"] = bits.sum(1, dtype=torch.uint8)
-    n_tiles = own.shape[0] // _PAIR_TILE
-    out["run_tiles"] = run_tiles = -(-n_tiles // (n_sm * _RUNS_PER_SM))
-    # rows that go on over the border of two runs, each with its first and its last run
-    border = torch.arange(run_tiles, n_tiles, run_tiles, device=dev) * _PAIR_TILE
-    rows = own[border].cpu().numpy()
-    runs = np.flatnonzero(rows == own[border - 1].cpu().numpy()) + 1
-    rows = rows[runs - 1]
-    first = np.flatnonzero(np.r_[True, rows[1:] != rows[:-1]][: len(rows)])
-    last = np.r_[first[1:] - 1, len(rows) - 1][: len(first)]
-    out["n_cuts"] = len(first)
-    out["cuts"] = torch.from_numpy(np.stack([rows[first], runs[first] - 1, runs[last]], 1).astype(np.int32)).to(dev)
+        out["weight"] = torch.zeros(max(n_items, 1), dtype=torch.float32, device=dev)
+        out["weight"][place[0]] = out["weight"][place[1]] = weight
+
+    n_of = -(-size // _CHUNK_ITEMS)                      # chunks of a row
+    which = torch.repeat_interleave(torch.arange(many.shape[0], device=dev), n_of)
+    first = n_of.cumsum(0) - n_of
+    step = (torch.arange(which.shape[0], device=dev) - first[which]) * _CHUNK_ITEMS
+    split = (n_of > 1).to(torch.int64)
+    count = torch.minimum(size[which] - step, torch.full_like(step, _CHUNK_ITEMS))
+    better = (n_chosen[many][which] - step).clamp(min=0).minimum(count)
+    out["n_chunks"], out["n_split"] = which.shape[0], int(split.sum())
+    out["chunks"] = torch.stack([many[which], begin[which] + step, count, better, (split.cumsum(0) - split)[which], first[which],
+                                 n_of[which], torch.zeros_like(step)], 1).to(torch.int32)
     return out
 
 
@@ -187,13 +217,13 @@ def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
     return group, n_groups
 
 
-_TEAM_ROWS = (4, 8, 16, 32, 64, 128, 256)
-_MEDIUM, _LARGE, _PIECE = 1024, 8192, 4096
+_TEAM_ROWS = (8, 16, 32, 64, 128, 256)            # of 1, 2, 4 ... 32 lanes
+_BLOCK_ROWS, _PIECE = 8192, 2048
 
 
 def _lay_out_groups(group: torch.Tensor) -> dict:
-    """The rows by group where they are in another order, and the groups by length: teams of lanes for short ones, a
-    list of those that a CTA holds, pieces of long ones."""
+    """The rows by group where they are in another order, and the groups by length: teams of lanes for short ones, a CTA, pieces
+    of long ones."""
     n, dev = group.shape[0], group.device
     if n == 0:
         return {"n_groups": 0}
@@ -205,29 +235,35 @@ def _lay_out_groups(group: torch.Tensor) -> dict:
     heads[1:] = group[1:] != group[:-1]
     starts = torch.nonzero(heads)[:, 0]
     lengths = torch.diff(starts, append=starts.new_full((1,), n))
-    # class 0 .. 6: teams, 7 and 8: held, 9: pieces; groups of a class in the order of their rows
-    limits = torch.tensor(_TEAM_ROWS + (_MEDIUM, _LARGE), device=dev)
+    # short ones by length (a warp's groups should be alike), the others by kind: in the order of their rows
+    limits = torch.tensor(_TEAM_ROWS + (_BLOCK_ROWS,), device=dev)
     kind = torch.bucketize(lengths, limits)
-    table = torch.stack([starts, lengths], 1).to(torch.int32)[torch.sort(kind, stable=True).indices]
-    count = torch.bincount(kind, minlength=10).tolist()
+    key = torch.where(kind < len(_TEAM_ROWS), lengths, kind + _TEAM_ROWS[-1])
+    table = torch.stack([starts, lengths], 1).to(torch.int32)[torch.sort(key, stable=True).indices]
+    count = torch.bincount(kind, minlength=len(limits) + 1).tolist()
     parts = list(torch.split(table, count))
-    out = {"rows": rows, "n_groups": starts.shape[0]}
-    teams, warps = [], []
-    for c in range(7):
-        per_warp = 32 >> min(c, 5)
-        warps.append(-(-count[c] // per_warp))
-        teams += [parts[c], table.new_zeros((warps[c] * per_warp - count[c], 2))]
-    out["team_warps"] = tuple(warps)
-    out["teams"] = torch.cat(teams)
-    out["n_medium"], out["n_large"] = count[7], count[8]
-    out["medium_rows"], out["large_rows"] = (int(parts[c][:, 1].max()) if count[c] else 0 for c in (7, 8))
-    out["held"] = torch.cat(parts[7:9])
-    begin, length = parts[9].cpu().numpy().astype(np.int64).T
-    count = -(-length // _PIECE)
-    first = np.cumsum(count) - count
-    which = np.repeat(np.arange(len(count)), count)
+    teams, warps, entry = [], [], 0
+    for c in range(len(_TEAM_ROWS)):
+        n_warps = -(-count[c] // (32 >> c))
+        if n_warps == 0:
+            continue
+        own = torch.cat([parts[c], table.new_zeros((n_warps * (32 >> c) - count[c], 2))]).view(n_warps, 32 >> c, 2)
+        most = (own[:, :, 1].amax(1) + (1 << c) - 1) >> c
+        first = entry + torch.arange(n_warps, device=dev) * (32 >> c)
+        warps.append(torch.stack([first, c | (most << 8)], 1).to(torch.int32))
+        teams.append(own.view(-1, 2))
+        entry += n_warps * (32 >> c)
+    none = table.new_zeros((0, 2))
+    out = {"rows": rows, "n_groups": starts.shape[0], "teams": torch.cat(teams or [none]),
+           "team_warps": torch.cat(warps or [none]).flip(0),     # (the warps with most to do first)
+           "n_blocks": count[6], "blocks": parts[6], "block_rows": int(parts[6][:, 1].max()) if count[6] else 0}
+    out["n_team_warps"] = out["team_warps"].shape[0]
+    begin, length = parts[7].cpu().numpy().astype(np.int64).T
+    n_of = -(-length // _PIECE)
+    first = np.cumsum(n_of) - n_of
+    which = np.repeat(np.arange(len(n_of)), n_of)
     step = (np.arange(len(which)) - first[which]) * _PIECE
-    pieces = np.stack([begin[which] + step, np.minimum(length[which] - step, _PIECE), first[which], count[which]], 1)
+    pieces = np.stack([begin[which] + step, np.minimum(length[which] - step, _PIECE), first[which], n_of[which]], 1)
     out["n_pieces"] = len(which)
     out["pieces"] = torch.from_numpy(pieces.astype(np.int32)).to(dev)
     return out
@@ -248,6 +284,8 @@ class _Layout:
         self.device = device
         self._tensors = [t for t in tensors.values() if isinstance(t, torch.Tensor)]
         self._structs: dict = {}   # descriptors of objectives on this layout, by their options
+        self._rooms: dict = {}     # scratch of evaluations, by thread and stream
+        self._scratch_bytes = 0
         stream = torch.cuda.current_stream(device)
         self._stream = stream.cuda_stream
         stream.synchronize()
@@ -260,6 +298,19 @@ class _Layout:
             for t in self._tensors:
                 t.record_stream(current)
         return stream
+
+    def _room(self, stream: int) -> torch.Tensor:
+        """Scratch that no other evaluation uses at the same time: one per thread and stream, which a call leaves as the
+        next needs it.  A captured call has its own, since its graph may run beside anything."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        key = (threading.get_ident(), stream)
+        room = self._rooms.get(key)
+        if room is None:
+            if len(self._rooms) >= 16:
+                self._rooms = {}
+            room = self._rooms[key] = torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        return room
 
 
 class RowPairs(_Layout):
@@ -280,8 +331,7 @@ class RowPairs(_Layout):
         home = _home(chosen, rejected, weight, reference, device=device)
         with torch.cuda.device(home):
             parts = _lay_out_pairs(c.to(home), r.to(home), n_rows, None if weight is None else weight.to(home),
-                                   None if reference is None else reference.to(home),
-                                   torch.cuda.get_device_properties(home).multi_processor_count)
+                                   None if reference is None else reference.to(home))
             if parts.get("offset") is not None and not bool(torch.isfinite(parts["offset"]).all()):
                 raise ValueError("reference scores of compared rows must be finite")
             self.n_rows, self.n_pairs = n_rows, int(c.shape[0])
@@ -405,19 +455,21 @@ def _evaluate(struct: B.Objective, layout: _Layout, scores: torch.Tensor, policy
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return _evaluate(struct, layout, scores, policy)
-    stream, nbytes = layout._used_now(), layout._scratch_bytes
+    stream = layout._used_now()
+    room = layout._room(stream)
     grad = torch.empty_like(scores)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None   # (the allocator takes it back in the stream's order)
-    if not policy:
-        B.check(B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(),
-                                              loss.data_ptr(), None, None, scratch, nbytes, stream))
-        return LossAndGradient(loss, grad)
-    kl = torch.empty((), dtype=torch.float32, device=dev)
-    clipped = torch.empty((), dtype=torch.int64, device=dev)
-    B.check(B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
-                                          kl.data_ptr(), clipped.data_ptr(), scratch, nbytes, stream))
-    return PolicyLoss(loss, grad, kl, clipped)
+    kl = clipped = None
+    if policy:
+        kl = torch.empty((), dtype=torch.float32, device=dev)
+        clipped = torch.empty((), dtype=torch.int64, device=dev)
+    rc = B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
+                                       kl.data_ptr() if policy else None, clipped.data_ptr() if policy else None, room.data_ptr(),
+                                       layout._scratch_bytes, stream)
+    if rc:
+        layout._rooms = {}    # (a call that broke off may not have left its scratch in order)
+        B.check(rc)
+    return PolicyLoss(loss, grad, kl, clipped) if policy else LossAndGradient(loss, grad)
 
 
 def preference_loss(scores: torch.Tensor, pairs: RowPairs, *, beta: float = 1.0, label_smoothing: float = 0.0,
@@ -493,7 +545,7 @@ class _FitObjective:
 
     def __init__(self, struct: B.Objective, layout: _Layout, kept: tuple) -> None:
         self.struct, self.layout, self._kept = struct, layout, kept
-        self.workspace = torch.empty(layout._scratch_bytes, dtype=torch.uint8, device=layout.device)
+        self.workspace = torch.zeros(layout._scratch_bytes, dtype=torch.uint8, device=layout.device)
 
     def loss(self, preds: torch.Tensor) -> float:
         return float(_evaluate(self.struct, self.layout, preds).loss)

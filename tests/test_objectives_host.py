@@ -69,41 +69,55 @@ def _pairs(rng, rows, pairs, hubs, touched):
     return c, j + (j >= c)
 
 
-@pytest.mark.parametrize("rows,pairs,hubs,touched,n_sm", [(1, 0, 0, 1, 148), (9, 23, 0, 7, 148), (5000, 2000, 0, 5000, 148),
-                                                          (400, 9000, 1, 300, 1), (30_000, 40_000, 2, 30_000, 1),
-                                                          (2, 20_000, 0, 2, 1), (8192, 0, 0, 8192, 1)])
-def test_layout_of_pairs(rows, pairs, hubs, touched, n_sm):
+@pytest.mark.parametrize("rows,pairs,hubs,touched", [(1, 0, 0, 1), (9, 23, 0, 7), (5000, 2000, 0, 5000), (400, 9000, 1, 300),
+                                                     (30_000, 40_000, 2, 30_000), (2, 20_000, 0, 2), (8192, 0, 0, 8192),
+                                                     (60, 1100, 0, 60), (20_000, 100_000, 0, 20_000)])
+def test_layout_of_pairs(rows, pairs, hubs, touched):
     rng = np.random.default_rng(rows + pairs)
     c, j = _pairs(rng, rows, pairs, hubs, touched)
     w, r = rng.random(pairs).astype(np.float32), rng.normal(size=rows)
-    lay = O._lay_out_pairs(torch.from_numpy(c), torch.from_numpy(j), rows, torch.from_numpy(w), torch.from_numpy(r), n_sm)
-    n = lay["n_items"]
-    assert n % O._PAIR_TILE == 0
-    word = lay["other"].numpy().view(np.uint32)
-    other, rejected = (word & 0x7FFFFFFF).astype(np.int64), word >> 31 == 1
-    heads = np.unpackbits(lay["chunk_heads"].numpy(), bitorder="little").astype(bool)
-    own = np.cumsum(heads) - 1                      # every row has items
-    assert heads[0] and own[-1] == rows - 1
-    np.testing.assert_array_equal(lay["chunk_rows"].numpy(), own[::8])
-    real = other != own
-    assert real.sum() == 2 * pairs and not rejected[~real].any() and ((0 <= other) & (other < rows)).all()
-    np.testing.assert_array_equal(lay["offset"].numpy()[real], (r[own] - r[other]).astype(np.float32)[real])
-    for side, a, b in ((False, own, other), (True, other, own)):
-        at = real & (rejected == side)
-        got = np.lexsort((lay["weight"].numpy()[at], b[at], a[at]))
-        want = np.lexsort((w, j, c))
-        np.testing.assert_array_equal(a[at][got], c[want])
-        np.testing.assert_array_equal(b[at][got], j[want])
-        np.testing.assert_array_equal(lay["weight"].numpy()[at][got], w[want])
-    # a row is in the cuts if, and as, its items lie in several runs
-    run = np.arange(n) // (lay["run_tiles"] * O._PAIR_TILE)
-    first, last = run[np.flatnonzero(heads)], run[np.r_[np.flatnonzero(heads)[1:] - 1, n - 1]]
-    cut = np.flatnonzero(first != last)
-    np.testing.assert_array_equal(lay["cuts"].numpy(), np.stack([cut, first[cut], last[cut]], 1))
-    assert lay["n_cuts"] == len(cut) and run[-1] < n_sm * O._RUNS_PER_SM
+    lay = O._lay_out_pairs(torch.from_numpy(c), torch.from_numpy(j), rows, torch.from_numpy(w), torch.from_numpy(r))
+    n_c, n_j = np.bincount(c, minlength=rows), np.bincount(j, minlength=rows)
+    other, offset, weight = (lay[k].numpy() for k in ("other", "offset", "weight"))
+    assert ((0 <= other) & (other < rows)).all()
+    used, done, got = np.zeros(len(other), int), np.zeros(rows, int), []
+
+    def take(row, items, chosen):
+        used[items] += 1
+        np.testing.assert_array_equal(offset[items], (r[row] - r[other[items]]).astype(np.float32))
+        for o, x in zip(other[items].tolist(), weight[items].tolist()):
+            got.append((row, o, x) if chosen else (o, row, x))
+
+    slices, lanes = lay["slices"].numpy(), lay["slice_rows"].numpy().reshape(-1, 64, 2)
+    for (column, tall), slice_rows in zip(slices, lanes):
+        chosen, rejected = tall & 0xFFFF, tall >> 16
+        assert 64 * (column + chosen + rejected) <= len(other) or chosen + rejected == 0
+        for lane, (row, have) in enumerate(slice_rows):
+            if row < 0:
+                assert have == 0
+                continue
+            done[row] += 1
+            assert have & 0xFFFF == n_c[row] <= chosen <= 32 and have >> 16 == n_j[row] <= rejected <= 32
+            take(int(row), 64 * (column + np.arange(n_c[row])) + lane, True)
+            take(int(row), 64 * (column + chosen + np.arange(n_j[row])) + lane, False)
+    assert len(slices) == lay["n_slices"] == len(lanes)
+    left = {}
+    chunks = lay["chunks"].numpy()
+    for k, (row, begin, count, better, number, first, n_of, zero) in enumerate(chunks):
+        assert 0 < count <= O._CHUNK_ITEMS and 0 <= better <= count and first <= k < first + n_of and zero == 0
+        assert chunks[first: first + n_of, 0].tolist() == [row] * n_of and chunks[first: first + n_of, 2].sum() == n_c[row] + n_j[row]
+        if n_of > 1:
+            assert left.setdefault(int(row), int(number)) == number and 0 <= number < lay["n_split"]
+        assert begin + count <= len(other)
+        done[row] += k == first
+        take(int(row), begin + np.arange(better), True)
+        take(int(row), begin + np.arange(better, count), False)
+    assert len(set(left.values())) == len(left) == lay["n_split"] and len(chunks) == lay["n_chunks"]
+    assert (done == 1).all() and used.max(initial=0) <= 1
+    assert sorted(got) == sorted([(int(a), int(b), float(x)) for a, b, x in zip(c, j, w)] * 2)
 
 
-@pytest.mark.parametrize("lengths", [[], [1], [1] * 5000, [128] * 40, [256, 257, 129, 1, 128, 1024, 1025, 3, 8192, 8193, 5, 4096 * 3, 1],
+@pytest.mark.parametrize("lengths", [[], [1], [1] * 5000, [128] * 40, [256, 257, 129, 1, 128, 2048, 2049, 3, 4096, 4097, 8192, 8193, 5, 2048 * 9, 1, 16384, 16385],
                                      [7, 13, 127, 2] * 400, [20_000], [895, 1, 1, 128, 900, 128]])
 @pytest.mark.parametrize("mixed", [False, True])
 def test_layout_of_groups(lengths, mixed):
@@ -129,24 +143,21 @@ def test_layout_of_groups(lengths, mixed):
             assert length_of[begin] == size and low < size <= high
             done[begin: begin + size] += 1
 
-    team, low = lay["teams"].numpy(), 0
-    for c, high in enumerate(O._TEAM_ROWS):
-        own = team[: lay["team_warps"][c] * (32 >> min(c, 5))]
-        team = team[len(own):]
+    teams, seen = lay["teams"].numpy(), np.zeros(len(lay["teams"]), int)
+    for first, word in lay["team_warps"].numpy():
+        c, most = word & 0xFF, word >> 8
+        own = teams[first: first + (32 >> c)]
+        seen[first: first + (32 >> c)] += 1
         real = own[own[:, 1] > 0]
-        assert (own[len(real):] == 0).all() and len(own) - len(real) < 32
-        take(real.tolist(), low, high)
-        low = high
-    assert len(team) == 0
-    held = lay["held"].numpy().tolist()
-    take(held[: lay["n_medium"]], 256, O._MEDIUM)
-    take(held[lay["n_medium"]:], O._MEDIUM, O._LARGE)
-    assert len(held) == lay["n_medium"] + lay["n_large"]
-    assert lay["medium_rows"] == max([s for _, s in held[: lay["n_medium"]]], default=0)
-    assert lay["large_rows"] == max([s for _, s in held[lay["n_medium"]:]], default=0)
+        take(real.tolist(), O._TEAM_ROWS[c - 1] if c else 0, O._TEAM_ROWS[c])
+        assert most == -(-real[:, 1].max() // (1 << c)) and 1 <= most <= 8 and (own[own[:, 1] == 0] == 0).all()
+    assert (seen == 1).all() and len(lay["team_warps"]) == lay["n_team_warps"]
+    blocks = lay["blocks"].numpy().tolist()
+    take(blocks, O._TEAM_ROWS[-1], O._BLOCK_ROWS)
+    assert len(blocks) == lay["n_blocks"] and lay["block_rows"] == max([s for _, s in blocks], default=0)
     for i, (begin, size, first, count) in enumerate(lay["pieces"].numpy()):
         start = begin - (i - first) * O._PIECE
-        assert 0 < size <= O._PIECE and first <= i < first + count and length_of[start] > O._LARGE
+        assert 0 < size <= O._PIECE and first <= i < first + count and length_of[start] > O._BLOCK_ROWS
         assert (i == first + count - 1) == (begin + size == start + length_of[start])
         done[begin: begin + size] += 1
     assert (done == 1).all() and lay["n_pieces"] == len(lay["pieces"])
@@ -237,28 +248,28 @@ def test_library_refuses_bad_descriptors():
         assert lib.pb_objective_workspace_bytes(C.byref(o)) < 0
 
     def pairs(**kw):
-        return B.Pairs(**dict(dict(n_rows=4, n_items=1024, other=16, chunk_rows=16, chunk_heads=16, run_tiles=1), **kw))
+        return B.Pairs(**dict(dict(n_rows=4, n_slices=1, slices=16, slice_rows=16, other=16), **kw))
 
     def groups(**kw):
-        return B.Groups(**dict(dict(n_rows=3, n_groups=1, n_medium=1, medium_rows=3, held=16), **kw))
+        return B.Groups(**dict(dict(n_rows=3, n_groups=1, n_team_warps=1, team_warps=16, teams=16), **kw))
 
-    ok, good = pairs(n_items=2048), groups()
+    ok, good = pairs(), groups()
     refused(B.Objective(kind=9), "unknown objective")
     refused(B.Objective(kind=0), "pairs are null")
     refused(B.Objective(kind=1), "groups are null")
-    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "n_rows"), (dict(n_items=1 << 31), "n_items"),
-                      (dict(n_items=1000), "tiles"), (dict(n_rows=0), "tiles"), (dict(other=None), "null"),
-                      (dict(chunk_rows=None), "null"), (dict(chunk_heads=None), "null"), (dict(run_tiles=0), "null"),
-                      (dict(n_cuts=2, cuts=16), "cuts"), (dict(n_cuts=1), "cuts"), (dict(offset=8), "aligned")):
+    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "n_rows"), (dict(n_slices=1 << 26), "range"),
+                      (dict(n_slices=0), "not laid out"), (dict(slices=None), "null"), (dict(slice_rows=None), "null"),
+                      (dict(other=None), "null"), (dict(n_chunks=1), "null"), (dict(n_chunks=-1), "range"),
+                      (dict(n_split=1), "range"), (dict(slices=20), "aligned"), (dict(offset=20), "aligned"), (dict(n_chunks=1, chunks=24), "aligned")):
         refused(B.Objective(kind=0, pairs=C.pointer(pairs(**kw)), beta=1.0), match)
     for kw, match in ((dict(beta=0.0), "beta"), (dict(beta=1.0, smoothing=0.5), "smoothing"),
                       (dict(beta=1.0, scale=float("nan")), "scale")):
         refused(B.Objective(kind=0, pairs=C.pointer(ok), **kw), match)
     for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_groups=4), "n_groups"), (dict(n_groups=0), "without a group"),
-                      (dict(n_medium=0), "not laid out"), (dict(held=None), "null"), (dict(held=20), "aligned"),
-                      (dict(team_warps=(0, 1, 0, 0, 0, 0, 0)), "null"), (dict(team_warps=(-1, 0, 0, 0, 0, 0, 0)), "range"),
-                      (dict(n_pieces=1), "null"), (dict(n_large=-1), "range"), (dict(medium_rows=0), "range"),
-                      (dict(medium_rows=1025), "range"), (dict(n_medium=0, n_large=1, large_rows=9000), "range")):
+                      (dict(n_team_warps=0), "not laid out"), (dict(teams=None), "null"), (dict(team_warps=None), "null"),
+                      (dict(teams=20), "aligned"), (dict(n_blocks=1, block_rows=300), "null"), (dict(n_blocks=-1), "range"),
+                      (dict(n_blocks=2), "range"), (dict(n_blocks=1, block_rows=8193, blocks=16), "range"),
+                      (dict(n_blocks=1, blocks=16), "range"), (dict(n_pieces=1), "null"), (dict(n_pieces=-1), "range")):
         refused(B.Objective(kind=1, groups=C.pointer(groups(**kw))), match)
     refused(B.Objective(kind=1, groups=C.pointer(good)), "target")
     rows = dict(groups=C.pointer(good), advantage=16, old=16)
@@ -277,7 +288,7 @@ def test_library_refuses_bad_descriptors():
         B.check(lib.pb_group_log_probs(C.byref(good), None, 0, 16, None, 0, None))
     with pytest.raises(ValueError, match="type"):
         B.check(lib.pb_group_log_probs(C.byref(good), 16, 5, 16, None, 0, None))
-    long = groups(n_medium=0, n_pieces=1, pieces=16)
+    long = groups(n_team_warps=0, n_pieces=1, pieces=16)
     with pytest.raises(ValueError, match="workspace"):
         B.check(lib.pb_group_log_probs(C.byref(long), 16, 0, 16, None, 0, None))
     with pytest.raises(RuntimeError, match="bytes given"):
