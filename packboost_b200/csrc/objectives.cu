@@ -12,6 +12,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace pb {
@@ -338,12 +340,11 @@ struct Pair32 {  // hi + lo
     float hi, lo;
 };
 
-// a - b without rounding, plus a small `lo`.  (Where hi is infinite, lo comes out as NaN and is made 1, with which
-// exp and sums still come out right; where it is above 1 by itself, hi is beyond 2^24.)
+// a - b without rounding, plus a small `lo`.  Where hi is infinite, lo comes out as NaN; fminf(lo, 1) is then 1, with which sums
+// and exp come out right, and changes nothing else: lo is above 1 only where hi is beyond 2^24.
 __device__ __forceinline__ Pair32 difference(float a, float b, float lo) {
     const float t = a - b, v = t - a;
-    const float err = (a - (t - v)) - (b + v);
-    return Pair32{t, fminf(err + lo, 1.f)};
+    return Pair32{t, (a - (t - v)) - (b + v) + lo};
 }
 
 __host__ __device__ __forceinline__ Pair32 split(double x) {
@@ -351,9 +352,16 @@ __host__ __device__ __forceinline__ Pair32 split(double x) {
     return Pair32{hi, lo - lo == 0.f ? lo : 0.f};
 }
 
+__device__ __forceinline__ float sum_of(Pair32 x) { return x.hi + fminf(x.lo, 1.f); }
+
+// exp(hi + lo): 2^y with y = hi log2 e rounded, by the unit that has 2^x to 2 ulp, times 1 + what y left out.
 __device__ __forceinline__ float exp_of(Pair32 x) {
-    const float e = expf(x.hi);
-    return fmaf(e, x.lo, e);
+    const float log2e = 1.44269502f, rest = 1.33687e-8f;  // log2 e as a float, and (log2 e - that) ln 2
+    const float y = x.hi * log2e;
+    float more = fmaf(fmaf(x.hi, log2e, -y), 0.693147181f, x.lo);
+    more = fminf(fmaf(x.hi, rest, more), 1.f);
+    const float e = exp2_of(y);
+    return fmaf(e, more, e);
 }
 
 // exp(x) for x <= 0, to 7e-15 of the value and exactly 1 at 0: with n = rint(x / ln 2), 2^n times the Taylor
@@ -398,53 +406,68 @@ struct GroupArgs {
     float scale;
 };
 
-__device__ __forceinline__ float gradient_of(const GroupArgs& a, float p, float fixed, float total) {
-    return (p == 0.f ? fixed : fmaf(p, total, fixed)) * a.scale;  // (the total may be infinite)
-}
-
-// Up to N rows of one group that a thread has: places first, first + stride ... below end.
-template <typename T, int OP, int N>
+// Up to N rows of one group that a thread has: places first, first + stride ... of those from `low` to below `end`.  VECTOR:
+// four neighbouring ones, whose first is a multiple of 4, moved as one word where all are in the table and the arrays allow it (which
+// changes nothing in the order of sums).  FULL (of the members): all are the group's.
+template <typename T, int OP, int N, bool VECTOR = false>
 struct Rows {
     const GroupArgs& a;
-    int first, stride, end;  // places
-    int used;                // rows that any thread of the warp has
-    int row[N];              // only with a list of rows
+    int first, stride, low, end;  // places
+    int used;                     // rows that any thread of the warp has
+    bool words;                   // VECTOR: all arrays begin on the border of a word
+    int row[N];                   // only with a list of rows
     float s[N], main[N], old[N], reference[N];  // s becomes p, main (target or advantage) the fixed part
     double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
+    static_assert(!VECTOR || N == 4, "rows of a word");
 
     __device__ __forceinline__ Rows(const GroupArgs& args) : a(args) {}
 
-    __device__ __forceinline__ bool has(int u) const { return first + u * stride < end; }
-    __device__ __forceinline__ int row_of(int u) const { return a.g.rows ? row[u] : first + u * stride; }
+    __device__ __forceinline__ int place(int u) const { return VECTOR ? first + u : first + u * stride; }
+    template <bool FULL>
+    __device__ __forceinline__ bool has(int u) const { return FULL || (place(u) < end && (!VECTOR || place(u) >= low)); }
+    __device__ __forceinline__ int row_of(int u) const { return !VECTOR && a.g.rows ? row[u] : place(u); }
     // (half of the rows are there more often than not: only the others are worth a branch)
-    __device__ __forceinline__ bool on(int u) const { return u < N / 2 || u < used; }
+    template <bool FULL>
+    __device__ __forceinline__ bool on(int u) const { return VECTOR || FULL || u < N / 2 || u < used; }
+
+    template <bool FULL, typename V>
+    __device__ __forceinline__ void take(const V* from, V to[N]) const {
+        if (VECTOR && words && (FULL || first + 3 < (int)a.g.n_rows)) {
+            if (sizeof(V) == 4)
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + first);
+            else
+                *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from + first);
+        } else {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (on<FULL>(u) && has<FULL>(u)) to[u] = from[row_of(u)];
+        }
+    }
 
     // Everything is asked for before anything is used.
+    template <bool FULL>
     __device__ __forceinline__ void load(const T* scores, bool inputs) {
-        T raw[N];
+        alignas(16) T raw[N];
+        if (!VECTOR && a.g.rows) {
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (on(u) && a.g.rows && has(u)) row[u] = a.g.rows[first + u * stride];
-#pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (on(u) && has(u)) raw[u] = scores[row_of(u)];
+            for (int u = 0; u < N; ++u)
+                if (on<FULL>(u) && has<FULL>(u)) row[u] = a.g.rows[place(u)];
+        }
+        take<FULL>(scores, raw);
         if (OP != kLogProbs && inputs) {
-#pragma unroll
-            for (int u = 0; u < N; ++u) {
-                main[u] = old[u] = reference[u] = 0.f;
-                if (on(u) && has(u)) {
-                    const int r = row_of(u);
-                    main[u] = OP == kChoice ? a.target[r] : a.advantage[r];
-                    if (OP == kPolicy) {
-                        old[u] = a.old[r];
-                        if (a.reference) reference[u] = a.reference[r];
-                    }
-                }
+            take<FULL>(OP == kChoice ? a.target : a.advantage, main);
+            if (OP == kPolicy) {
+                take<FULL>(a.old, old);
+                if (a.reference) take<FULL>(a.reference, reference);
             }
         }
 #pragma unroll
-        for (int u = 0; u < N; ++u) s[u] = on(u) && has(u) ? to_f32(raw[u]) : -INFINITY;
+        for (int u = 0; u < N; ++u) {
+            const bool mine = on<FULL>(u) && has<FULL>(u);
+            s[u] = mine ? to_f32(raw[u]) : -INFINITY;
+            if (OP == kChoice && inputs) main[u] = mine ? main[u] : 0.f;
+        }
     }
 
     __device__ __forceinline__ float largest() const {
@@ -455,24 +478,27 @@ struct Rows {
     }
 
     // Sum of exp(s - m).  (m = -inf: no row is left, all of them add exp(-inf) to 0.)
+    template <bool FULL>
     __device__ __forceinline__ double mass(float m) const {
         const double top = m == -INFINITY ? 0.0 : (double)m;
         double z = 0.0;
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            if (on(u)) z += exp_negative((double)s[u] - top);
+            if (on<FULL>(u)) z += exp_negative((double)s[u] - top);
         return z;
     }
 
     // With the log of the group's sum: p, the part of the gradient that does not hang on the rest of the group, and what
     // goes into the sums.  A row's gradient is (fixed + p * share) * scale: of a choice -t + p * sum t, of a policy, with h
-    // the slopes of the taken rows and D the divergence, h + p (k (l - reference - D) - sum h).
+    // the slopes of the taken rows and D the divergence, h + p (k (l - reference - D) - sum h).  A masked row's other
+    // inputs, and the old log-probability of a row that was not taken, may be anything.
+    template <bool FULL>
     __device__ __forceinline__ void terms(double lse64) {
         const Pair32 lse = split(lse64);
         float part = 0.f, part_loss = 0.f, part_kl = 0.f;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            if (on(u)) {
+            if (on<FULL>(u)) {
                 const bool live = s[u] != -INFINITY;
                 const Pair32 l = difference(s[u], lse.hi, -lse.lo);
                 const float p = live ? exp_of(l) : 0.f;
@@ -486,16 +512,16 @@ struct Rows {
                     const float adv = live ? main[u] : 0.f;
                     const bool up = adv > 0.f, taken = adv != 0.f;
                     const Pair32 x = difference(l.hi, old[u], l.lo);
-                    const float past = (x.hi - (up ? a.log_high.hi : a.log_low.hi)) + (x.lo - (up ? a.log_high.lo : a.log_low.lo));
-                    const bool beyond = taken && (up ? past > 0.f : past < 0.f);
-                    const float cost = -adv * (beyond ? (up ? a.bound_high : a.bound_low) : exp_of(x));
-                    fixed = taken && !beyond ? cost : 0.f;
-                    part_loss += taken ? cost : 0.f;
+                    const float past = (x.hi - (up ? a.log_high.hi : a.log_low.hi)) + (fminf(x.lo, 1.f) - (up ? a.log_high.lo : a.log_low.lo));
+                    const bool beyond = taken && (up ? past : -past) > 0.f;
+                    const float q = beyond ? (up ? a.bound_high : a.bound_low) : exp_of(x);
+                    const float cost = -adv * (taken ? q : 0.f);
+                    fixed = beyond ? 0.f : cost;
+                    part_loss += cost;
                     clipped += beyond ? 1 : 0;
                     own = -fixed;
                     if (a.reference) {
-                        const Pair32 gap = difference(l.hi, reference[u], l.lo);
-                        const float k = live ? p * (gap.hi + gap.lo) : 0.f;
+                        const float k = live ? p * sum_of(difference(l.hi, reference[u], l.lo)) : 0.f;
                         fixed = fmaf(a.kl_coef, k, fixed);
                         own = fmaf(-a.kl_coef, k, own);
                         part_kl += k;
@@ -505,10 +531,10 @@ struct Rows {
                 s[u] = p;
                 main[u] = fixed;
             }
-            if ((u & 3) == 3 && on(u - 3)) {  // (four terms in 32 bits, the sums of fours in 64)
+            if ((u & 3) == 3 && on<FULL>(u - 3)) {  // (four terms in 32 bits, the sums of fours in 64)
                 share += (double)part;
                 if (OP == kPolicy) {
-                    loss += (double)part_loss + (double)a.kl_coef * (double)part_kl;
+                    loss += (double)fmaf(a.kl_coef, part_kl, part_loss);
                     kl += (double)part_kl;
                 }
                 part = part_loss = part_kl = 0.f;
@@ -516,21 +542,37 @@ struct Rows {
         }
     }
 
-    __device__ __forceinline__ void gradient(float total, T* out) const {
+    // (v becomes what is written)
+    template <bool FULL>
+    __device__ __forceinline__ void put(const float v[N], T* out) const {
+        if (VECTOR && words && (FULL || (first >= low && first + 3 < end))) {
+            alignas(16) const T w[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+            if (sizeof(T) == 4)
+                *reinterpret_cast<uint4*>(out + first) = *reinterpret_cast<const uint4*>(w);
+            else
+                *reinterpret_cast<uint2*>(out + first) = *reinterpret_cast<const uint2*>(w);
+        } else {
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (on(u) && has(u))
-                out[row_of(u)] = from_f32<T>(gradient_of(a, s[u], main[u], total));
+            for (int u = 0; u < N; ++u)
+                if (on<FULL>(u) && has<FULL>(u)) out[row_of(u)] = from_f32<T>(v[u]);
+        }
     }
 
+    template <bool FULL>
+    __device__ __forceinline__ void gradient(float total, T* out) const {
+        float g[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) g[u] = (s[u] == 0.f ? main[u] : fmaf(s[u], total, main[u])) * a.scale;  // (the total may be infinite)
+        put<FULL>(g, out);
+    }
+
+    template <bool FULL>
     __device__ __forceinline__ void log_probs(double lse64, T* out) const {
         const Pair32 lse = split(lse64);
+        float l[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (on(u) && has(u)) {
-                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
-                out[row_of(u)] = from_f32<T>(l.hi + l.lo);
-            }
+        for (int u = 0; u < N; ++u) l[u] = sum_of(difference(s[u], lse.hi, -lse.lo));
+        put<FULL>(l, out);
     }
 };
 
@@ -546,8 +588,10 @@ __device__ __forceinline__ double rescaled(double z, float m, float top) {
 constexpr int kTeamThreads = 256;
 constexpr int kTeamRows = PB_TEAM_ROWS / 32;
 
+// (registers: what keeps most warps on an SM; 3 CTAs of a policy took 37 us over 1M rows in interleaved lists, 4 CTAs with registers
+// spilled 42, as many as fit without a limit 41; of a choice, 4 took 27 us over 2.7M rows, 2 took 33, 5 took 30)
 template <typename T, int OP>
-__global__ void __launch_bounds__(kTeamThreads) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
+__global__ void __launch_bounds__(kTeamThreads, OP == kPolicy ? 3 : 4) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
                                                             Totals totals) {
     __shared__ double scratch[kTeamThreads / 32];
     let_next_start();
@@ -561,22 +605,23 @@ __global__ void __launch_bounds__(kTeamThreads) team_kernel(GroupArgs a, int slo
         Rows<T, OP, kTeamRows> rows(a);
         rows.first = group.x + (lane & (lanes - 1));
         rows.stride = lanes;
+        rows.low = group.x;
         rows.end = group.x + group.y;
         rows.used = what.y >> 8;
-        rows.load(scores, true);
+        rows.template load<false>(scores, true);
         float m = rows.largest();
         for (int d = lanes >> 1; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        double z = rows.mass(m);
+        double z = rows.template mass<false>(m);
         for (int d = lanes >> 1; d > 0; d >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, d);
         const double lse = log_sum(m, z);
         if (OP == kLogProbs) {
-            rows.log_probs(lse, out);
+            rows.template log_probs<false>(lse, out);
             continue;
         }
-        rows.terms(lse);
+        rows.template terms<false>(lse);
         double share = rows.share;
         for (int d = lanes >> 1; d > 0; d >>= 1) share += __shfl_xor_sync(0xFFFFFFFFu, share, d);
-        rows.gradient((float)share, out);
+        rows.template gradient<false>((float)share, out);
         loss += rows.loss;
         kl += rows.kl;
         clipped += rows.clipped;
@@ -608,66 +653,78 @@ __device__ __forceinline__ double cta_log_sum(float m, double z, float* s_m, dou
 
 constexpr int kBlockRows = 4;  // of a thread at a time
 
-template <typename T, int OP, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2* __restrict__ list, int slot0,
+template <typename T, int OP, int THREADS, bool VECTOR>
+__global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2* __restrict__ list, int most, bool words, int slot0,
                                                         const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
-    extern __shared__ float2 kept[];
+    extern __shared__ float4 kept4[];  // p, then the fixed parts, `most` each: a thread's four are one word
     __shared__ float s_m[THREADS / 32];
     __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
     let_next_start();
     const int2 group = list[blockIdx.x];
     constexpr int kStep = THREADS * kBlockRows;
-    auto rows_at = [&](auto& rows, int i0) {
-        rows.first = group.x + i0 + (int)threadIdx.x;
-        rows.stride = THREADS;
-        rows.end = group.x + group.y;
-        rows.used = (group.y - i0 + THREADS - 1) / THREADS;
+    using Four = Rows<T, OP, kBlockRows, VECTOR>;
+    const int begin = VECTOR ? group.x & ~3 : group.x, end = group.x + group.y;
+    // all steps of the group in turn: f(rows, step, whether all rows are the group's)
+    auto steps = [&](auto f) {
+        for (int at = begin, k = 0; at < end; at += kStep, ++k) {
+            Four rows(a);
+            rows.first = at + (int)threadIdx.x * (VECTOR ? kBlockRows : 1);
+            rows.stride = THREADS;
+            rows.low = group.x;
+            rows.end = end;
+            rows.used = (end - at + THREADS - 1) / THREADS;
+            rows.words = words;
+            if (at >= group.x && at + kStep <= end)
+                f(rows, k, std::true_type());
+            else
+                f(rows, k, std::false_type());
+        }
     };
     float m = -INFINITY;
     double z = 0.0;
-    for (int i0 = 0; i0 < group.y; i0 += kStep) {
-        Rows<T, OP, kBlockRows> rows(a);
-        rows_at(rows, i0);
-        rows.load(scores, false);
+    steps([&](Four& rows, int, auto full) {
+        rows.template load<decltype(full)::value>(scores, false);
         const float top = fmaxf(m, rows.largest());
-        z = rescaled(z, m, top) + rows.mass(top);
+        z = rescaled(z, m, top) + rows.template mass<decltype(full)::value>(top);
         m = top;
-    }
+    });
     const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
     if (OP == kLogProbs) {
-        for (int i0 = 0; i0 < group.y; i0 += kStep) {
-            Rows<T, OP, kBlockRows> rows(a);
-            rows_at(rows, i0);
-            rows.load(scores, false);
-            rows.log_probs(lse, out);
-        }
+        steps([&](Four& rows, int, auto full) {
+            rows.template load<decltype(full)::value>(scores, false);
+            rows.template log_probs<decltype(full)::value>(lse, out);
+        });
         wait_for_previous();
         return;
     }
     double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
-    for (int i0 = 0; i0 < group.y; i0 += kStep) {
-        Rows<T, OP, kBlockRows> rows(a);
-        rows_at(rows, i0);
-        rows.load(scores, true);
-        rows.terms(lse);
-#pragma unroll
-        for (int u = 0; u < kBlockRows; ++u) {
-            const int i = i0 + u * THREADS + threadIdx.x;
-            if (i < group.y) kept[i] = make_float2(rows.s[u], rows.main[u]);
+    float4* const kept_p = kept4 + threadIdx.x;
+    float4* const kept_fixed = kept4 + most / 4 + threadIdx.x;
+    steps([&](Four& rows, int k, auto full) {
+        rows.template load<decltype(full)::value>(scores, true);
+        rows.template terms<decltype(full)::value>(lse);
+        if (decltype(full)::value || (k * THREADS + (int)threadIdx.x) * 4 < most) {
+            kept_p[k * THREADS] = make_float4(rows.s[0], rows.s[1], rows.s[2], rows.s[3]);
+            kept_fixed[k * THREADS] = make_float4(rows.main[0], rows.main[1], rows.main[2], rows.main[3]);
         }
         loss += rows.loss;
         kl += rows.kl;
         share += rows.share;
         clipped += rows.clipped;
-    }
+    });
     const float total = (float)cta_sum<THREADS>(share, scratch);
-#pragma unroll 4
-    for (int i = threadIdx.x; i < group.y; i += THREADS) {
-        const float2 v = kept[i];
-        const int r = a.g.rows ? a.g.rows[group.x + i] : group.x + i;
-        out[r] = from_f32<T>(gradient_of(a, v.x, v.y, total));
-    }
+    steps([&](Four& rows, int k, auto full) {
+        if (!decltype(full)::value && (k * THREADS + (int)threadIdx.x) * 4 >= most) return;
+        *reinterpret_cast<float4*>(rows.s) = kept_p[k * THREADS];
+        *reinterpret_cast<float4*>(rows.main) = kept_fixed[k * THREADS];
+        if (!VECTOR && a.g.rows) {
+#pragma unroll
+            for (int u = 0; u < kBlockRows; ++u)
+                if (rows.template has<decltype(full)::value>(u)) rows.row[u] = a.g.rows[rows.place(u)];
+        }
+        rows.template gradient<decltype(full)::value>(total, out);
+    });
     put_totals<THREADS>(totals, slot0 + blockIdx.x, loss, kl, clipped, OP == kPolicy, scratch);
     wait_for_previous();
 }
@@ -698,13 +755,14 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     Rows<T, OP, kPieceRows> rows(a);
     rows.first = piece.x + threadIdx.x;
     rows.stride = kPieceThreads;
+    rows.low = piece.x;
     rows.end = piece.x + piece.y;
     rows.used = (piece.y + kPieceThreads - 1) / kPieceThreads;
-    rows.load(scores, STEP != kPieceMass);
+    rows.template load<false>(scores, STEP != kPieceMass);
     if (STEP == kPieceMass) {
         float m = rows.largest();
         const float wm = warp_max(m);
-        double z = warp_sum(rows.mass(wm));
+        double z = warp_sum(rows.template mass<false>(wm));
         if (lane == 0) {
             s_m[warp] = wm;
             s_z[warp] = z;
@@ -733,10 +791,10 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     }
     const double lse = cta_log_sum<kPieceThreads>(m, z, s_m, s_z);
     if (OP == kLogProbs) {
-        rows.log_probs(lse, out);
+        rows.template log_probs<false>(lse, out);
         return;
     }
-    rows.terms(lse);
+    rows.template terms<false>(lse);
     if (STEP == kPieceTerms) {
         const double share = cta_sum<kPieceThreads>(rows.share, scratch);
         if (threadIdx.x == 0) pieces[blockIdx.x].share = share;
@@ -745,7 +803,7 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     }
     double share = 0.0;
     for (int k = threadIdx.x; k < count; k += kPieceThreads) share += pieces[first + k].share;
-    rows.gradient((float)cta_sum<kPieceThreads>(share, scratch), out);
+    rows.template gradient<false>((float)cta_sum<kPieceThreads>(share, scratch), out);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
@@ -885,6 +943,9 @@ template <typename T, int OP>
 int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& totals, char* scratch, cudaStream_t stream) {
     const pb_groups& g = a.g;
     int slot = 0;
+    // (rows in order: four neighbouring ones to a thread, as one word where all arrays are on the border of one)
+    const uintptr_t bits = (uintptr_t)a.target | (uintptr_t)a.advantage | (uintptr_t)a.old | (uintptr_t)a.reference;
+    const bool words = bits % 16 == 0 && ((uintptr_t)scores | (uintptr_t)out) % (4 * sizeof(T)) == 0;
     bool early = false;  // the first launch waits for what is before it on the stream, the others may overlap with it
     if (g.n_team_warps) {
         const int64_t grid = warp_grid(g.n_team_warps);
@@ -893,20 +954,23 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
         early = true;
     }
     if (g.n_blocks) {
-        // threads of a group: as few as still fill the SMs (see block_kernel)
-        const size_t smem = OP == kLogProbs ? 0 : (size_t)g.block_rows * sizeof(float2);
+        // threads of a group: as few as still fill the SMs (see block_kernel); a step more than the longest group takes
+        // (its first place is rounded down)
+        const int threads = g.n_blocks >= 148 * 3 ? 256 : g.n_blocks >= 148 * 3 / 2 ? 512 : 1024;
+        const int most = (int)(g.block_rows + 7) / 4 * 4 + (g.rows ? threads * kBlockRows : 0);
+        const size_t smem = OP == kLogProbs ? 0 : (size_t)most * 8;
         const int2* list = reinterpret_cast<const int2*>(g.blocks);
-        auto block = [&](auto kernel, int threads) -> int {
+        auto block = [&](auto kernel) -> int {
             PB_TRY(allow_shared(kernel, smem));
-            PB_CUDA_TRY(launch(kernel, g.n_blocks, threads, smem, early, stream, a, list, slot, scores, out, totals));
+            PB_CUDA_TRY(launch(kernel, g.n_blocks, threads, smem, early, stream, a, list, most, words, slot, scores, out, totals));
             return PB_OK;
         };
-        if (g.n_blocks >= 148 * 3)
-            PB_TRY(block(block_kernel<T, OP, 256>, 256));
-        else if (g.n_blocks >= 148 * 3 / 2)
-            PB_TRY(block(block_kernel<T, OP, 512>, 512));
+        if (threads == 256)
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false>) : block(block_kernel<T, OP, 256, true>));
+        else if (threads == 512)
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false>) : block(block_kernel<T, OP, 512, true>));
         else
-            PB_TRY(block(block_kernel<T, OP, 1024>, 1024));
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 1024, false>) : block(block_kernel<T, OP, 1024, true>));
         slot += (int)g.n_blocks;
         early = true;
     }
