@@ -416,7 +416,11 @@ struct Rows {
     int used;                     // rows that any thread of the warp has
     bool words;                   // VECTOR: all arrays begin on the border of a word
     int row[N];                   // only with a list of rows
-    float s[N], main[N], old[N], reference[N];  // s becomes p, main (target or advantage) the fixed part
+    // (s becomes p, main (target or advantage) the fixed part; of more than four rows, the three inputs of a policy come four rows
+    // at a time: with all of them at once, half as many warps fit on an SM)
+    static constexpr bool LATE = OP == kPolicy && N > 4;
+    static constexpr int HELD = LATE ? 4 : N;
+    float s[N], main[N], old[HELD], reference[HELD];
     double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
     static_assert(!VECTOR || N == 4, "rows of a word");
@@ -431,8 +435,9 @@ struct Rows {
     template <bool FULL>
     __device__ __forceinline__ bool on(int u) const { return VECTOR || FULL || u < N / 2 || u < used; }
 
-    template <bool FULL, typename V>
-    __device__ __forceinline__ void take(const V* from, V to[N]) const {
+    // COUNT values from the u0-th on
+    template <bool FULL, int COUNT = N, typename V>
+    __device__ __forceinline__ void take(const V* from, V* to, int u0 = 0) const {
         if (VECTOR && words && (FULL || first + 3 < (int)a.g.n_rows)) {
             if (sizeof(V) == 4)
                 *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + first);
@@ -440,8 +445,8 @@ struct Rows {
                 *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from + first);
         } else {
 #pragma unroll
-            for (int u = 0; u < N; ++u)
-                if (on<FULL>(u) && has<FULL>(u)) to[u] = from[row_of(u)];
+            for (int u = 0; u < COUNT; ++u)
+                if (on<FULL>(u0 + u) && has<FULL>(u0 + u)) to[u] = from[row_of(u0 + u)];
         }
     }
 
@@ -455,11 +460,11 @@ struct Rows {
                 if (on<FULL>(u) && has<FULL>(u)) row[u] = a.g.rows[place(u)];
         }
         take<FULL>(scores, raw);
-        if (OP != kLogProbs && inputs) {
+        if (OP != kLogProbs && inputs && !LATE) {
             take<FULL>(OP == kChoice ? a.target : a.advantage, main);
             if (OP == kPolicy) {
-                take<FULL>(a.old, old);
-                if (a.reference) take<FULL>(a.reference, reference);
+                take<FULL, HELD>(a.old, old);
+                if (a.reference) take<FULL, HELD>(a.reference, reference);
             }
         }
 #pragma unroll
@@ -498,6 +503,11 @@ struct Rows {
         float part = 0.f, part_loss = 0.f, part_kl = 0.f;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
+            if (LATE && u % 4 == 0 && on<FULL>(u)) {
+                take<FULL, 4>(a.advantage, main + u, u);
+                take<FULL, 4>(a.old, old, u);
+                if (a.reference) take<FULL, 4>(a.reference, reference, u);
+            }
             if (on<FULL>(u)) {
                 const bool live = s[u] != -INFINITY;
                 const Pair32 l = difference(s[u], lse.hi, -lse.lo);
@@ -511,7 +521,7 @@ struct Rows {
                 } else {
                     const float adv = live ? main[u] : 0.f;
                     const bool up = adv > 0.f, taken = adv != 0.f;
-                    const Pair32 x = difference(l.hi, old[u], l.lo);
+                    const Pair32 x = difference(l.hi, old[u % HELD], l.lo);
                     const float past = (x.hi - (up ? a.log_high.hi : a.log_low.hi)) + (fminf(x.lo, 1.f) - (up ? a.log_high.lo : a.log_low.lo));
                     const bool beyond = taken && (up ? past : -past) > 0.f;
                     const float q = beyond ? (up ? a.bound_high : a.bound_low) : exp_of(x);
@@ -521,7 +531,7 @@ struct Rows {
                     clipped += beyond ? 1 : 0;
                     own = -fixed;
                     if (a.reference) {
-                        const float k = live ? p * sum_of(difference(l.hi, reference[u], l.lo)) : 0.f;
+                        const float k = live ? p * sum_of(difference(l.hi, reference[u % HELD], l.lo)) : 0.f;
                         fixed = fmaf(a.kl_coef, k, fixed);
                         own = fmaf(-a.kl_coef, k, own);
                         part_kl += k;
@@ -588,10 +598,10 @@ __device__ __forceinline__ double rescaled(double z, float m, float top) {
 constexpr int kTeamThreads = 256;
 constexpr int kTeamRows = PB_TEAM_ROWS / 32;
 
-// (registers: what keeps most warps on an SM; 3 CTAs of a policy took 37 us over 1M rows in interleaved lists, 4 CTAs with registers
-// spilled 42, as many as fit without a limit 41; of a choice, 4 took 27 us over 2.7M rows, 2 took 33, 5 took 30)
+// (Registers: of a choice, 4 CTAs per SM took 27 us over 2.7M rows, 2 took 33, 5 took 30.  Of a policy over 1M rows in interleaved
+// lists, where what the SMs can look up bounds it, 2 took 35, 3 took 39 and 4 took 37.)
 template <typename T, int OP>
-__global__ void __launch_bounds__(kTeamThreads, OP == kPolicy ? 3 : 4) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
+__global__ void __launch_bounds__(kTeamThreads, OP == kPolicy ? 2 : 4) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
                                                             Totals totals) {
     __shared__ double scratch[kTeamThreads / 32];
     let_next_start();
@@ -954,9 +964,10 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
         early = true;
     }
     if (g.n_blocks) {
-        // threads of a group: as few as still fill the SMs (see block_kernel); a step more than the longest group takes
-        // (its first place is rounded down)
-        const int threads = g.n_blocks >= 148 * 3 ? 256 : g.n_blocks >= 148 * 3 / 2 ? 512 : 1024;
+        // Threads of a group: as few as keep an SM busy, since each warp costs its group as much as five rows: 8 warps where an SM has
+        // three groups (574 groups of 4 700 rows: 27 us, 38 with 16), else 16.  (`most`: the first place is rounded down; with a list
+        // of rows the last step's threads have places that are not used.)
+        const int threads = g.n_blocks >= 148 * 3 ? 256 : 512;
         const int most = (int)(g.block_rows + 7) / 4 * 4 + (g.rows ? threads * kBlockRows : 0);
         const size_t smem = OP == kLogProbs ? 0 : (size_t)most * 8;
         const int2* list = reinterpret_cast<const int2*>(g.blocks);
@@ -967,10 +978,8 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
         };
         if (threads == 256)
             PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false>) : block(block_kernel<T, OP, 256, true>));
-        else if (threads == 512)
-            PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false>) : block(block_kernel<T, OP, 512, true>));
         else
-            PB_TRY(g.rows ? block(block_kernel<T, OP, 1024, false>) : block(block_kernel<T, OP, 1024, true>));
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false>) : block(block_kernel<T, OP, 512, true>));
         slot += (int)g.n_blocks;
         early = true;
     }
