@@ -596,12 +596,13 @@ __device__ __forceinline__ double rescaled(double z, float m, float top) {
 // 1, 2, 4 ... 32 neighbouring lanes have a group, up to eight rows each; the groups of a warp have equal lengths, or nearly,
 // because the layout sorts them by length; sums over a group are shuffles within its lanes.
 constexpr int kTeamThreads = 256;
+__host__ __device__ constexpr int team_ctas(bool policy) { return policy ? 2 : 4; }  // on an SM
 constexpr int kTeamRows = PB_TEAM_ROWS / 32;
 
 // (Registers: of a choice, 4 CTAs per SM took 27 us over 2.7M rows, 2 took 33, 5 took 30.  Of a policy over 1M rows in interleaved
 // lists, where what the SMs can look up bounds it, 2 took 35, 3 took 39 and 4 took 37.)
 template <typename T, int OP>
-__global__ void __launch_bounds__(kTeamThreads, OP == kPolicy ? 2 : 4) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
+__global__ void __launch_bounds__(kTeamThreads, team_ctas(OP == kPolicy)) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
                                                             Totals totals) {
     __shared__ double scratch[kTeamThreads / 32];
     let_next_start();
@@ -880,35 +881,34 @@ int64_t n_rows_of(const pb_objective* o) {
     return o->kind == PB_OBJECTIVE_PREFERENCE ? o->pairs->n_rows : o->groups->n_rows;
 }
 
-// CTAs of a launch whose warps take one task after the other: what the SMs hold at once, or as many as there are tasks.
-constexpr int64_t kWarpGrid = 148 * 4;
-int64_t warp_grid(int64_t warps) { return warps / 8 < kWarpGrid ? (warps + 7) / 8 : kWarpGrid; }
+// CTAs of the launch whose warps take one team task after the other: as many as the SMs hold at once (with more of them, 1M rows in
+// interleaved lists took 34 us for 31), or as there are tasks.
+int64_t team_grid(const pb_groups* g, bool policy) {
+    const int64_t most = 148 * team_ctas(policy);
+    return g->n_team_warps < most * (kTeamThreads / 32) ? (g->n_team_warps + kTeamThreads / 32 - 1) / (kTeamThreads / 32) : most;
+}
 
 // (two CTAs per SM: with more, of which each looks up scores in another window of rows, L1 holds too little of each)
 int64_t n_parts_of(const pb_pairs* p) {
     const int64_t tasks = p->n_slices > p->n_chunks ? p->n_slices : p->n_chunks;
     return tasks < 148 * 2 * kPairWarps ? (tasks + kPairWarps - 1) / kPairWarps : 148 * 2;
 }
-int64_t n_parts_of(const pb_groups* g) {
-    return warp_grid(g->n_team_warps) + g->n_blocks + g->n_pieces;
-}
+int64_t n_parts_of(const pb_groups* g, bool policy) { return team_grid(g, policy) + g->n_blocks + g->n_pieces; }
 
 // Scratch: the ticket; of pairs, counts and sums of the rows in several chunks; of groups, the sums of pieces; the totals.
 constexpr int64_t kTicketBytes = 16;
 int64_t sums_bytes(const pb_pairs* p) { return (int64_t)align_up((size_t)p->n_split * 4, 8) + (p->n_split ? p->n_chunks * 8 : 0); }
 int64_t sums_bytes(const pb_groups* g) { return g->n_pieces * (int64_t)sizeof(PieceSums); }
-template <typename L>
-int64_t scratch_bytes(const L* layout) {
-    return kTicketBytes + sums_bytes(layout) + n_parts_of(layout) * (int64_t)sizeof(Part);
-}
+// (a layout's scratch is the same whatever the objective)
+int64_t scratch_bytes(const pb_pairs* p) { return kTicketBytes + sums_bytes(p) + n_parts_of(p) * (int64_t)sizeof(Part); }
+int64_t scratch_bytes(const pb_groups* g) { return kTicketBytes + sums_bytes(g) + n_parts_of(g, false) * (int64_t)sizeof(Part); }
 int64_t scratch_bytes(const pb_objective* o) {
     return o->kind == PB_OBJECTIVE_PREFERENCE ? scratch_bytes(o->pairs) : scratch_bytes(o->groups);
 }
-template <typename L>
-Totals totals_of(const L* layout, double scale, float* loss, float* kl, int64_t* clipped, char* scratch) {
+Totals totals_of(int64_t n_parts, int64_t sums, double scale, float* loss, float* kl, int64_t* clipped, char* scratch) {
     const bool want = loss || kl || clipped;
-    return Totals{want ? reinterpret_cast<unsigned*>(scratch) : nullptr, reinterpret_cast<Part*>(scratch + kTicketBytes + sums_bytes(layout)),
-                  (int)n_parts_of(layout), scale, loss, kl, clipped};
+    return Totals{want ? reinterpret_cast<unsigned*>(scratch) : nullptr, reinterpret_cast<Part*>(scratch + kTicketBytes + sums),
+                  (int)n_parts, scale, loss, kl, clipped};
 }
 
 // A launch; `early`: it may begin before the one in front of it on the stream has ended, and waits for that itself.
@@ -958,7 +958,7 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
     const bool words = bits % 16 == 0 && ((uintptr_t)scores | (uintptr_t)out) % (4 * sizeof(T)) == 0;
     bool early = false;  // the first launch waits for what is before it on the stream, the others may overlap with it
     if (g.n_team_warps) {
-        const int64_t grid = warp_grid(g.n_team_warps);
+        const int64_t grid = team_grid(&g, OP == kPolicy);
         PB_CUDA_TRY(launch(team_kernel<T, OP>, grid, kTeamThreads, 0, early, stream, a, slot, scores, out, totals));
         slot += (int)grid;
         early = true;
@@ -1000,10 +1000,12 @@ int launch_objective(const pb_objective* o, const void* scores_, void* grad_, fl
     T* grad = static_cast<T*>(grad_);
     char* scratch = static_cast<char*>(scratch_);
     if (o->kind == PB_OBJECTIVE_PREFERENCE)
-        return launch_pairs<T>(o, scores, grad, totals_of(o->pairs, o->scale, loss, kl, clipped, scratch), scratch, stream);
+        return launch_pairs<T>(o, scores, grad, totals_of(n_parts_of(o->pairs), sums_bytes(o->pairs), o->scale, loss, kl, clipped, scratch), scratch,
+                               stream);
     const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(o->clip_high)), split(log1p(-o->clip_low)),
                       (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
-    const Totals totals = totals_of(o->groups, o->scale, loss, kl, clipped, scratch);
+    const Totals totals = totals_of(n_parts_of(o->groups, o->kind == PB_OBJECTIVE_POLICY), sums_bytes(o->groups), o->scale, loss, kl, clipped,
+                                    scratch);
     if (o->kind == PB_OBJECTIVE_CHOICE) return launch_groups<T, kChoice>(a, scores, grad, totals, scratch, stream);
     return launch_groups<T, kPolicy>(a, scores, grad, totals, scratch, stream);
 }

@@ -235,10 +235,11 @@ def _lay_out_groups(group: torch.Tensor) -> dict:
     heads[1:] = group[1:] != group[:-1]
     starts = torch.nonzero(heads)[:, 0]
     lengths = torch.diff(starts, append=starts.new_full((1,), n))
-    # short ones by length (a warp's groups should be alike), the others by kind: in the order of their rows
+    # short ones by length (a warp's groups should be alike), a CTA's longest first, long ones in the order of their rows
     limits = torch.tensor(_TEAM_ROWS + (_BLOCK_ROWS,), device=dev)
     kind = torch.bucketize(lengths, limits)
-    key = torch.where(kind < len(_TEAM_ROWS), lengths, kind + _TEAM_ROWS[-1])
+    key = torch.where(kind < len(_TEAM_ROWS), lengths,
+                      torch.where(kind == len(_TEAM_ROWS), 2 * _BLOCK_ROWS - lengths, 2 * _BLOCK_ROWS))
     table = torch.stack([starts, lengths], 1).to(torch.int32)[torch.sort(key, stable=True).indices]
     count = torch.bincount(kind, minlength=len(limits) + 1).tolist()
     parts = list(torch.split(table, count))
