@@ -407,6 +407,8 @@ typedef struct pb_round_log_header {
 #define PB_OBJECTIVE_CHOICE 1
 #define PB_OBJECTIVE_POLICY 2
 
+#define PB_OBJECTIVE_MOST_ROWS 2147418112ll /* 2^31 - 2^16; rows, and items of pairs */
+
 #define PB_SCORE_F32 0
 #define PB_SCORE_F16 1
 #define PB_SCORE_BF16 2
@@ -481,7 +483,7 @@ typedef struct pb_objective {
 int64_t pb_objective_struct_bytes(int64_t which);
 
 /* Scratch of an evaluation, 16-byte aligned.  It has to be zero when it is first used; what a call needs to be
- * zero it leaves so.  Evaluations that may run at the same time need one each. */
+ * zero it leaves so, unless it fails.  Evaluations that may run at the same time need one each. */
 int64_t pb_objective_workspace_bytes(const pb_objective* o);
 
 /* Gradient with respect to the scores [n_rows] (of the scores' type), the loss and, for a policy, the
@@ -501,7 +503,8 @@ int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_typ
 int pb_round_begin_objective(const pb_train_state* st, const pb_objective* o, int64_t apply_previous, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
-/* pb_loop_submit with such a round; objective and workspace stay the same for all rounds of a loop. */
+/* pb_loop_submit with such a round.  What the descriptor says stays the same as long as its address and the
+ * workspace's do (a round captured with them is replayed). */
 int pb_loop_submit_objective(void* loop, const pb_train_state* st, const pb_objective* o, void* workspace,
                              int64_t workspace_bytes, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
                              int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream);

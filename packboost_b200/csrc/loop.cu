@@ -18,6 +18,7 @@ struct RoundLoop {
     cudaGraphExec_t exec = nullptr;
     bool no_graph = false;  // a capture failed: rounds are launched one kernel at a time
     int64_t graph_k = 0, graph_launches = 0, replays = 0;
+    const void *graph_objective = nullptr, *graph_workspace = nullptr;  // what the captured round learns from
     ~RoundLoop() {
         if (exec) cudaGraphExecDestroy(exec);
         for (auto e : logged)
@@ -63,6 +64,8 @@ int capture_round(RoundLoop* loop, const pb_train_state* st, const RoundLoss& lo
     if (rc) return rc;
     if (e != cudaSuccess) return fail_cuda(e, "round graph");
     loop->graph_k = k;
+    loop->graph_objective = loss.objective;
+    loop->graph_workspace = loss.workspace;
     loop->graph_launches = pb_launch_count() - before;
     return PB_OK;
 }
@@ -100,7 +103,8 @@ static int submit_round(void* loop_, const pb_train_state* st, const RoundLoss& 
     PB_CUDA_TRY(cudaMemcpyAsync(lists_dev, lists_host, (size_t)(st->max_depth * 3 * k) * 4, cudaMemcpyHostToDevice, stream));
     // the launches of a round are the same every time: from the second round on they are replayed
     const bool graph = use_graph && apply_previous;
-    if (graph && !loop->no_graph && (!loop->exec || loop->graph_k != k)) {
+    if (graph && !loop->no_graph &&
+        (!loop->exec || loop->graph_k != k || loop->graph_objective != loss.objective || loop->graph_workspace != loss.workspace)) {
         if (loop->exec) cudaGraphExecDestroy(loop->exec);
         loop->exec = nullptr;
         if (capture_round(loop, st, loss, lists_dev, k) != PB_OK) {

@@ -438,7 +438,7 @@ struct Rows {
     // COUNT values from the u0-th on
     template <bool FULL, int COUNT = N, typename V>
     __device__ __forceinline__ void take(const V* from, V* to, int u0 = 0) const {
-        if (VECTOR && words && (FULL || first + 3 < (int)a.g.n_rows)) {
+        if (VECTOR && words && (FULL || (first < end && first + 3 < (int)a.g.n_rows))) {
             if (sizeof(V) == 4)
                 *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + first);
             else
@@ -820,10 +820,11 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
 // ---- launches ---------------------------------------------------------------------------------------
 
 constexpr int64_t kMost = (1ll << 31) - 1;
+constexpr int64_t kMostRows = PB_OBJECTIVE_MOST_ROWS;  // (a CTA's places past the last row are still 32-bit numbers)
 
 int check_groups(const pb_groups* g) {
     PB_REQUIRE(g != nullptr, "groups are null");
-    PB_REQUIRE(g->n_rows >= 0 && g->n_rows < kMost, "n_rows=%lld out of range", (long long)g->n_rows);
+    PB_REQUIRE(g->n_rows >= 0 && g->n_rows <= kMostRows, "n_rows=%lld out of range", (long long)g->n_rows);
     PB_REQUIRE(g->n_groups >= 0 && g->n_groups <= g->n_rows, "n_groups=%lld out of range", (long long)g->n_groups);
     PB_REQUIRE((g->n_groups == 0) == (g->n_rows == 0), "rows without a group");
     PB_REQUIRE(g->n_team_warps >= 0 && g->n_team_warps < kMost / 32 && g->n_pieces >= 0 && g->n_pieces < kMost && g->n_blocks >= 0 &&
@@ -840,7 +841,7 @@ int check_groups(const pb_groups* g) {
 
 int check_pairs(const pb_pairs* p) {
     PB_REQUIRE(p != nullptr, "pairs are null");
-    PB_REQUIRE(p->n_rows >= 0 && p->n_rows < kMost, "n_rows=%lld out of range", (long long)p->n_rows);
+    PB_REQUIRE(p->n_rows >= 0 && p->n_rows <= kMostRows, "n_rows=%lld out of range", (long long)p->n_rows);
     PB_REQUIRE(p->n_slices >= 0 && p->n_slices < kMost / 64 && p->n_chunks >= 0 && p->n_chunks < kMost && p->n_split >= 0 &&
                    2 * p->n_split <= p->n_chunks,
                "counts of the pairs' layout are out of range");

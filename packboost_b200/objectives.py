@@ -40,7 +40,7 @@ import torch
 from . import backends as B
 
 _SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_MOST = (1 << 31) - 2    # rows, and items (two per pair): 32-bit indices, bit 31 of a row id is a flag
+_MOST = (1 << 31) - (1 << 16)    # rows, and items (two per pair): 32-bit numbers
 _PREFERENCE, _CHOICE, _POLICY = 0, 1, 2
 
 
@@ -163,13 +163,13 @@ def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict:
            "slices": torch.stack([column, tall[:, 0] | (tall[:, 1] << 16)], 1).to(torch.int32),
            "slice_rows": torch.stack([lanes, have[:, 0] | (have[:, 1] << 16)], 1).to(torch.int32)}
     first_many = _SLICE_ROWS * int(tall.sum())
-    if first_many > _MOST:
-        raise ValueError("more items than 32-bit numbers count")
 
     many = torch.nonzero(~few)[:, 0]
     size = n_chosen[many] + n_rejected[many]
     begin = first_many + size.cumsum(0) - size
     n_items = first_many + int(size.sum())
+    if n_items > _MOST:
+        raise ValueError("more items than 32-bit numbers count")
     # where an item goes: base + stride * its rank among its row's items of its side
     base = torch.empty((n_rows, 2), dtype=torch.int64, device=dev)
     stride = torch.ones(n_rows, dtype=torch.int64, device=dev)
@@ -563,9 +563,14 @@ def _trainer_groups(group, n_rows: int, era_offsets: np.ndarray, order, device) 
     return RowGroups(group if order is None else group[torch.from_numpy(order).to(group.device)], n_groups, device=device)
 
 
-def _trainer_rows(values, name: str, n_rows: int, order, device) -> torch.Tensor:
+def _trainer_rows(values, name: str, n_rows: int, order, device, where: torch.Tensor | None = None) -> torch.Tensor:
+    """A row's number of a fit, in the trainer's order; finite (``where`` it is looked at: no score of a fit is masked)."""
     values = _numbers(values, name, n_rows, device).to(torch.float32).contiguous()
-    return values if order is None else values[torch.from_numpy(order).to(device)]
+    if order is not None:
+        values = values[torch.from_numpy(order).to(device)]
+    if not bool((torch.isfinite(values) if where is None else torch.isfinite(values) | ~where).all()):
+        raise ValueError(f"{name} must be finite")
+    return values
 
 
 class PreferenceObjective:
@@ -599,6 +604,8 @@ class ChoiceObjective:
     def _bind(self, n_rows: int, era_offsets, order, device) -> _FitObjective:
         groups = _trainer_groups(self.group, n_rows, era_offsets, order, device)
         target = _trainer_rows(self.target, "target", n_rows, order, device)
+        if bool((target < 0).any()):
+            raise ValueError("targets must not be negative")
         return _FitObjective(_choice_struct(groups, target, self.reduction), groups, (target,))
 
 
@@ -612,7 +619,10 @@ class PolicyObjective:
 
     def _bind(self, n_rows: int, era_offsets, order, device) -> _FitObjective:
         groups = _trainer_groups(self.group, n_rows, era_offsets, order, device)
-        rows = [None if v is None else _trainer_rows(v, name, n_rows, order, device)
-                for v, name in ((self.advantage, "advantage"), (self.old_log_probs, "old_log_probs"),
-                                (self.reference_log_probs, "reference_log_probs"))]
-        return _FitObjective(_policy_struct(groups, *rows, *self.options), groups, tuple(rows))
+        advantage = _trainer_rows(self.advantage, "advantage", n_rows, order, device)
+        old = _trainer_rows(self.old_log_probs, "old_log_probs", n_rows, order, device, advantage != 0)
+        reference = self.reference_log_probs
+        if reference is not None:
+            reference = _trainer_rows(reference, "reference_log_probs", n_rows, order, device)
+        rows = (advantage, old, reference)
+        return _FitObjective(_policy_struct(groups, *rows, *self.options), groups, rows)

@@ -298,6 +298,43 @@ def test_streams_and_graphs():
     assert all(torch.equal(o, w) for o, w in zip(outs[0], want_y))
 
 
+def test_threads_share_layouts():
+    import threading
+    x, groups, a, old, pairs = _problem(8)
+    want = _all(x, groups, a, old, pairs)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = _all(x, groups, a, old, pairs)
+                stream.synchronize()
+                if not all(torch.equal(g, w) for g, w in zip(got, want)):
+                    wrong.append(1)
+
+    shared = torch.cuda.Stream()
+    threads = [threading.Thread(target=work, args=(s,)) for s in (shared, shared, torch.cuda.Stream(), torch.cuda.Stream())]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_many_options_and_streams():
+    """More descriptors and more streams than a layout keeps."""
+    x, groups, a, old, pairs = _problem(9, 9500)
+    want = O.preference_loss(x, pairs, beta=1.0)
+    for i in range(70):
+        O.preference_loss(x, pairs, beta=0.5 + i / 100)
+    for _ in range(20):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = O.preference_loss(x, pairs, beta=1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(got.loss, want.loss) and torch.equal(got.grad, want.grad)
+
+
 def test_a_layout_may_go_while_its_call_runs():
     want = _all(*_problem(7))
     side = torch.cuda.Stream()
@@ -493,6 +530,12 @@ def test_refused_fits():
             b.fit(X, None, era, num_rounds=1, objective=objective)
     with pytest.raises(ValueError):
         b.fit(X, None, era, num_rounds=1)
+    z, one, bad = np.zeros(200), np.ones(200), np.full(200, np.nan)
+    for objective in (O.ChoiceObjective(bad), O.ChoiceObjective(-one), O.PolicyObjective(bad, z), O.PolicyObjective(one, bad),
+                      O.PolicyObjective(z, z, reference_log_probs=bad), O.PolicyObjective(z, z, reference_log_probs=bad, kl_coef=1.0)):
+        with pytest.raises(ValueError):
+            b.fit(X, None, era, num_rounds=1, objective=objective)
+    b.fit(X, None, era, num_rounds=2, objective=O.PolicyObjective(z, bad))    # (nothing was taken: nothing is looked at)
     x = torch.zeros(200, device="cuda")
     with pytest.raises(ValueError):
         O.choice_loss(x, O.RowGroups([0] * 200), x.cpu())

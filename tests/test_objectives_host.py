@@ -167,7 +167,7 @@ def test_layout_of_groups(lengths, mixed):
     (([0.0], [1], 3), {}, TypeError), (([True], [1], 3), {}, TypeError), (([[0]], [[1]], 3), {}, ValueError),
     (([0, 1], [1], 3), {}, ValueError), (([0], [3], 3), {}, ValueError), (([-1], [0], 3), {}, ValueError),
     (([1], [1], 3), {}, ValueError), (([0], [1], -1), {}, ValueError), (([0], [1], 2.0), {}, TypeError),
-    (([0], [1], 1 << 31), {}, ValueError), (([0], [1], True), {}, TypeError),
+    (([0], [1], 1 << 31), {}, ValueError), (([0], [1], O._MOST + 1), {}, ValueError), (([0], [1], True), {}, TypeError),
     (([0], [1], 2), {"weight": [-1.0]}, ValueError), (([0], [1], 2), {"weight": [float("nan")]}, ValueError),
     (([0], [1], 2), {"weight": [1.0, 2.0]}, ValueError), (([0], [1], 2), {"weight": [1e300]}, ValueError),
     (([0], [1], 2), {"reference": [1.0]}, ValueError), (([0], [1], 2), {"reference": [1j, 2]}, TypeError),
@@ -257,7 +257,7 @@ def test_library_refuses_bad_descriptors():
     refused(B.Objective(kind=9), "unknown objective")
     refused(B.Objective(kind=0), "pairs are null")
     refused(B.Objective(kind=1), "groups are null")
-    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_rows=1 << 31), "n_rows"), (dict(n_slices=1 << 26), "range"),
+    for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_rows=O._MOST + 1), "n_rows"), (dict(n_slices=1 << 26), "range"),
                       (dict(n_slices=0), "not laid out"), (dict(slices=None), "null"), (dict(slice_rows=None), "null"),
                       (dict(other=None), "null"), (dict(n_chunks=1), "null"), (dict(n_chunks=-1), "range"),
                       (dict(n_split=1), "range"), (dict(slices=20), "aligned"), (dict(offset=20), "aligned"), (dict(n_chunks=1, chunks=24), "aligned")):
