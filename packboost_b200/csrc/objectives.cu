@@ -76,11 +76,25 @@ struct Totals {
 template <int THREADS>
 __device__ __forceinline__ void put_totals(const Totals& out, int slot, double loss, double kl, int clipped, bool policy, double* scratch) {
     if (!out.ticket) return;
+    constexpr int kWarps = THREADS / 32;
+    __shared__ Part s_part[kWarps];
     __shared__ int s_last;
-    Part mine{cta_sum<THREADS>(loss, scratch), 0.0, 0.0};
+    const int lane = threadIdx.x & 31;
+    loss = warp_sum(loss);
     if (policy) {
-        mine.kl = cta_sum<THREADS>(kl, scratch);
-        mine.clipped = cta_sum<THREADS>((double)clipped, scratch);
+        kl = warp_sum(kl);
+        clipped = __reduce_add_sync(0xFFFFFFFFu, clipped);
+    }
+    if (lane == 0) s_part[threadIdx.x >> 5] = Part{loss, kl, (double)clipped};
+    __syncthreads();
+    Part mine{0.0, 0.0, 0.0};
+    if (threadIdx.x < 32) {
+        if (lane < kWarps) mine = s_part[lane];
+        mine.loss = warp_sum(mine.loss);
+        if (policy) {
+            mine.kl = warp_sum(mine.kl);
+            mine.clipped = warp_sum(mine.clipped);
+        }
     }
     if (out.n_parts > 1) {
         if (threadIdx.x == 0) {
@@ -753,8 +767,8 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
 // ---- long groups: many CTAs each ----
 //
 // Pieces of up to 2048 rows; the sums of a group's pieces go through memory from one launch to the next: sums of
-// exponentials, then shares, then the gradient.  The rows are read again each time, from L2 mostly, while the launch
-// before still runs.
+// exponentials, then (of a policy; a choice's are its targets, known at once) shares, then the gradient.  The rows are read
+// again each time, from L2 mostly, while the launch before still runs.
 struct PieceSums {
     double z, share;
     float m, unused;
@@ -779,8 +793,16 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     rows.low = piece.x;
     rows.end = piece.x + piece.y;
     rows.used = (piece.y + kPieceThreads - 1) / kPieceThreads;
-    rows.template load<false>(scores, STEP != kPieceMass);
+    rows.template load<false>(scores, STEP != kPieceMass || OP == kChoice);
+    constexpr bool kTotalsAtEnd = OP == kChoice;
     if (STEP == kPieceMass) {
+        if (OP == kChoice) {
+            double targets = 0.0;
+#pragma unroll
+            for (int u = 0; u < kPieceRows; ++u) targets += (double)rows.main[u];
+            targets = cta_sum<kPieceThreads>(targets, scratch);
+            if (threadIdx.x == 0) pieces[blockIdx.x].share = targets;
+        }
         float m = rows.largest();
         const float wm = warp_max(m);
         double z = warp_sum(rows.template mass<false>(wm));
@@ -825,6 +847,7 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     double share = 0.0;
     for (int k = threadIdx.x; k < count; k += kPieceThreads) share += pieces[first + k].share;
     rows.template gradient<false>((float)cta_sum<kPieceThreads>(share, scratch), out);
+    if (kTotalsAtEnd) put_totals<kPieceThreads>(totals, slot0 + blockIdx.x, rows.loss, 0.0, 0, false, scratch);
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
@@ -997,7 +1020,7 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
     if (g.n_pieces) {
         PieceSums* sums = reinterpret_cast<PieceSums*>(scratch + kTicketBytes);
         PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, early, stream, a, sums, slot, scores, out, totals));
-        if (OP != kLogProbs)
+        if (OP == kPolicy)
             PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
         PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceOut>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
     }
