@@ -817,6 +817,8 @@ class PackBoost:
         # torch tensors (device-resident, or pinned host memory) are consumed without conversion
         on_device = isinstance(X, torch.Tensor)
         X_np = X.detach() if on_device else np.asarray(X)
+        if objective is not None and not hasattr(objective, "_bind"):
+            raise TypeError("objective must be a PreferenceObjective, ChoiceObjective or PolicyObjective")
         if y is None and objective is not None:
             y = np.zeros(X_np.shape[0], dtype=np.float32)
         # (targets that are on the GPU stay there: they are gathered and copied on the device)

@@ -6,8 +6,8 @@
 // whether a policy's ratio is beyond its border must not hang on the rounding of a sum over a whole era, and
 // with a reference near the policy the difference of the two log-probabilities is all there is.
 //
-// All of it is bound by the instructions that the SMs issue, not by memory, until it is written tightly: a
-// row of a policy is 20 bytes and about a hundred instructions.
+// Groups of rows in order are bound by the instructions that the SMs issue more than by memory: 32 rows of a policy are 640
+// bytes and some 180 instructions of a warp.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -447,7 +447,7 @@ struct Rows {
     bool words;                   // VECTOR: all arrays begin on the border of a word
     int row[N];                   // only with a list of rows
     // (s becomes p, main (target or advantage) the fixed part; of more than four rows, the three inputs of a policy come four rows
-    // at a time: with all of them at once, half as many warps fit on an SM)
+    // at a time: interleaved lists of 1M rows took 39 us with all at once, which spills, and 35 so)
     static constexpr bool LATE = OP == kPolicy && N > 4;
     static constexpr int HELD = LATE ? 4 : N;
     float s[N], main[N], old[HELD], reference[HELD];
@@ -632,8 +632,8 @@ constexpr int kTeamRows = PB_TEAM_ROWS / 32;
 // (Registers: of a choice, 4 CTAs per SM took 27 us over 2.7M rows, 2 took 33, 5 took 30.  Of a policy over 1M rows in interleaved
 // lists, where what the SMs can look up bounds it, 2 took 35, 3 took 39 and 4 took 37.)
 template <typename T, int OP>
-__global__ void __launch_bounds__(kTeamThreads, team_ctas(OP == kPolicy)) team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out,
-                                                            Totals totals) {
+__global__ void __launch_bounds__(kTeamThreads, team_ctas(OP == kPolicy))
+    team_kernel(GroupArgs a, int slot0, const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
     let_next_start();
     const int lane = threadIdx.x & 31;
     double loss = 0.0, kl = 0.0;
@@ -700,72 +700,74 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
     __shared__ float s_m[THREADS / 32];
     __shared__ double s_z[THREADS / 32], scratch[THREADS / 32];
     let_next_start();
-    const int2 group = list[blockIdx.x];
     constexpr int kStep = THREADS * kBlockRows;
     using Four = Rows<T, OP, kBlockRows, VECTOR>;
-    const int begin = VECTOR ? group.x & ~3 : group.x, end = group.x + group.y;
-    // all steps of the group in turn: f(rows, step, whether all rows are the group's)
-    auto steps = [&](auto f) {
-        for (int at = begin, k = 0; at < end; at += kStep, ++k) {
-            Four rows(a);
-            rows.first = at + (int)threadIdx.x * (VECTOR ? kBlockRows : 1);
-            rows.stride = THREADS;
-            rows.low = group.x;
-            rows.end = end;
-            rows.used = (end - at + THREADS - 1) / THREADS;
-            rows.words = words;
-            if (at >= group.x && at + kStep <= end)
-                f(rows, k, std::true_type());
-            else
-                f(rows, k, std::false_type());
-        }
-    };
-    float m = -INFINITY;
-    double z = 0.0;
-    steps([&](Four& rows, int, auto full) {
-        rows.template load<decltype(full)::value>(scores, false);
-        const float top = fmaxf(m, rows.largest());
-        z = rescaled(z, m, top) + rows.template mass<decltype(full)::value>(top);
-        m = top;
-    });
-    const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
-    if (OP == kLogProbs) {
-        steps([&](Four& rows, int, auto full) {
-            rows.template load<decltype(full)::value>(scores, false);
-            rows.template log_probs<decltype(full)::value>(lse, out);
-        });
-        wait_for_previous();
-        return;
-    }
-    double loss = 0.0, kl = 0.0, share = 0.0;
-    int clipped = 0;
     float4* const kept_p = kept4 + threadIdx.x;
     float4* const kept_fixed = kept4 + most / 4 + threadIdx.x;
-    steps([&](Four& rows, int k, auto full) {
-        rows.template load<decltype(full)::value>(scores, true);
-        rows.template terms<decltype(full)::value>(lse);
-        if (decltype(full)::value || (k * THREADS + (int)threadIdx.x) * 4 < most) {
-            kept_p[k * THREADS] = make_float4(rows.s[0], rows.s[1], rows.s[2], rows.s[3]);
-            kept_fixed[k * THREADS] = make_float4(rows.main[0], rows.main[1], rows.main[2], rows.main[3]);
+    double loss = 0.0, kl = 0.0;
+    int clipped = 0;
+    for (int g = blockIdx.x; g < (int)a.g.n_blocks; g += gridDim.x) {
+        const int2 group = list[g];
+        const int begin = VECTOR ? group.x & ~3 : group.x, end = group.x + group.y;
+        // all steps of the group in turn: f(rows, step, whether all rows are the group's)
+        auto steps = [&](auto f) {
+            for (int at = begin, k = 0; at < end; at += kStep, ++k) {
+                Four rows(a);
+                rows.first = at + (int)threadIdx.x * (VECTOR ? kBlockRows : 1);
+                rows.stride = THREADS;
+                rows.low = group.x;
+                rows.end = end;
+                rows.used = (end - at + THREADS - 1) / THREADS;
+                rows.words = words;
+                if (at >= group.x && at + kStep <= end)
+                    f(rows, k, std::true_type());
+                else
+                    f(rows, k, std::false_type());
+            }
+        };
+        float m = -INFINITY;
+        double z = 0.0, share = 0.0;
+        steps([&](Four& rows, int, auto full) {
+            rows.template load<decltype(full)::value>(scores, false);
+            const float top = fmaxf(m, rows.largest());
+            z = rescaled(z, m, top) + rows.template mass<decltype(full)::value>(top);
+            m = top;
+        });
+        const double lse = cta_log_sum<THREADS>(m, z, s_m, s_z);
+        if (OP == kLogProbs) {
+            steps([&](Four& rows, int, auto full) {
+                rows.template load<decltype(full)::value>(scores, false);
+                rows.template log_probs<decltype(full)::value>(lse, out);
+            });
+            __syncthreads();  // (the next group's sums go where this one's were)
+            continue;
         }
-        loss += rows.loss;
-        kl += rows.kl;
-        share += rows.share;
-        clipped += rows.clipped;
-    });
-    const float total = (float)cta_sum<THREADS>(share, scratch);
-    steps([&](Four& rows, int k, auto full) {
-        if (!decltype(full)::value && (k * THREADS + (int)threadIdx.x) * 4 >= most) return;
-        *reinterpret_cast<float4*>(rows.s) = kept_p[k * THREADS];
-        *reinterpret_cast<float4*>(rows.main) = kept_fixed[k * THREADS];
-        if (!VECTOR && a.g.rows) {
+        steps([&](Four& rows, int k, auto full) {
+            rows.template load<decltype(full)::value>(scores, true);
+            rows.template terms<decltype(full)::value>(lse);
+            if (decltype(full)::value || (k * THREADS + (int)threadIdx.x) * 4 < most) {
+                kept_p[k * THREADS] = make_float4(rows.s[0], rows.s[1], rows.s[2], rows.s[3]);
+                kept_fixed[k * THREADS] = make_float4(rows.main[0], rows.main[1], rows.main[2], rows.main[3]);
+            }
+            loss += rows.loss;
+            kl += rows.kl;
+            share += rows.share;
+            clipped += rows.clipped;
+        });
+        const float total = (float)cta_sum<THREADS>(share, scratch);
+        steps([&](Four& rows, int k, auto full) {
+            if (!decltype(full)::value && (k * THREADS + (int)threadIdx.x) * 4 >= most) return;
+            *reinterpret_cast<float4*>(rows.s) = kept_p[k * THREADS];
+            *reinterpret_cast<float4*>(rows.main) = kept_fixed[k * THREADS];
+            if (!VECTOR && a.g.rows) {
 #pragma unroll
-            for (int u = 0; u < kBlockRows; ++u)
-                if (rows.template has<decltype(full)::value>(u)) rows.row[u] = a.g.rows[rows.place(u)];
-        }
-        rows.template gradient<decltype(full)::value>(total, out);
-    });
-    put_totals<THREADS>(totals, slot0 + blockIdx.x, loss, kl, clipped, OP == kPolicy);
+                for (int u = 0; u < kBlockRows; ++u)
+                    if (rows.template has<decltype(full)::value>(u)) rows.row[u] = a.g.rows[rows.place(u)];
+            }
+            rows.template gradient<decltype(full)::value>(total, out);
+        });
+    }
+    if (OP != kLogProbs) put_totals<THREADS>(totals, slot0 + blockIdx.x, loss, kl, clipped, OP == kPolicy);
     wait_for_previous();
 }
 
@@ -932,7 +934,10 @@ int64_t n_parts_of(const pb_pairs* p) {
     const int64_t tasks = p->n_slices > p->n_chunks ? p->n_slices : p->n_chunks;
     return tasks < 148 * 2 * kPairWarps ? (tasks + kPairWarps - 1) / kPairWarps : 148 * 2;
 }
-int64_t n_parts_of(const pb_groups* g, bool policy) { return team_grid(g, policy) + g->n_blocks + g->n_pieces; }
+// CTAs of the launch for longer groups: one each, up to so many that the totals are few against the rows.
+int64_t block_grid(const pb_groups* g) { return g->n_blocks < 148 * 16 ? g->n_blocks : 148 * 16; }
+
+int64_t n_parts_of(const pb_groups* g, bool policy) { return team_grid(g, policy) + block_grid(g) + g->n_pieces; }
 
 // Scratch: the ticket; of pairs, counts and sums of the rows in several chunks; of groups, the sums of pieces; the totals.
 constexpr int64_t kTicketBytes = 16;
@@ -1026,14 +1031,14 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
         const int2* list = reinterpret_cast<const int2*>(g.blocks);
         auto block = [&](auto kernel) -> int {
             PB_TRY(allow_shared(kernel, smem));
-            PB_CUDA_TRY(launch(kernel, g.n_blocks, threads, smem, early, stream, a, list, most, words, slot, scores, out, totals));
+            PB_CUDA_TRY(launch(kernel, block_grid(&g), threads, smem, early, stream, a, list, most, words, slot, scores, out, totals));
             return PB_OK;
         };
         if (threads == 256)
             PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false>) : block(block_kernel<T, OP, 256, true>));
         else
             PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false>) : block(block_kernel<T, OP, 512, true>));
-        slot += (int)g.n_blocks;
+        slot += (int)block_grid(&g);
         early = true;
     }
     if (g.n_pieces) {

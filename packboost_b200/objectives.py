@@ -293,15 +293,19 @@ class _Layout:
         self._count = torch.empty((), dtype=torch.int64, device=device)
         stream = torch.cuda.current_stream(device)
         self._stream = stream.cuda_stream
+        self._streams = {self._stream}
         stream.synchronize()
 
     def _used_now(self) -> int:
         """The current stream of the layout's device, which must be the current one."""
         stream = torch._C._cuda_getCurrentRawStream(self.device.index)
-        if stream != self._stream:
+        if stream not in self._streams:
+            if len(self._streams) >= 64:
+                self._streams = {self._stream}
             current = torch.cuda.current_stream()
-            for t in self._tensors:
+            for t in self._tensors:   # (once for a stream: what counts is where it stands when they are freed)
                 t.record_stream(current)
+            self._streams.add(stream)
         return stream
 
     def _room(self, stream: int) -> torch.Tensor:
@@ -398,8 +402,9 @@ def _scale(reduction: str, total: float, what: str) -> float:
 def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) -> B.Objective:
     beta, smoothing = float(beta), float(label_smoothing)
     options = (beta, smoothing, kind, reduction)
-    if options in pairs._structs:
-        return pairs._structs[options]
+    kept = pairs._structs.get(options)
+    if kept is not None:
+        return kept
     if not (beta > 0 and math.isfinite(beta)):
         raise ValueError("beta must be positive")
     if not 0 <= smoothing < 0.5:
@@ -415,10 +420,11 @@ def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) 
 
 def _choice_struct(groups: RowGroups, target: torch.Tensor, reduction) -> B.Objective:
     options = (_CHOICE, reduction)
-    if options not in groups._structs:
-        _kept_struct(groups, options, B.Objective(kind=_CHOICE, groups=C.pointer(groups._struct), target=16,
-                                                  scale=_scale(reduction, groups.n_groups, "groups")))
-    struct = B.Objective.from_buffer_copy(groups._structs[options])
+    kept = groups._structs.get(options)
+    if kept is None:
+        kept = _kept_struct(groups, options, B.Objective(kind=_CHOICE, groups=C.pointer(groups._struct), target=16,
+                                                         scale=_scale(reduction, groups.n_groups, "groups")))
+    struct = B.Objective.from_buffer_copy(kept)
     struct.target = target.data_ptr()
     return struct
 
@@ -427,17 +433,18 @@ def _policy_struct(groups: RowGroups, advantage, old, reference, clip, kl_coef, 
     low, high = clip
     low, high, kl = float(low), float(high), float(kl_coef)
     options = (_POLICY, low, high, kl, reduction)
-    if options not in groups._structs:
+    kept = groups._structs.get(options)
+    if kept is None:
         if not (0 <= low <= 1 and high >= 0):
             raise ValueError("clip must be (low, high) with low in [0, 1] and high not negative")
         if not math.isfinite(kl):
             raise ValueError("kl_coef must be finite")
-        _kept_struct(groups, options, B.Objective(
+        kept = _kept_struct(groups, options, B.Objective(
             kind=_POLICY, groups=C.pointer(groups._struct), advantage=16, old=16, reference=16, clip_low=low, clip_high=high,
             kl_coef=kl, scale=_scale(reduction, groups.n_groups, "groups")))
     if reference is None and kl:
         raise ValueError("kl_coef needs reference_log_probs")
-    struct = B.Objective.from_buffer_copy(groups._structs[options])
+    struct = B.Objective.from_buffer_copy(kept)
     struct.advantage, struct.old = advantage.data_ptr(), old.data_ptr()
     struct.reference = None if reference is None else reference.data_ptr()
     return struct

@@ -150,6 +150,31 @@ def test_groups(lengths, dtype, mixed):
             assert_close(got.grad, grad, err_g)
 
 
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+def test_more_groups_than_ctas(mixed):
+    """CTAs that take one group after the other."""
+    rng = np.random.default_rng(12)
+    lengths = rng.integers(257, 420, 3000).tolist() + [5000] * 3
+    n, n_groups = sum(lengths), len(lengths)
+    group = _groups(rng, lengths, mixed)
+    plan = O.RowGroups(group)
+    x, s = _scores(rng, n, torch.float32, 2.0)
+    l = ref.log_probs(s, group, n_groups)
+    assert_close(O.group_log_probs(x, plan), l, ref.U * np.abs(l))
+    t = rng.random(n).astype(np.float32)
+    got = O.choice_loss(x, plan, _cuda(t))
+    loss, grad, err_l, err_g = ref.choice(s, group, n_groups, t)
+    assert_close(got.loss, loss, err_l)
+    assert_close(got.grad, grad, err_g)
+    a, old = rng.normal(size=n).astype(np.float32), (l + 0.3 * rng.normal(size=n)).astype(np.float32)
+    got = O.policy_loss(x, plan, _cuda(a), _cuda(old), reference_log_probs=_cuda(old), kl_coef=0.1)
+    loss, grad, kl, clipped, err_l, err_g, err_k = ref.policy(s, group, n_groups, a, old, old, kl_coef=0.1)
+    assert int(got.clipped) == clipped
+    assert_close(got.loss, loss, err_l)
+    assert_close(got.kl, kl, err_k)
+    assert_close(got.grad, grad, err_g)
+
+
 def test_ratios_at_their_borders():
     """Ratios a few steps of float32 from a border fall on the side on which the definition has them."""
     n = 4096
@@ -530,6 +555,8 @@ def test_refused_fits():
             b.fit(X, None, era, num_rounds=1, objective=objective)
     with pytest.raises(ValueError):
         b.fit(X, None, era, num_rounds=1)
+    with pytest.raises(TypeError):
+        b.fit(X, None, era, num_rounds=1, objective="preference")
     z, one, bad = np.zeros(200), np.ones(200), np.full(200, np.nan)
     for objective in (O.ChoiceObjective(bad), O.ChoiceObjective(-one), O.PolicyObjective(bad, z), O.PolicyObjective(one, bad),
                       O.PolicyObjective(z, z, reference_log_probs=bad), O.PolicyObjective(z, z, reference_log_probs=bad, kl_coef=1.0)):
