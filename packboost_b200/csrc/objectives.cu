@@ -693,7 +693,8 @@ __device__ __forceinline__ double cta_log_sum(float m, double z, float* s_m, dou
 
 constexpr int kBlockRows = 4;  // of a thread at a time
 
-template <typename T, int OP, int THREADS, bool VECTOR>
+// (MANY: a CTA takes one group after the other; as a loop that runs once it costs ragged eras 2 us of 18.)
+template <typename T, int OP, int THREADS, bool VECTOR, bool MANY>
 __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2* __restrict__ list, int most, bool words, int slot0,
                                                         const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
     extern __shared__ float4 kept4[];  // p, then the fixed parts, `most` each: a thread's four are one word
@@ -706,7 +707,7 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
     float4* const kept_fixed = kept4 + most / 4 + threadIdx.x;
     double loss = 0.0, kl = 0.0;
     int clipped = 0;
-    for (int g = blockIdx.x; g < (int)a.g.n_blocks; g += gridDim.x) {
+    for (int g = blockIdx.x; MANY ? g < (int)a.g.n_blocks : g == (int)blockIdx.x; g += gridDim.x) {
         const int2 group = list[g];
         const int begin = VECTOR ? group.x & ~3 : group.x, end = group.x + group.y;
         // all steps of the group in turn: f(rows, step, whether all rows are the group's)
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
                 rows.template load<decltype(full)::value>(scores, false);
                 rows.template log_probs<decltype(full)::value>(lse, out);
             });
-            __syncthreads();  // (the next group's sums go where this one's were)
+            if (MANY) __syncthreads();  // (the next group's sums go where this one's were)
             continue;
         }
         steps([&](Four& rows, int k, auto full) {
@@ -1034,10 +1035,12 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
             PB_CUDA_TRY(launch(kernel, block_grid(&g), threads, smem, early, stream, a, list, most, words, slot, scores, out, totals));
             return PB_OK;
         };
-        if (threads == 256)
-            PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false>) : block(block_kernel<T, OP, 256, true>));
+        if (block_grid(&g) < g.n_blocks)
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false, true>) : block(block_kernel<T, OP, 256, true, true>));
+        else if (threads == 256)
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 256, false, false>) : block(block_kernel<T, OP, 256, true, false>));
         else
-            PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false>) : block(block_kernel<T, OP, 512, true>));
+            PB_TRY(g.rows ? block(block_kernel<T, OP, 512, false, false>) : block(block_kernel<T, OP, 512, true, false>));
         slot += (int)block_grid(&g);
         early = true;
     }
