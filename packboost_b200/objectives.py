@@ -39,6 +39,12 @@ import torch
 
 from . import backends as B
 
+# (what torch.cuda.current_device, current_stream().cuda_stream and is_current_stream_capturing come down to; a call of ten
+# microseconds notices the rest)
+_device_now = getattr(torch._C, "_cuda_getDevice", None)
+_stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+
 _SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MOST = (1 << 31) - (1 << 16)    # rows, and items (two per pair): 32-bit numbers
 _PREFERENCE, _CHOICE, _POLICY = 0, 1, 2
@@ -298,7 +304,7 @@ class _Layout:
 
     def _used_now(self) -> int:
         """The current stream of the layout's device, which must be the current one."""
-        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        stream = _stream_now(self.device.index)
         if stream not in self._streams:
             if len(self._streams) >= 64:
                 self._streams = {self._stream}
@@ -311,14 +317,15 @@ class _Layout:
     def _room(self, stream: int) -> torch.Tensor:
         """Scratch that no other evaluation uses at the same time: one per thread and stream, which a call leaves as the
         next needs it.  A captured call has its own, since its graph may run beside anything."""
-        if torch.cuda.is_current_stream_capturing():
-            return torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=self.device)
-        key = (threading.get_ident(), stream)
-        room = self._rooms.get(key)
-        if room is None:
+        if not _capturing():
+            room = self._rooms.get((threading.get_ident(), stream))
+            if room is not None:
+                return room
             if len(self._rooms) >= 16:
                 self._rooms = {}
-            room = self._rooms[key] = torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        room = torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        if not _capturing():
+            self._rooms[threading.get_ident(), stream] = room
         return room
 
 
@@ -463,18 +470,19 @@ def _kept_struct(layout: _Layout, options: tuple, struct: B.Objective) -> B.Obje
 
 
 def _evaluate(struct: B.Objective, layout: _Layout, scores: torch.Tensor, policy: bool = False):
-    if torch.cuda.current_device() != layout.device.index:
+    if _device_now() != layout.device.index:
         with torch.cuda.device(layout.device):
             return _evaluate(struct, layout, scores, policy)
     stream = layout._used_now()
     room = layout._room(stream)
     grad, loss = torch.empty_like(scores), torch.empty_like(layout._number)
-    kl = clipped = None
     if policy:
         kl, clipped = torch.empty_like(layout._number), torch.empty_like(layout._count)
-    rc = B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
-                                       kl.data_ptr() if policy else None, clipped.data_ptr() if policy else None, room.data_ptr(),
-                                       layout._scratch_bytes, stream)
+        rc = B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
+                                           kl.data_ptr(), clipped.data_ptr(), room.data_ptr(), layout._scratch_bytes, stream)
+    else:
+        rc = B.lib().pb_objective_evaluate(struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], grad.data_ptr(), loss.data_ptr(),
+                                           None, None, room.data_ptr(), layout._scratch_bytes, stream)
     if rc:
         layout._rooms = {}    # (a call that broke off may not have left its scratch in order)
         B.check(rc)
@@ -532,7 +540,7 @@ def policy_loss(scores: torch.Tensor, groups: RowGroups, advantage: torch.Tensor
 def group_log_probs(scores: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     """``s - log sum exp s`` over each row's group, in the scores' type; -inf where the score is."""
     scores = _check_scores(scores, groups)
-    if torch.cuda.current_device() != groups.device.index:
+    if _device_now() != groups.device.index:
         with torch.cuda.device(groups.device):
             return group_log_probs(scores, groups)
     lib, stream = B.lib(), groups._used_now()
@@ -540,9 +548,10 @@ def group_log_probs(scores: torch.Tensor, groups: RowGroups) -> torch.Tensor:
     if groups._log_probs_bytes is None:
         groups._log_probs_bytes = int(lib.pb_group_log_probs_bytes(groups._struct))
     nbytes = groups._log_probs_bytes
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=groups.device).data_ptr() if nbytes else None
-    B.check(lib.pb_group_log_probs(groups._struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], out.data_ptr(), scratch,
-                                   nbytes, stream))
+    # (held until the launches are enqueued: given back before, it could be another thread's by then)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=groups.device) if nbytes else None
+    B.check(lib.pb_group_log_probs(groups._struct, scores.data_ptr(), _SCORE_TYPES[scores.dtype], out.data_ptr(),
+                                   scratch.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
