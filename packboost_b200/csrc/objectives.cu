@@ -860,6 +860,7 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
 
 // ---- launches ---------------------------------------------------------------------------------------
 
+constexpr double kMostFactor = 1e30;
 constexpr int64_t kMost = (1ll << 31) - 1;
 constexpr int64_t kMostRows = PB_OBJECTIVE_MOST_ROWS;  // (a CTA's places past the last row are still 32-bit numbers)
 
@@ -898,10 +899,11 @@ int check_pairs(const pb_pairs* p) {
 
 int check_objective(const pb_objective* o) {
     PB_REQUIRE(o != nullptr, "objective is null");
-    PB_REQUIRE(isfinite(o->scale), "scale is not finite");
+    // (factors that stay numbers in 32 bits)
+    PB_REQUIRE(fabs(o->scale) <= kMostFactor, "scale is out of range");
     if (o->kind == PB_OBJECTIVE_PREFERENCE) {
         PB_TRY(check_pairs(o->pairs));
-        PB_REQUIRE(o->beta > 0.0 && isfinite(o->beta), "beta must be positive");
+        PB_REQUIRE(o->beta >= 1.0 / kMostFactor && o->beta <= kMostFactor, "beta outside [1e-30, 1e30]");
         PB_REQUIRE(o->smoothing >= 0.0 && o->smoothing < 0.5, "smoothing outside [0, 0.5)");
         return PB_OK;
     }
@@ -915,7 +917,8 @@ int check_objective(const pb_objective* o) {
     PB_REQUIRE(o->advantage && o->old, "advantage or old is null");
     PB_REQUIRE(o->clip_low >= 0.0 && o->clip_low <= 1.0, "clip_low outside [0, 1]");
     PB_REQUIRE(o->clip_high >= 0.0, "clip_high must not be negative");
-    PB_REQUIRE(isfinite(o->kl_coef) && (o->reference || o->kl_coef == 0.0), "kl_coef needs a reference");
+    PB_REQUIRE(fabs(o->kl_coef) <= kMostFactor, "kl_coef is out of range");
+    PB_REQUIRE(o->reference || o->kl_coef == 0.0, "kl_coef needs a reference");
     return PB_OK;
 }
 
@@ -1063,8 +1066,9 @@ int launch_objective(const pb_objective* o, const void* scores_, void* grad_, fl
     if (o->kind == PB_OBJECTIVE_PREFERENCE)
         return launch_pairs<T>(o, scores, grad, totals_of(n_parts_of(o->pairs), sums_bytes(o->pairs), o->scale, loss, kl, clipped, scratch), scratch,
                                stream);
-    const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(o->clip_high)), split(log1p(-o->clip_low)),
-                      (float)(1.0 + o->clip_high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
+    const double high = 1.0 + o->clip_high > kMostFactor ? INFINITY : o->clip_high;  // (beyond it nothing is cut off)
+    const GroupArgs a{*o->groups, o->target, o->advantage, o->old, o->reference, split(log1p(high)), split(log1p(-o->clip_low)),
+                      (float)(1.0 + high), (float)(1.0 - o->clip_low), (float)o->kl_coef, (float)o->scale};
     const Totals totals = totals_of(n_parts_of(o->groups, o->kind == PB_OBJECTIVE_POLICY), sums_bytes(o->groups), o->scale, loss, kl, clipped,
                                     scratch);
     if (o->kind == PB_OBJECTIVE_CHOICE) return launch_groups<T, kChoice>(a, scores, grad, totals, scratch, stream);

@@ -30,7 +30,6 @@ used from any stream, and have to outlive the graphs that use them.
 from __future__ import annotations
 
 import ctypes as C
-import math
 import threading
 from typing import NamedTuple
 
@@ -412,8 +411,8 @@ def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) 
     kept = pairs._structs.get(options)
     if kept is not None:
         return kept
-    if not (beta > 0 and math.isfinite(beta)):
-        raise ValueError("beta must be positive")
+    if not 1e-30 <= beta <= 1e30:
+        raise ValueError("beta must be positive, and between 1e-30 and 1e30")
     if not 0 <= smoothing < 0.5:
         raise ValueError("label_smoothing outside [0, 0.5)")
     if kind not in ("logistic", "squared"):
@@ -444,8 +443,8 @@ def _policy_struct(groups: RowGroups, advantage, old, reference, clip, kl_coef, 
     if kept is None:
         if not (0 <= low <= 1 and high >= 0):
             raise ValueError("clip must be (low, high) with low in [0, 1] and high not negative")
-        if not math.isfinite(kl):
-            raise ValueError("kl_coef must be finite")
+        if not abs(kl) <= 1e30:
+            raise ValueError("kl_coef must be finite, and at most 1e30")
         kept = _kept_struct(groups, options, B.Objective(
             kind=_POLICY, groups=C.pointer(groups._struct), advantage=16, old=16, reference=16, clip_low=low, clip_high=high,
             kl_coef=kl, scale=_scale(reduction, groups.n_groups, "groups")))

@@ -139,7 +139,7 @@ def test_groups(lengths, dtype, mixed):
         prior[off] = np.nan
         a[off & (rng.random(n) < 0.5)] = np.nan
         for opts in (dict(), dict(reference=prior, kl_coef=0.1, clip=(0.1, 0.3), reduction="mean"),
-                     dict(reference=prior), dict(clip=(1.0, np.inf)), dict(clip=(0.0, 0.0))):
+                     dict(reference=prior), dict(clip=(1.0, np.inf)), dict(clip=(0.0, 0.0)), dict(clip=(0.5, 1e39))):
             kw = {k: v for k, v in opts.items() if k != "reference"}
             got = O.policy_loss(x, plan, _cuda(a), _cuda(old),
                                 reference_log_probs=_cuda(prior) if "reference" in opts else None, **kw)

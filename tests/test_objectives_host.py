@@ -211,7 +211,7 @@ def test_refused_scores_and_rows():
 
 
 @pytest.mark.parametrize("kw", [
-    dict(beta=0.0), dict(beta=-1.0), dict(beta=float("inf")), dict(beta=float("nan")), dict(smoothing=0.5),
+    dict(beta=0.0), dict(beta=-1.0), dict(beta=float("inf")), dict(beta=float("nan")), dict(beta=1e39), dict(beta=1e-40), dict(smoothing=0.5),
     dict(smoothing=-0.1), dict(kind="hinge"), dict(kind="squared", smoothing=0.1), dict(reduction="none"),
 ])
 def test_refused_preference_options(kw):
@@ -229,7 +229,7 @@ def test_refused_means_over_nothing():
 
 
 @pytest.mark.parametrize("clip,kl,with_reference", [((-0.1, 0.2), 0.0, True), ((1.1, 0.2), 0.0, True), ((0.2, -0.1), 0.0, True),
-                                                    ((float("nan"), 0.2), 0.0, True), ((0.2, 0.2), float("nan"), True),
+                                                    ((float("nan"), 0.2), 0.0, True), ((0.2, 0.2), float("nan"), True), ((0.2, 0.2), 1e39, True),
                                                     ((0.2, 0.2), 0.1, False)])
 def test_refused_policy_options(clip, kl, with_reference):
     groups = _Stub(2, struct=B.Groups(2, 1), n_groups=1)
@@ -262,8 +262,8 @@ def test_library_refuses_bad_descriptors():
                       (dict(other=None), "null"), (dict(n_chunks=1), "null"), (dict(n_chunks=-1), "range"),
                       (dict(n_split=1), "range"), (dict(slices=20), "aligned"), (dict(offset=20), "aligned"), (dict(n_chunks=1, chunks=24), "aligned")):
         refused(B.Objective(kind=0, pairs=C.pointer(pairs(**kw)), beta=1.0), match)
-    for kw, match in ((dict(beta=0.0), "beta"), (dict(beta=1.0, smoothing=0.5), "smoothing"),
-                      (dict(beta=1.0, scale=float("nan")), "scale")):
+    for kw, match in ((dict(beta=0.0), "beta"), (dict(beta=1e31), "beta"), (dict(beta=1.0, smoothing=0.5), "smoothing"),
+                      (dict(beta=1.0, scale=float("nan")), "scale"), (dict(beta=1.0, scale=1e40), "scale")):
         refused(B.Objective(kind=0, pairs=C.pointer(ok), **kw), match)
     for kw, match in ((dict(n_rows=-1), "n_rows"), (dict(n_groups=4), "n_groups"), (dict(n_groups=0), "without a group"),
                       (dict(n_team_warps=0), "not laid out"), (dict(teams=None), "null"), (dict(team_warps=None), "null"),
@@ -274,7 +274,8 @@ def test_library_refuses_bad_descriptors():
     refused(B.Objective(kind=1, groups=C.pointer(good)), "target")
     rows = dict(groups=C.pointer(good), advantage=16, old=16)
     refused(B.Objective(kind=2, groups=C.pointer(good), advantage=16), "old")
-    for kw, match in ((dict(clip_low=1.5), "clip_low"), (dict(clip_high=-1.0), "clip_high"), (dict(kl_coef=0.1), "reference")):
+    for kw, match in ((dict(clip_low=1.5), "clip_low"), (dict(clip_high=-1.0), "clip_high"), (dict(kl_coef=0.1), "reference"),
+                      (dict(kl_coef=1e40, reference=16), "kl_coef")):
         refused(B.Objective(kind=2, **rows, **kw), match)
     # scores, types and scratch
     o = B.Objective(kind=0, pairs=C.pointer(ok), beta=1.0, scale=1.0)
