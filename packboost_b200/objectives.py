@@ -116,11 +116,11 @@ def _check_pairs(chosen, rejected, n_rows: int) -> tuple[torch.Tensor, torch.Ten
         raise ValueError(f"more than {_MOST // 2} pairs")
     rejected = rejected.to(chosen.device)
     if chosen.shape[0]:
-        low = min(int(chosen.min()), int(rejected.min()))
-        high = max(int(chosen.max()), int(rejected.max()))
+        both = torch.cat([chosen, rejected])
+        low, high, same = torch.stack([both.min(), both.max(), (chosen == rejected).any().to(torch.int64)]).tolist()
         if low < 0 or high >= n_rows:
             raise ValueError(f"pairs name rows outside [0, {n_rows})")
-        if bool((chosen == rejected).any()):
+        if same:
             raise ValueError("a pair compares a row with itself")
     return chosen, rejected
 
@@ -132,89 +132,95 @@ def _check_weight(weight, n_pairs: int, device) -> torch.Tensor:
     return weight
 
 
-# (the layouts below are the ones of include/packboost_b200.h; they are made by torch, on any device)
+# (the layouts below are the ones of include/packboost_b200.h; they are made by torch, on any device: small ones on the host,
+# where a step costs less than a launch)
 _SLICE_ROWS, _SLICE_ITEMS, _CHUNK_ITEMS = 64, 32, 512
 _WINDOW = 8192   # rows whose order a slice may change: its rows stay near the ones they are compared with
-
-
-def _rank_in_row(rows: torch.Tensor, others: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
-    """For each entry, how many entries of the same row come before it in the order of the other rows: neighbouring items
-    of a row then look up neighbouring scores (a row of 670 000 items among 500 000 rows: 25 us with its items as given, 16 so)."""
-    order = torch.sort((rows << 32) | others, stable=True).indices
-    rank = torch.empty_like(rows)
-    rank[order] = torch.arange(rows.shape[0], device=rows.device) - (counts.cumsum(0) - counts)[rows[order]]
-    return rank
+_HOST_PAIRS, _HOST_ROWS = 4096, 32768   # 500 pairs 0.4 ms there and 0.75 on the GPU, 5 000 pairs 1.3 and 0.8; 20 groups of 1 000 rows 0.3 and 0.5
 
 
 def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict:
     """The items of every row: by columns of 64 rows with equally many, in chunks where there are many."""
-    dev = chosen.device
+    dev, n_pairs = chosen.device, chosen.shape[0]
     if n_rows == 0:
         return {}
-    n_chosen = torch.bincount(chosen, minlength=n_rows)
-    n_rejected = torch.bincount(rejected, minlength=n_rows)
-    few = (n_chosen <= _SLICE_ITEMS) & (n_rejected <= _SLICE_ITEMS)
-    row = torch.nonzero(few)[:, 0]
+    # both sides in one: the items of row r that chose it have the owner r, those that rejected it n_rows + r
+    owner, other = torch.cat([chosen, rejected + n_rows]), torch.cat([rejected, chosen])
+    counts = torch.zeros(2 * n_rows, dtype=torch.int64, device=dev).index_add_(0, owner, torch.ones_like(owner))
+    n_chosen, n_rejected = counts[:n_rows], counts[n_rows:]
+    few = torch.maximum(n_chosen, n_rejected) <= _SLICE_ITEMS
+    all_few = n_pairs == 0 or bool(few.all())
+    row = torch.arange(n_rows, device=dev) if all_few else torch.nonzero(few)[:, 0]
     # (by turns up and down: rows on either side of a step differ by one item)
-    turn = torch.where(n_chosen[row] % 2 == 0, n_rejected[row], _SLICE_ITEMS - n_rejected[row])
-    key = ((row // _WINDOW) * (_SLICE_ITEMS + 1) + n_chosen[row]) * (_SLICE_ITEMS + 1) + turn
+    key_c, key_r = n_chosen[row], n_rejected[row]
+    key = ((row // _WINDOW) * (_SLICE_ITEMS + 1) + key_c) * (_SLICE_ITEMS + 1) + torch.where(key_c % 2 == 0, key_r, _SLICE_ITEMS - key_r)
     row = row[torch.sort(key, stable=True).indices]
-    n_slices = -(-row.shape[0] // _SLICE_ROWS)
-    lanes = torch.full((_SLICE_ROWS * n_slices,), -1, dtype=torch.int64, device=dev)
-    lanes[: row.shape[0]] = row
-    have = torch.stack([torch.where(lanes >= 0, c[lanes.clamp_min(0)], torch.zeros_like(lanes)) for c in (n_chosen, n_rejected)], 1)
-    tall = have.view(n_slices, _SLICE_ROWS, 2).amax(1) if n_slices else have.new_zeros((0, 2))
+    n_few = row.shape[0]
+    n_slices = -(-n_few // _SLICE_ROWS)
+    have = torch.zeros((_SLICE_ROWS * n_slices, 2), dtype=torch.int64, device=dev)
+    have[:n_few, 0], have[:n_few, 1] = n_chosen[row], n_rejected[row]
+    tall = have.view(n_slices, _SLICE_ROWS, 2).amax(1) if n_slices else have
     column = tall.sum(1).cumsum(0) - tall.sum(1)
+    lanes = torch.full((_SLICE_ROWS * n_slices,), -1, dtype=torch.int64, device=dev)
+    lanes[:n_few] = row
     out = {"n_slices": n_slices,
            "slices": torch.stack([column, tall[:, 0] | (tall[:, 1] << 16)], 1).to(torch.int32),
            "slice_rows": torch.stack([lanes, have[:, 0] | (have[:, 1] << 16)], 1).to(torch.int32)}
-    first_many = _SLICE_ROWS * int(tall.sum())
-
-    many = torch.nonzero(~few)[:, 0]
-    size = n_chosen[many] + n_rejected[many]
-    begin = first_many + size.cumsum(0) - size
-    n_items = first_many + int(size.sum())
+    n_items = _SLICE_ROWS * int(tall.sum())
+    # where an item goes: base + stride * its rank among its owner's items
+    base = torch.zeros(2 * n_rows, dtype=torch.int64, device=dev)
+    at = torch.arange(n_few, device=dev)
+    first = column[at // _SLICE_ROWS] * _SLICE_ROWS + at % _SLICE_ROWS
+    base[row], base[row + n_rows] = first, first + tall[at // _SLICE_ROWS, 0] * _SLICE_ROWS
+    stride = None
+    if not all_few:
+        many = torch.nonzero(~few)[:, 0]
+        size = n_chosen[many] + n_rejected[many]
+        begin = n_items + size.cumsum(0) - size
+        n_items += int(size.sum())
+        stride = torch.where(few, _SLICE_ROWS, 1).repeat(2)
+        base[many], base[many + n_rows] = begin, begin + n_chosen[many]
+        out.update(_lay_out_chunks(many, n_chosen[many], size, begin))
     if n_items > _MOST:
         raise ValueError("more items than 32-bit numbers count")
-    # where an item goes: base + stride * its rank among its row's items of its side
-    base = torch.empty((n_rows, 2), dtype=torch.int64, device=dev)
-    stride = torch.ones(n_rows, dtype=torch.int64, device=dev)
-    at = torch.arange(row.shape[0], device=dev)
-    base[row, 0] = column[at // _SLICE_ROWS] * _SLICE_ROWS + at % _SLICE_ROWS
-    base[row, 1] = base[row, 0] + tall[at // _SLICE_ROWS, 0] * _SLICE_ROWS
-    stride[row] = _SLICE_ROWS
-    base[many, 0], base[many, 1] = begin, begin + n_chosen[many]
-    place = [base[own, k] + stride[own] * _rank_in_row(own, other, count)
-             for k, (own, other, count) in enumerate(((chosen, rejected, n_chosen), (rejected, chosen, n_rejected)))]
+    # Ranks in the order of the other rows: neighbouring items of a row then look up neighbouring scores (rows of 670 000 items
+    # among 500 000 rows: 25 us with the items as given, 19 so).
+    order = torch.sort((owner << 32) | other, stable=True).indices
+    owner = owner[order]
+    rank = torch.arange(2 * n_pairs, device=dev) - (counts.cumsum(0) - counts)[owner]
+    place = base[owner] + rank * (_SLICE_ROWS if stride is None else stride[owner])
     out["other"] = torch.zeros(max(n_items, 1), dtype=torch.int32, device=dev)
-    out["other"][place[0]], out["other"][place[1]] = rejected.to(torch.int32), chosen.to(torch.int32)
+    out["other"][place] = other[order].to(torch.int32)
     if reference is not None:
         r = reference.to(torch.float64)
         away = (r[chosen] - r[rejected]).to(torch.float32)
         out["offset"] = torch.zeros(max(n_items, 1), dtype=torch.float32, device=dev)
-        out["offset"][place[0]], out["offset"][place[1]] = away, -away
+        out["offset"][place] = torch.cat([away, -away])[order]
     if weight is not None:
         out["weight"] = torch.zeros(max(n_items, 1), dtype=torch.float32, device=dev)
-        out["weight"][place[0]] = out["weight"][place[1]] = weight
+        out["weight"][place] = weight.repeat(2)[order]
+    return out
 
+
+def _lay_out_chunks(row, n_chosen, size, begin) -> dict:
+    """Chunks of rows with ``size`` items from ``begin`` on, of which the first ``n_chosen`` chose the row."""
     n_of = -(-size // _CHUNK_ITEMS)                      # chunks of a row
-    which = torch.repeat_interleave(torch.arange(many.shape[0], device=dev), n_of)
+    which = torch.repeat_interleave(torch.arange(row.shape[0], device=row.device), n_of)
     first = n_of.cumsum(0) - n_of
-    step = (torch.arange(which.shape[0], device=dev) - first[which]) * _CHUNK_ITEMS
+    step = (torch.arange(which.shape[0], device=row.device) - first[which]) * _CHUNK_ITEMS
     split = (n_of > 1).to(torch.int64)
     count = torch.minimum(size[which] - step, torch.full_like(step, _CHUNK_ITEMS))
-    better = (n_chosen[many][which] - step).clamp(min=0).minimum(count)
-    out["n_chunks"], out["n_split"] = which.shape[0], int(split.sum())
-    out["chunks"] = torch.stack([many[which], begin[which] + step, count, better, (split.cumsum(0) - split)[which], first[which],
-                                 n_of[which], torch.zeros_like(step)], 1).to(torch.int32)
-    return out
+    better = (n_chosen[which] - step).clamp(min=0).minimum(count)
+    chunks = torch.stack([row[which], begin[which] + step, count, better, (split.cumsum(0) - split)[which], first[which],
+                          n_of[which], torch.zeros_like(step)], 1).to(torch.int32)
+    return {"n_chunks": which.shape[0], "n_split": int(split.sum()), "chunks": chunks}
 
 
 def _check_groups(group, n_groups) -> tuple[torch.Tensor, int]:
     group = _indices(group, "group")
     if group.shape[0] > _MOST:
         raise ValueError(f"more than {_MOST} rows")
-    low, high = (int(group.min()), int(group.max())) if group.shape[0] else (0, -1)
+    low, high = torch.stack([group.min(), group.max()]).tolist() if group.shape[0] else (0, -1)
     n_groups = high + 1 if n_groups is None else _count(n_groups, "n_groups")
     if low < 0 or high >= n_groups:
         raise ValueError(f"group ids outside [0, {n_groups})")
@@ -288,6 +294,9 @@ class _Layout:
         return struct(**fields)
 
     def _settle(self, device: torch.device, tensors: dict) -> None:
+        for name, t in tensors.items():   # (of a layout made on the host)
+            if isinstance(t, torch.Tensor):
+                tensors[name] = t.to(device)
         self.device = device
         self._tensors = [t for t in tensors.values() if isinstance(t, torch.Tensor)]
         self._structs: dict = {}   # descriptors of objectives on this layout, by their options
@@ -344,9 +353,10 @@ class RowPairs(_Layout):
         if reference is not None:
             reference = _numbers(reference, "reference", n_rows, c.device)
         home = _home(chosen, rejected, weight, reference, device=device)
+        where = torch.device("cpu") if 2 * c.shape[0] + n_rows <= _HOST_PAIRS else home
         with torch.cuda.device(home):
-            parts = _lay_out_pairs(c.to(home), r.to(home), n_rows, None if weight is None else weight.to(home),
-                                   None if reference is None else reference.to(home))
+            parts = _lay_out_pairs(c.to(where), r.to(where), n_rows, None if weight is None else weight.to(where),
+                                   None if reference is None else reference.to(where))
             if parts.get("offset") is not None and not bool(torch.isfinite(parts["offset"]).all()):
                 raise ValueError("reference scores of compared rows must be finite")
             self.n_rows, self.n_pairs = n_rows, int(c.shape[0])
@@ -365,7 +375,7 @@ class RowGroups(_Layout):
         g, n_groups = _check_groups(group, n_groups)
         home = _home(group, device=device)
         with torch.cuda.device(home):
-            parts = _lay_out_groups(g.to(home))
+            parts = _lay_out_groups(g.to("cpu" if g.shape[0] <= _HOST_ROWS else home))
             self.n_rows, self.n_groups = int(g.shape[0]), n_groups
             self._settle(home, parts)
         self._struct = self._point(B.Groups, parts, n_rows=self.n_rows)
