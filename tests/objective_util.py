@@ -1,7 +1,7 @@
 """The objectives from their definitions in float64 numpy, and how far a float32 kernel may be off.
 
-Bounds count roundings.  u = 2^-24 is half a step of float32 relative to the value; CUDA documents expf with 2 ulp
-(4 u) and log1pf with 1 ulp (2 u).  Each function returns values and bounds of the same shape; the bounds of
+Bounds count roundings.  u = 2^-24 is half a step of float32 relative to the value; the GPU's 2^x is documented with 2 ulp
+(4 u) and its 1 / x with 1 ulp (2 u).  Each function returns values and bounds of the same shape; the bounds of
 gradients do not hold the rounding to the scores' type, which `assert_close` adds (half a step, or half the smallest
 number of the type)."""
 
@@ -26,7 +26,7 @@ def pair_loss(scores, chosen, rejected, *, weight=None, reference=None, beta=1.0
         err_z = beta * err_d + 2 * U * np.abs(z)             # beta and the product
         loss = (1 - smoothing) * np.logaddexp(0, -z) + smoothing * np.logaddexp(0, z)
         slope = beta * (smoothing - 1 / (1 + np.exp(np.clip(z, -700, 700))))
-        # sigmoid has a slope of at most 1/4; exp 4 u of a value whose share of 1 + exp is below 1, sum, quotient,
+        # sigmoid has a slope of at most 1/4; 2^x 4 u of a value whose share of 1 + 2^x is below 1, sum, 1 / x,
         # difference, product, beta and smoothing in 32 bits
         err_s = beta * (err_z / 4 + 12 * U)
         err_l = err_z + 12 * U * (1 + np.abs(loss))
@@ -77,7 +77,7 @@ def choice(scores, group, n_groups, target, reduction="sum"):
     loss = -(t[on] * l[on]).sum()
     p, mass = np.exp(l), total(t)
     grad = p * mass - t
-    # p: expf and the correction of its argument; the group's sum in 32 bits; product, difference, scale
+    # p: 2^x and the correction of its argument; the group's sum in 32 bits; product, difference, scale
     err_g = 10 * U * p * mass + 3 * U * np.abs(grad)
     return loss * norm, grad * norm, 2 * U * abs(loss * norm) + 1e-12 * np.abs(t[on] * l[on]).sum() * norm, err_g * norm
 
@@ -109,7 +109,7 @@ def policy(scores, group, n_groups, advantage, old, reference=None, clip=(0.2, 0
         grad = grad + kl_coef * p * (gap - kl_group)
     norm = 1.0 if reduction == "sum" else 1.0 / n_groups
     inner = np.abs(kl_coef * (gap - kl_group) - h)
-    # ratio: expf (4 u), correction, product with the advantage; the sum in brackets rounded once to 32 bits;
+    # ratio: 2^x (4 u), correction, product with the advantage; the sum in brackets rounded once to 32 bits;
     # p as above, product, sum, scale
     err_g = 8 * U * np.abs(slope) + p * (8 * U * size + abs(kl_coef) * err_kl_row + 10 * U * inner) + 4 * U * np.abs(grad)
     err_kl = 8 * U * (p * np.abs(gap)).sum() + 2 * U * abs(kl)
