@@ -347,6 +347,38 @@ def test_threads_share_layouts():
     assert not wrong
 
 
+def test_arguments_of_other_kinds():
+    """Lists, arrays and tensors of any integer type, on the host or the GPU, make the same layouts; sizes on both sides of
+    where a layout is made on the host."""
+    for n in (700, 40_000):
+        rng = np.random.default_rng(n)
+        c, j = _pairs(rng, n, 2 * n, 0, n)
+        group = rng.integers(0, 40, n)
+        w, r = rng.integers(0, 3, 2 * n), rng.normal(size=n)
+        x, _ = _scores(rng, n, torch.float32)
+        want_p = O.preference_loss(x, O.RowPairs(c, j, n, weight=w, reference=r), reduction="mean")
+        want_l = O.group_log_probs(x, O.RowGroups(group))
+        for make in (list, lambda v: torch.from_numpy(v.astype(np.int32)).cuda(), lambda v: v.astype(np.uint16), torch.from_numpy):
+            got = O.preference_loss(x, O.RowPairs(make(c), make(j), np.int64(n), weight=_cuda(w), reference=_cuda(r)), reduction="mean")
+            assert torch.equal(got.loss, want_p.loss) and torch.equal(got.grad, want_p.grad)
+            assert torch.equal(O.group_log_probs(x, O.RowGroups(make(group), 50)), want_l)
+        leaf = x.clone().requires_grad_()
+        got = O.preference_loss(leaf, O.RowPairs(c, j, n, weight=w, reference=r), reduction="mean")
+        assert torch.equal(got.grad, want_p.grad) and not got.loss.requires_grad and not got.grad.requires_grad
+
+
+def test_fit_without_eras():
+    X, _, rng = _table(n=3000, seed=8)
+    n = len(X)
+    c, j = _pairs(rng, n, 5000, 0, n)
+    t = rng.random(n).astype(np.float32)
+    for objective, other in ((O.PreferenceObjective(_cuda(c), _cuda(j)), O.PreferenceObjective(c.tolist(), j.tolist())),
+                             (O.ChoiceObjective(t), O.ChoiceObjective(_cuda(t), group=np.zeros(n, np.int64)))):
+        a = PackBoost(PackBoostConfig(**CFG)).fit(X, None, None, num_rounds=3, objective=objective)
+        b = PackBoost(PackBoostConfig(**CFG)).fit(torch.from_numpy(X).cuda(), np.ones(n, np.float32), None, num_rounds=3, objective=other)
+        _same_trees(a, b)
+
+
 def test_many_options_and_streams():
     """More descriptors and more streams than a layout keeps."""
     x, groups, a, old, pairs = _problem(9, 9500)
