@@ -306,6 +306,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
                 last = atomicAdd(a.counts + of.x, mine) + mine == (unsigned)of.z;
             }
             if (!__shfl_sync(0xFFFFFFFFu, last, 0)) continue;
+            __syncwarp();  // (orders the lanes' reads after the first lane's count)
             fence();
             double sum = 0.0;
 #pragma unroll 8
