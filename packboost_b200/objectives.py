@@ -20,8 +20,8 @@ and as what a fit learns from::
 
     booster.fit(X, None, era, num_rounds=100, objective=PreferenceObjective(chosen, rejected, beta=1.0))
 
-Scores are float32, float16 or bfloat16 and gradients have their type; sums are held in 64 bits or, over the few
-pairs of a row, in 32, in an order that does not change from run to run.  The results are not attached to an
+Scores are float32, float16 or bfloat16 and gradients have their type; sums are held in 64 bits, of up to eight terms
+each in 32, in an order that does not change from run to run.  The results are not attached to an
 autograd graph: the gradient is there already.  Calls only enqueue work on the current stream of the scores'
 device and may be captured into a CUDA graph; ``RowPairs`` and ``RowGroups`` wait for their own layout, may be
 used from any stream, and have to outlive the graphs that use them.
