@@ -176,7 +176,9 @@ def _run_own(state):
     from packboost_b200 import objectives
     case = state["case"]
     if case["op"] == "preference":
-        return objectives.preference_loss(state["scores"], state["plan"], beta=case["beta"], label_smoothing=case["smoothing"],
+        # (the squared form has no smoothing: neither the plain form nor the definition looks at it there)
+        smoothing = case["smoothing"] if case["kind"] == "logistic" else 0.0
+        return objectives.preference_loss(state["scores"], state["plan"], beta=case["beta"], label_smoothing=smoothing,
                                           kind=case["kind"], reduction=case["reduction"])
     if case["op"] == "choice":
         return objectives.choice_loss(state["scores"], state["plan"], state["target"], reduction=case["reduction"])
