@@ -303,3 +303,39 @@ def test_library_refuses_bad_descriptors():
 def test_structs_mirror_the_library():
     for i, t in enumerate((B.Pairs, B.Groups, B.Objective)):
         assert B.lib().pb_objective_struct_bytes(i) == C.sizeof(t)
+
+
+def test_drawn_performance_cases_pass_the_checks(monkeypatch):
+    """Every call that a drawn case makes gets past the checks of its options."""
+    import random
+    from perf import operators as cases
+    taken = []
+
+    def preference(scores, pairs, *, beta, label_smoothing, kind, reduction):
+        taken.append((kind, O._preference_struct(pairs, beta, label_smoothing, kind, reduction).smoothing))
+        return None, None
+
+    def choice(scores, groups, target, *, reduction):
+        O._choice_struct(groups, target, reduction)
+        return None, None
+
+    def policy(scores, groups, advantage, old, *, reference_log_probs, clip, kl_coef, reduction):
+        O._policy_struct(groups, advantage, old, reference_log_probs, clip, kl_coef, reduction)
+        return None, None
+
+    for name, stand_in in (("preference_loss", preference), ("choice_loss", choice), ("policy_loss", policy),
+                           ("group_log_probs", lambda scores, groups: None)):
+        monkeypatch.setattr(O, name, stand_in)
+    rng, rows = random.Random(5), torch.zeros(1)
+    for case in cases.listed() + [cases.draw(rng) for _ in range(2000)]:
+        if case["op"] == "preference":
+            struct = B.Pairs(n_rows=case["rows"], n_slices=1, slices=16, slice_rows=16, other=16)
+            plan = _Stub(case["rows"], struct=struct, total_weight=1.0)
+        else:
+            struct = B.Groups(n_rows=case["rows"], n_groups=1, n_team_warps=1, team_warps=16, teams=16)
+            plan = _Stub(case["rows"], struct=struct, n_groups=case["groups"])
+        state = dict(case=case, scores=rows, plan=plan, target=rows, advantage=rows, old=rows,
+                     reference=rows if case["reference"] else None)
+        cases._run_own(state)
+    assert {kind for kind, _ in taken} == {"logistic", "squared"} and not any(e for kind, e in taken if kind == "squared")
+    assert any(e for _, e in taken)
