@@ -183,9 +183,7 @@ def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict:
         out.update(_lay_out_chunks(many, n_chosen[many], size, begin))
     if n_items > _MOST:
         raise ValueError("more items than 32-bit numbers count")
-    # Ranks in the order of the other rows: neighbouring items of a row then look up neighbouring scores (rows of 670 000 items
-    # among 500 000 rows: 25 us with the items as given, 19 so).
-    order = torch.sort((owner << 32) | other, stable=True).indices
+    order = _item_order(owner, other, n_rows)
     owner = owner[order]
     rank = torch.arange(2 * n_pairs, device=dev) - (counts.cumsum(0) - counts)[owner]
     place = base[owner] + rank * (_SLICE_ROWS if stride is None else stride[owner])
@@ -200,6 +198,13 @@ def _lay_out_pairs(chosen, rejected, n_rows, weight, reference) -> dict:
         out["weight"] = torch.zeros(max(n_items, 1), dtype=torch.float32, device=dev)
         out["weight"][place] = weight.repeat(2)[order]
     return out
+
+
+def _item_order(owner: torch.Tensor, other: torch.Tensor, n_rows: int) -> torch.Tensor:
+    """Items by owner (below 2 n_rows), those of an owner in the order of the other rows: neighbouring items of a row then look
+    up neighbouring scores (rows of 670 000 items among 500 000 rows: 25 us with the items as given, 19 so)."""
+    # (at most 2 n_rows^2 - 1, which 63 bits hold for all rows that are allowed; two halves of 32 bits would not hold the owner)
+    return torch.sort(owner * n_rows + other, stable=True).indices
 
 
 def _lay_out_chunks(row, n_chosen, size, begin) -> dict:

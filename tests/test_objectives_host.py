@@ -339,3 +339,14 @@ def test_drawn_performance_cases_pass_the_checks(monkeypatch):
         cases._run_own(state)
     assert {kind for kind, _ in taken} == {"logistic", "squared"} and not any(e for kind, e in taken if kind == "squared")
     assert any(e for _, e in taken)
+
+
+@pytest.mark.parametrize("n_rows", [3, 1 << 16, (1 << 30) + 1, O._MOST])
+def test_items_are_ordered_for_any_number_of_rows(n_rows):
+    """Owners go up to twice the number of rows, the rejected rows at the end of the largest tables among them."""
+    rng = np.random.default_rng(n_rows)
+    near = np.array([0, 1, 2, n_rows - 2, n_rows - 1], np.int64).clip(0)
+    other = rng.choice(near, 400)
+    owner = rng.choice(near, 400) + n_rows * rng.integers(0, 2, 400)
+    order = O._item_order(torch.from_numpy(owner), torch.from_numpy(other), n_rows).numpy()
+    np.testing.assert_array_equal(order, np.lexsort((other, owner)))   # (stable, like the sort)
