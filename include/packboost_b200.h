@@ -402,7 +402,8 @@ typedef struct pb_round_log_header {
  *      1 + clip_high) A), and kl_coef times the sum over the group of exp(l) (l - reference).
  *
  * The sum over pairs or groups is multiplied by `scale`.  A row with the score -inf is masked: in
- * groups its probability is 0 and, in a policy, nothing else of it is looked at. */
+ * groups its probability is 0 and, in a policy, nothing else of it is looked at.  A ratio q beyond float32 is
+ * infinite, and with it the loss and the gradients of its group. */
 #define PB_OBJECTIVE_PREFERENCE 0
 #define PB_OBJECTIVE_CHOICE 1
 #define PB_OBJECTIVE_POLICY 2

@@ -385,10 +385,14 @@ __host__ __device__ __forceinline__ Pair32 split(double x) {
 
 __device__ __forceinline__ float sum_of(Pair32 x) { return x.hi + fminf(x.lo, 1.f); }
 
-// exp(hi + lo): 2^y with y = hi log2 e rounded, by the unit that has 2^x to 2 ulp, times 1 + what y left out.
+// exp(hi + lo): 2^y with y = hi log2 e rounded, by the unit that has 2^x to 2 ulp, times 1 + what y left out.  BEYOND: it may be
+// beyond 32 bits.  y is then held below 128, where 2^y is a number, and what that leaves out makes it infinite: infinity less a
+// part of itself would be no number.  (574 groups of a policy: 27.5 us so, 28.1 with a choice after the product, 26.7 without.)
+template <bool BEYOND>
 __device__ __forceinline__ float exp_of(Pair32 x) {
     const float log2e = 1.44269502f, rest = 1.33687e-8f;  // log2 e as a float, and (log2 e - that) ln 2
-    const float y = x.hi * log2e;
+    float y = x.hi * log2e;
+    if (BEYOND) asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(127.999992f));  // (the largest float below 128)
     float more = fmaf(fmaf(x.hi, log2e, -y), 0.693147181f, x.lo);
     more = fminf(fmaf(x.hi, rest, more), 1.f);
     const float e = exp2_of(y);
@@ -542,7 +546,7 @@ struct Rows {
             if (on<FULL>(u)) {
                 const bool live = s[u] != -INFINITY;
                 const Pair32 l = difference(s[u], lse.hi, -lse.lo);
-                const float p = live ? exp_of(l) : 0.f;
+                const float p = live ? exp_of<false>(l) : 0.f;
                 float fixed, own;
                 if (OP == kChoice) {
                     const float t = main[u];
@@ -555,7 +559,7 @@ struct Rows {
                     const Pair32 x = difference(l.hi, old[u % HELD], l.lo);
                     const float past = (x.hi - (up ? a.log_high.hi : a.log_low.hi)) + (fminf(x.lo, 1.f) - (up ? a.log_high.lo : a.log_low.lo));
                     const bool beyond = taken && (up ? past : -past) > 0.f;
-                    const float q = beyond ? (up ? a.bound_high : a.bound_low) : exp_of(x);
+                    const float q = beyond ? (up ? a.bound_high : a.bound_low) : exp_of<true>(x);
                     const float cost = -adv * (taken ? q : 0.f);
                     fixed = beyond ? 0.f : cost;
                     part_loss += cost;
@@ -603,7 +607,14 @@ struct Rows {
     __device__ __forceinline__ void gradient(float total, T* out) const {
         float g[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u) g[u] = (s[u] == 0.f ? main[u] : fmaf(s[u], total, main[u])) * a.scale;  // (the total may be infinite)
+        for (int u = 0; u < N; ++u) g[u] = fmaf(s[u], total, main[u]) * a.scale;
+        // The total may be infinite, and with it the fixed part of a row whose ratio is: that row's gradient is its own part, and
+        // rows without a share of the total have none.
+        if (!(fabsf(total) < INFINITY)) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+                if (s[u] == 0.f || fabsf(main[u]) == INFINITY) g[u] = main[u] * a.scale;
+        }
         put<FULL>(g, out);
     }
 

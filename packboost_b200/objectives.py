@@ -542,8 +542,9 @@ def policy_loss(scores: torch.Tensor, groups: RowGroups, advantage: torch.Tensor
     ``sum_i exp(l_i) (l_i - reference_i)``, over all its rows.
 
     A row with the score -inf is masked: its probability is 0, its gradient is 0, and whatever else is given
-    for it is not looked at; neither is the old log-probability of a row that was not taken.  ``reduction``:
-    ``"sum"``, or ``"mean"`` over the groups."""
+    for it is not looked at; neither is the old log-probability of a row that was not taken.  A ratio that
+    float32 does not hold (``l - old`` above 88.7, where it is not cut off) is infinite, and with it the loss
+    and the gradients of the group's rows.  ``reduction``: ``"sum"``, or ``"mean"`` over the groups."""
     advantage = _per_row(advantage, "advantage", groups)
     old = _per_row(old_log_probs, "old_log_probs", groups)
     reference = None if reference_log_probs is None else _per_row(reference_log_probs, "reference_log_probs", groups)

@@ -600,3 +600,58 @@ def test_refused_fits():
         O.choice_loss(x, O.RowGroups([0] * 200), x.cpu())
     with pytest.raises(ValueError):
         O.preference_loss(x.cpu(), O.RowPairs([0], [1], 200))
+
+
+# ---- numbers that 32 bits do not hold, kernels that take many groups ------------------------------------
+
+# how many groups of which lengths: lanes of a warp, CTAs of 512 and of 256 threads, CTAs that take several, pieces
+KINDS = {"teams": [1 + k % 256 for k in range(600)], "few": [257, 900, 8192], "blocks": [257 + k * 13 % 644 for k in range(500)],
+         "many": [257 + k * 7 % 160 for k in range(2500)], "pieces": [8193, 20_001]}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_ratios_beyond_float32(kind, mixed, sign):
+    """exp(l - old) above the largest float32 is infinite: never a number that is none, and in no other group.  (95 and 100: just
+    beyond; what the 2^x unit's argument leaves out is of either sign.)"""
+    lengths = KINDS[kind]
+    n, n_groups = sum(lengths), len(lengths)
+    rng = np.random.default_rng(n)
+    group = _groups(rng, lengths, mixed)
+    x, s = _scores(rng, n, torch.float32)
+    l = ref.log_probs(s, group, n_groups)
+    a = np.where(rng.random(n) < 0.5, 0.0, rng.normal(size=n)).astype(np.float32)
+    old = (l + 0.3 * rng.normal(size=n)).astype(np.float32)
+    plan = O.RowGroups(group, n_groups)
+    over = np.zeros(n_groups, bool)
+    over[::2] = True
+    rows = np.array([np.flatnonzero(group == g)[-1] for g in np.flatnonzero(over)])
+    clip = (0.2, 0.2) if sign < 0 else (0.2, np.inf)      # (a gain is cut off, a loss is not)
+    for far in (95.0, 97.3, 100.0, 1e3, 1e30, np.inf):
+        b, o = a.copy(), old.copy()
+        b[over[group]] = 0.0
+        b[rows], o[rows] = sign * 0.7, l[rows] - far
+        got = O.policy_loss(x, plan, _cuda(b), _cuda(o.astype(np.float32)), reference_log_probs=_cuda(old), kl_coef=0.1, clip=clip)
+        assert got.loss.item() == -sign * np.inf
+        rest = ~over[group]
+        ids = np.unique(group[rest], return_inverse=True)[1]
+        _, grad, _, clipped, _, err_g, _ = ref.policy(s[rest], ids, ids.max() + 1, b[rest], o[rest], old[rest], clip, 0.1)
+        g = got.grad.cpu()
+        assert int(got.clipped) == clipped
+        assert_close(g[torch.from_numpy(rest)], grad, err_g)
+        own = np.zeros(n, bool)
+        own[rows] = True
+        assert (g[torch.from_numpy(own)] == -sign * np.inf).all()
+        assert (g[torch.from_numpy(over[group] & ~own)] == sign * np.inf).all()
+        assert torch.isfinite(got.kl)
+
+
+def test_an_old_log_probability_that_is_no_number():
+    """Of a taken row it makes the loss and its group's gradients no numbers, and no other group's."""
+    group, s = np.repeat([0, 1], 40), np.random.default_rng(1).normal(size=80)
+    a, old = np.full(80, -0.5, np.float32), ref.log_probs(s, group, 2).astype(np.float32)
+    old[3] = np.nan
+    x = _cuda(s.astype(np.float32))
+    got = O.policy_loss(x, O.RowGroups(group), _cuda(a), _cuda(old))
+    assert torch.isnan(got.loss) and torch.isnan(got.grad[:40]).all() and torch.isfinite(got.grad[40:]).all()
