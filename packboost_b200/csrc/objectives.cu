@@ -797,8 +797,10 @@ enum PieceStep { kPieceMass, kPieceTerms, kPieceOut };
 constexpr int kPieceThreads = 256;
 constexpr int kPieceRows = PB_PIECE_ROWS / kPieceThreads;
 
+// (A launch begins before the one in front has left its sums: they are read from L2, after the wait, and nothing tells the compiler
+// that they stay as they are.)
 template <typename T, int OP, int STEP>
-__global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, PieceSums* __restrict__ pieces, int slot0,
+__global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, PieceSums* pieces, int slot0,
                                                               const T* __restrict__ scores, T* __restrict__ out, Totals totals) {
     constexpr int kWarps = kPieceThreads / 32;
     __shared__ float s_m[kWarps];
@@ -848,8 +850,8 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     float m = -INFINITY;
     double z = 0.0;
     for (int k = threadIdx.x; k < count; k += kPieceThreads) {
-        const float mk = pieces[first + k].m, top = fmaxf(m, mk);
-        z = rescaled(z, m, top) + rescaled(pieces[first + k].z, mk, top);
+        const float mk = __ldcg(&pieces[first + k].m), top = fmaxf(m, mk);
+        z = rescaled(z, m, top) + rescaled(__ldcg(&pieces[first + k].z), mk, top);
         m = top;
     }
     const double lse = cta_log_sum<kPieceThreads>(m, z, s_m, s_z);
@@ -865,7 +867,7 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
         return;
     }
     double share = 0.0;
-    for (int k = threadIdx.x; k < count; k += kPieceThreads) share += pieces[first + k].share;
+    for (int k = threadIdx.x; k < count; k += kPieceThreads) share += __ldcg(&pieces[first + k].share);
     rows.template gradient<false>((float)cta_sum<kPieceThreads>(share, scratch), out);
     if (kTotalsAtEnd) put_totals<kPieceThreads>(totals, slot0 + blockIdx.x, rows.loss, 0.0, 0, false);
 }

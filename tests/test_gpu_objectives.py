@@ -655,3 +655,30 @@ def test_an_old_log_probability_that_is_no_number():
     x = _cuda(s.astype(np.float32))
     got = O.policy_loss(x, O.RowGroups(group), _cuda(a), _cuda(old))
     assert torch.isnan(got.loss) and torch.isnan(got.grad[:40]).all() and torch.isfinite(got.grad[40:]).all()
+
+
+def test_long_groups_one_call_after_the_other():
+    """The sums that a long group's launches hand on are those of their own call: calls in a row whose sums differ."""
+    rng = np.random.default_rng(21)
+    lengths = [70_001, 300, 9001, 5, 120_000]
+    n, group = sum(lengths), np.repeat(np.arange(5), lengths)
+    plan = O.RowGroups(group)
+    x, s = _scores(rng, n, torch.float32)
+    l = ref.log_probs(s, group, 5)
+    old = (l + 0.2 * rng.normal(size=n)).astype(np.float32)
+    base = np.abs(rng.normal(size=n)).astype(np.float32)
+    t = rng.random(n).astype(np.float32)
+    scales = [1.0, -3.0, 0.01, 50.0] * 8
+    rows = [_cuda(base * np.float32(k)) for k in scales]
+    o, target = _cuda(old), [_cuda(t), _cuda(3 * t)]
+    torch.cuda.synchronize()
+    got = [(O.policy_loss(x, plan, a, o), O.choice_loss(x, plan, target[i % 2]), O.group_log_probs(x, plan)) for i, a in enumerate(rows)]
+    for i, (policy, choice, log_probs) in enumerate(got):
+        loss, grad, _, clipped, err_l, err_g, _ = ref.policy(s, group, 5, base * np.float32(scales[i]), old)
+        assert int(policy.clipped) == clipped
+        assert_close(policy.loss, loss, err_l)
+        assert_close(policy.grad, grad, err_g)
+        loss, grad, err_l, err_g = ref.choice(s, group, 5, t if i % 2 == 0 else 3 * t)
+        assert_close(choice.loss, loss, err_l)
+        assert_close(choice.grad, grad, err_g)
+        assert_close(log_probs, l, ref.U * np.abs(l))
