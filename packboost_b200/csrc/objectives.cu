@@ -199,7 +199,7 @@ struct LaneRows {
 
 // N columns from the c0-th on.
 template <int N, typename T, bool SQUARED>
-__device__ __forceinline__ void slice_columns(const PairArgs& a, const T* __restrict__ scores, int64_t item, int c0, int chosen, bool want,
+__device__ __forceinline__ void slice_columns(const PairArgs& a, const T* scores, int64_t item, int c0, int chosen, bool want,
                                               LaneRows& r) {
     int2 o[N];
     float2 off[N], w[N];
@@ -241,8 +241,10 @@ __device__ __forceinline__ void slice_columns(const PairArgs& a, const T* __rest
     r.loss += (double)cost;
 }
 
+// (The scores may still be written by the kernel in front when this one begins: nothing tells the compiler that they stay as they
+// are.)
 template <typename T, bool SQUARED>
-__global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T* __restrict__ scores, T* __restrict__ grad, Totals totals) {
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T* scores, T* __restrict__ grad, Totals totals) {
     let_next_start();
     wait_for_previous();  // (see launch_pairs)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

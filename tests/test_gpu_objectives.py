@@ -682,3 +682,21 @@ def test_long_groups_one_call_after_the_other():
         assert_close(choice.loss, loss, err_l)
         assert_close(choice.grad, grad, err_g)
         assert_close(log_probs, l, ref.U * np.abs(l))
+
+
+def test_pairs_of_scores_that_the_call_before_makes():
+    """Log-probabilities as the scores of pairs: the launch of the pairs may begin before they are written."""
+    rng = np.random.default_rng(31)
+    lengths = [40, 3000, 60_000, 7] * 3
+    n, group = sum(lengths), np.repeat(np.arange(12), lengths)
+    groups = O.RowGroups(group)
+    c, j = _pairs(rng, n, 400_000, 2, n)
+    pairs = O.RowPairs(c, j, n)
+    inputs = [_scores(rng, n, torch.float32, spread) for spread in (1.0, 3.0, 0.1)]
+    torch.cuda.synchronize()
+    got = [O.preference_loss(O.group_log_probs(x, groups), pairs, beta=0.5) for _ in range(6) for x, _ in inputs]
+    for i, (loss, grad) in enumerate(got):
+        l = O.group_log_probs(inputs[i % 3][0], groups).double().cpu().numpy()
+        want, want_grad, err_l, err_g = ref.pair_loss(l, c, j, beta=0.5)
+        assert_close(loss, want, err_l)
+        assert_close(grad, want_grad, err_g)
