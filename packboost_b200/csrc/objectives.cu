@@ -457,7 +457,7 @@ struct Rows {
     // at a time: interleaved lists of 1M rows took 39 us with all at once, which spills, and 35 so)
     static constexpr bool LATE = OP == kPolicy && N > 4;
     static constexpr int HELD = LATE ? 4 : N;
-    float s[N], main[N], old[HELD], reference[HELD];
+    alignas(16) float s[N], main[N], old[HELD], reference[HELD];  // (four of them are moved as one word)
     double loss = 0.0, kl = 0.0, share = 0.0;
     int clipped = 0;
     static_assert(!VECTOR || N == 4, "rows of a word");
@@ -717,6 +717,7 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
     let_next_start();
     constexpr int kStep = THREADS * kBlockRows;
     using Four = Rows<T, OP, kBlockRows, VECTOR>;
+    static_assert(alignof(Four) % 16 == 0, "four rows are moved as one word");
     float4* const kept_p = kept4 + threadIdx.x;
     float4* const kept_fixed = kept4 + most / 4 + threadIdx.x;
     double loss = 0.0, kl = 0.0;
