@@ -137,7 +137,7 @@ __device__ __forceinline__ void put_totals(const Totals& out, int slot, double l
 struct PairArgs {
     pb_pairs p;
     float beta, beta_log2e, smoothing, half_tau;  // half_tau: 1 / (2 beta)
-    float factor;                                 // of the sum of a row's terms: scale and what the terms leave out
+    double factor;                                // of the sum of a row's terms: scale and what the terms leave out (32 bits need not hold it)
     double* sums;                                 // [n_chunks]
     unsigned* counts;                             // [n_split], 0 before and after
 };
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
         sum = warp_sum(sum);
         if (lane == 0) {
             if (of.z == 1)
-                grad[row] = from_f32<T>((float)sum * a.factor);
+                grad[row] = from_f32<T>((float)(sum * a.factor));
             else
                 a.sums[k] = sum;
         }
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
             for (int i = lane; i < of.z; i += 32) sum += __ldcg(a.sums + of.y + i);
             sum = warp_sum(sum);
             if (lane == 0) {
-                grad[a.p.chunks[8 * (int64_t)k]] = from_f32<T>((float)sum * a.factor);
+                grad[a.p.chunks[8 * (int64_t)k]] = from_f32<T>((float)(sum * a.factor));
                 a.counts[of.x] = 0u;
             }
         }
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(PairArgs a, const T*
         else if (columns - c == 1)
             slice_columns<1, T, SQUARED>(a, scores, item, c, chosen, want, r);
         loss = r.loss;
-        if (mine.x >= 0) grad[mine.x] = from_f32<T>((float)r.sum0 * a.factor);
-        if (mine.z >= 0) grad[mine.z] = from_f32<T>((float)r.sum1 * a.factor);
+        if (mine.x >= 0) grad[mine.x] = from_f32<T>((float)(r.sum0 * a.factor));
+        if (mine.z >= 0) grad[mine.z] = from_f32<T>((float)(r.sum1 * a.factor));
         slice = next_slice;
         mine = next_mine;
     }
@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
 
 // ---- launches ---------------------------------------------------------------------------------------
 
-constexpr double kMostFactor = 1e30;
+constexpr double kMostFactor = 1e30, kLeastSquaredBeta = 1e-15;
 constexpr int64_t kMost = (1ll << 31) - 1;
 constexpr int64_t kMostRows = PB_OBJECTIVE_MOST_ROWS;  // (a CTA's places past the last row are still 32-bit numbers)
 
@@ -921,6 +921,8 @@ int check_objective(const pb_objective* o) {
     if (o->kind == PB_OBJECTIVE_PREFERENCE) {
         PB_TRY(check_pairs(o->pairs));
         PB_REQUIRE(o->beta >= 1.0 / kMostFactor && o->beta <= kMostFactor, "beta outside [1e-30, 1e30]");
+        // (1 / (2 beta) and its square)
+        PB_REQUIRE(!o->squared || o->beta >= kLeastSquaredBeta, "beta of the squared form below 1e-15");
         PB_REQUIRE(o->smoothing >= 0.0 && o->smoothing < 0.5, "smoothing outside [0, 0.5)");
         return PB_OK;
     }
@@ -1016,7 +1018,7 @@ int launch_pairs(const pb_objective* o, const T* scores, T* grad, const Totals& 
     const pb_pairs& p = *o->pairs;
     unsigned* counts = reinterpret_cast<unsigned*>(scratch + kTicketBytes);
     double* sums = reinterpret_cast<double*>(scratch + kTicketBytes + align_up((size_t)p.n_split * 4, 8));
-    const PairArgs a{p, (float)o->beta, (float)(o->beta * 1.4426950408889634), (float)o->smoothing, (float)(0.5 / o->beta), (float)(o->scale * (o->squared ? 2.0 : o->beta)), sums, counts};
+    const PairArgs a{p, (float)o->beta, (float)(o->beta * 1.4426950408889634), (float)o->smoothing, (float)(0.5 / o->beta), o->scale * (o->squared ? 2.0 : o->beta), sums, counts};
     // It may be launched before the kernel in front of it has ended, and waits for that: 1.3 us less from one evaluation to the next
     // (of 18 for 2M pairs).  The SMs are full with its CTAs, so none of them waits where another should run; the kernels of groups
     // lose by it: CTAs that are early crowd on the SMs that are free first, 100 groups of 5 000 rows took 14 us for 10.

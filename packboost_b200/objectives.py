@@ -345,7 +345,7 @@ class _Layout:
 class RowPairs(_Layout):
     """Pairs of rows, the first preferred to the second, laid out for :func:`preference_loss`.
 
-    ``weight`` counts a pair so many times; ``reference`` holds the scores of a reference model for all rows
+    ``weight`` counts a pair so many times (its product with the pair's loss or slope is a float32); ``reference`` holds the scores of a reference model for all rows
     (those of compared rows finite), so that differences of scores become differences of log ratios: where the
     scores are log-probabilities, or differ from them by something the two rows share, that is the paired log
     ratio of the model to the reference.  A pair may occur more than once; a row is not compared with itself."""
@@ -434,6 +434,8 @@ def _preference_struct(pairs: RowPairs, beta, label_smoothing, kind, reduction) 
         raise ValueError(f"unknown kind {kind!r}")
     if kind == "squared" and smoothing:
         raise ValueError("the squared form has no label smoothing")
+    if kind == "squared" and beta < 1e-15:
+        raise ValueError("beta of the squared form below 1e-15: float32 does not hold the square of 1 / (2 beta)")
     struct = B.Objective(kind=_PREFERENCE, pairs=C.pointer(pairs._struct), beta=beta, smoothing=smoothing,
                          squared=int(kind == "squared"), scale=_scale(reduction, pairs.total_weight, "pairs"))
     return _kept_struct(pairs, options, struct)

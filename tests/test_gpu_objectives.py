@@ -700,3 +700,28 @@ def test_pairs_of_scores_that_the_call_before_makes():
         want, want_grad, err_l, err_g = ref.pair_loss(l, c, j, beta=0.5)
         assert_close(loss, want, err_l)
         assert_close(grad, want_grad, err_g)
+
+
+@pytest.mark.parametrize("hubs", [0, 1], ids=["slices", "chunks"])
+@pytest.mark.parametrize("beta,size,kind", [(1e20, 1e-24, "logistic"), (1e30, 1e-25, "logistic"), (1e-30, 1e30, "logistic"), (1e-15, 1e-25, "squared")])
+def test_factors_beyond_float32(beta, size, kind, hubs):
+    """Beta, the weights and a mean over them are float32 numbers, their product need not be one: the gradients are still the
+    definition's, and 0 for rows in no pair."""
+    rng = np.random.default_rng(41)
+    rows, pairs = 3000, 4000
+    c, j = _pairs(rng, rows, pairs, hubs, 2000)
+    # whole numbers: differences are 0 or beyond what the sigmoid notices at a large beta
+    s = rng.integers(-3, 4, rows).astype(np.float64)
+    w = (rng.integers(1, 5, pairs) * size).astype(np.float32)
+    got = O.preference_loss(_cuda(s.astype(np.float32)), O.RowPairs(c, j, rows, weight=w), beta=beta, kind=kind, reduction="mean")
+    loss, grad, err_l, err_g = ref.pair_loss(s, c, j, weight=w, beta=beta, kind=kind, reduction="mean")
+    if beta > 1:
+        # (a step of d = 0, and differences that are exact: only the sigmoid's roundings and the sums' are left, 23 of them)
+        z = beta * (s[c] - s[j])
+        slope = np.where(z == 0, -0.5, np.where(z > 0, 0.0, -1.0)) * beta
+        w64 = w.astype(np.float64)
+        grad = (np.bincount(c, w64 * slope, rows) - np.bincount(j, w64 * slope, rows)) / w64.sum()
+        err_g = 24 * ref.U * (np.bincount(c, w64, rows) + np.bincount(j, w64, rows)) * beta / w64.sum()
+    assert_close(got.grad, grad, err_g)
+    assert_close(got.loss, loss, err_l)
+    assert (got.grad[2000:] == 0).all()

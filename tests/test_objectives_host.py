@@ -350,3 +350,19 @@ def test_items_are_ordered_for_any_number_of_rows(n_rows):
     owner = rng.choice(near, 400) + n_rows * rng.integers(0, 2, 400)
     order = O._item_order(torch.from_numpy(owner), torch.from_numpy(other), n_rows).numpy()
     np.testing.assert_array_equal(order, np.lexsort((other, owner)))   # (stable, like the sort)
+
+
+def test_refused_squared_forms_of_tiny_beta():
+    """1 / (2 beta) squared is a float32 number."""
+    pairs = B.Pairs(n_rows=2, n_slices=1, slices=16, slice_rows=16, other=16)
+    for beta in (9e-16, 1e-20, 1e-30):
+        with pytest.raises(ValueError, match="squared"):
+            O._preference_struct(_Stub(2, struct=pairs, total_weight=1.0), beta, 0.0, "squared", "sum")
+        o = B.Objective(kind=0, pairs=C.pointer(pairs), beta=beta, squared=1, scale=1.0)
+        with pytest.raises(ValueError, match="squared"):
+            B.check(B.lib().pb_objective_evaluate(C.byref(o), 16, 0, 16, 16, None, None, 16, 1 << 20, None))
+        assert B.lib().pb_objective_workspace_bytes(C.byref(o)) < 0
+        o.squared = 0
+        assert B.lib().pb_objective_workspace_bytes(C.byref(o)) > 0
+        O._preference_struct(_Stub(2, struct=pairs, total_weight=1.0), beta, 0.0, "logistic", "sum")
+    O._preference_struct(_Stub(2, struct=pairs, total_weight=1.0), 1e-15, 0.0, "squared", "sum")
