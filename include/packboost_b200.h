@@ -379,7 +379,7 @@ typedef struct pb_winner {
 typedef struct pb_round_log_header {
     double root_value;
     float scale;          /* gq = rint(g * scale) */
-    float max_abs_grad;
+    float max_abs_grad;   /* of an objective's gradient: not finite where one of a row is not; the round is not to be used */
     int64_t root_gq;
     int32_t n_ctx[PB_MAX_DEPTH + 1]; /* frontier nodes per depth; winners of depth d start at (1<<d)-1 */
     int32_t n_tree_nodes;

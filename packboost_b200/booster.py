@@ -801,7 +801,8 @@ class PackBoost:
         ``objective`` (a ``PreferenceObjective``, ``ChoiceObjective`` or ``PolicyObjective`` of
         :mod:`packboost_b200.objectives`, on the rows of ``X``) takes the place of the squared loss; ``y``
         then only serves the correlations of ``round_metrics``, which have a ``train_loss`` beside them, and
-        may be ``None``."""
+        may be ``None``.  A round whose gradient is not finite ends the fit with a ``RuntimeError``; the trees of
+        the rounds before it stay."""
         self._start(X, y, era, feature_names=feature_names, eval_sets=eval_sets, objective=objective)
         for round_idx in range(num_rounds):
             metrics = self._boost_one_round(round_idx, num_rounds, round_callback is not None)
@@ -1026,6 +1027,11 @@ class PackBoost:
         ticket, state0 = inflight
         D = int(self.config.max_depth)
         head, winners = self._trainer.read_log(ticket)
+        if self._trainer.objective is not None and not np.isfinite(head["max_abs_grad"]):
+            self._inflight = self._predrawn = None     # (a round that follows stands on this one)
+            self._trainer.release_graph()
+            self._trainer.close_comm()
+            raise RuntimeError(f"round {len(self._round_depths) + 1}: the objective's gradient is not finite")
         n_ctx = head["n_ctx"][: D + 1].tolist()
         self._last_n_ctx = n_ctx
         used = next((d for d in range(D) if n_ctx[d] == 0), D)

@@ -139,9 +139,10 @@ __global__ void __launch_bounds__(kRowThreads) quantise_kernel(
     }
 }
 
-// The same two steps for a gradient that an objective left, as float32 bits, in the place of gq.
+// The same two steps for a gradient that an objective left, as float32 bits, in the place of gq.  The largest is that of the bits
+// without the sign: a NaN is above infinity and both above all numbers, so that the round's log tells of them.
 __global__ void __launch_bounds__(kRowThreads) gradient_absmax_kernel(const int32_t* __restrict__ gq, int64_t n, CtlHead* head) {
-    float m = 0.f;
+    uint32_t m = 0u;
     const int64_t n4 = (n + 3) >> 2;   // (gq is padded beyond n; what lies there is not looked at)
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n4; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i << 2;
@@ -149,10 +150,10 @@ __global__ void __launch_bounds__(kRowThreads) gradient_absmax_kernel(const int3
         const int q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-            if (r + u < n) m = fmaxf(m, fabsf(__int_as_float(q[u])));
+            if (r + u < n) m = max(m, (uint32_t)q[u] & 0x7FFFFFFFu);
     }
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    if ((threadIdx.x & 31) == 0) atomicMax(&head->max_abs_bits, __float_as_uint(m));
+    m = __reduce_max_sync(0xFFFFFFFFu, m);
+    if ((threadIdx.x & 31) == 0) atomicMax(&head->max_abs_bits, m);
 }
 
 __global__ void __launch_bounds__(kRowThreads) quantise_gradient_kernel(int32_t* __restrict__ gq, uint16_t* __restrict__ slot,
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kRowThreads) quantise_gradient_kernel(int32_t*
                                                                         CtlHead* head, int gq_bits) {
     float inv;
     const float scale = scale_from_max(__uint_as_float(head->max_abs_bits), gq_bits, &inv);
-    const float most = ldexpf(1.f, gq_bits);   // (only a gradient that is not finite is beyond it)
+    const float most = ldexpf(1.f, gq_bits);   // (only where one is not finite are there any beyond it)
     long long acc = 0;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (n_pad >> 2); i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i << 2;

@@ -725,3 +725,46 @@ def test_factors_beyond_float32(beta, size, kind, hubs):
     assert_close(got.grad, grad, err_g)
     assert_close(got.loss, loss, err_l)
     assert (got.grad[2000:] == 0).all()
+
+
+@pytest.mark.parametrize("env", [{}, {"PACKBOOST_CUDA_GRAPH": "0"}, {"PACKBOOST_RUN_AHEAD": "0"}, {"PACKBOOST_TRAIN_METRICS": "1"}])
+@pytest.mark.parametrize("both", [False, True], ids=["infinite", "no number"])
+def test_fit_with_a_gradient_that_is_not_finite(env, both, monkeypatch):
+    """A ratio beyond float32 (two of either sign in a group: infinity less infinity) ends the fit."""
+    for k, v in env.items():
+        monkeypatch.setenv(k, v)
+    X, era, rng = _table(seed=9)
+    n = len(X)
+    group = np.arange(n) // 12
+    a, old = rng.normal(size=n), np.full(n, -np.log(12.0))
+    a[120], old[120] = -1.0, -120.0
+    if both:
+        a[121], old[121] = 1.0, -120.0
+    objective = O.PolicyObjective(a, old, group=group, clip=(0.2, np.inf))
+    b = PackBoost(PackBoostConfig(**CFG))
+    with pytest.raises(RuntimeError, match="round 1: .*not finite"):
+        b.fit(X, None, era, num_rounds=5, objective=objective)
+    assert len(b.trees) == 0
+    # and the same booster goes on to other fits
+    b._rng.manual_seed(CFG["random_state"])
+    b.fit(X, a, era, num_rounds=3)
+    _same_trees(b, PackBoost(PackBoostConfig(**CFG)).fit(X, a, era, num_rounds=3))
+
+
+def test_fit_whose_gradient_overflows_later_keeps_the_trees_before():
+    """Tiny gains of a ratio near the end of float32 (e^87.5) raise the chosen rows' scores until it is beyond."""
+    n = 1200
+    group, chosen = np.arange(n) // 12, np.arange(n) % 12 == 0
+    X = np.random.default_rng(10).normal(size=(n, 4)).astype(np.float32)
+    X[:, 0] = chosen                                  # a leaf of its own: all chosen rows, with a slope of -10 (1 - 1/12) each
+    a = np.where(chosen, 1e-37, 0.0)
+    old = np.full(n, -np.log(12.0) - 87.5)
+    b = PackBoost(PackBoostConfig(**dict(CFG, layer_feature_fraction=1.0)))
+    with pytest.raises(RuntimeError, match="not finite") as e:
+        b.fit(X, None, np.zeros(n, np.int16), num_rounds=50, objective=O.PolicyObjective(a, old, group=group, clip=(0.2, np.inf)))
+    done = int(str(e.value).split(":")[0].split()[1]) - 1
+    assert done >= 1 and len(b.trees) == done * CFG["pack_size"]
+    value = b.trees[0].arrays()["value"]
+    # (the leaf of the chosen rows: 10 (1 - 1/12) 100 / (100 + lambda), up to the float32 of advantage and old)
+    want = 1e-37 * np.exp(87.5) * (11 / 12) * 100 / 101
+    assert abs(value.max() / want - 1) < 1e-4
