@@ -186,6 +186,8 @@ inline int64_t rows_padded(int64_t n) { return (n + 255) / 256 * 256; }
 
 // Checks a descriptor; n_rows >= 0: it has to be about so many rows.
 int objective_check(const pb_objective* o, int64_t n_rows);
+// Checks the workspace of a checked one.
+int objective_check_workspace(const pb_objective* o, const void* workspace, int64_t workspace_bytes);
 // Gradient and totals (null: not wanted; the workspace is theirs) of a checked objective.
 int objective_gradient(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss, float* kl,
                        int64_t* clipped, void* workspace, int64_t workspace_bytes, cudaStream_t stream);

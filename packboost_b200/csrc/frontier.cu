@@ -985,6 +985,7 @@ extern "C" int pb_round_begin_objective(const pb_train_state* st, const pb_objec
     NvtxRange nvtx("pb.round_begin_objective apply=%lld", (long long)apply_previous);
     PB_TRY(check_state(st));
     PB_TRY(objective_check(o, st->n_rows));
+    PB_TRY(objective_check_workspace(o, workspace, workspace_bytes));  // (a call that is refused leaves the state as it was)
     cudaStream_t stream = (cudaStream_t)stream_;
     Ctl c = ctl_view(st->ctl);
     const int g = row_grid(st->n_rows);

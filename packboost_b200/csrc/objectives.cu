@@ -1110,10 +1110,14 @@ int objective_gradient(const pb_objective* o, const void* scores, int64_t score_
     PB_REQUIRE(score_type >= PB_SCORE_F32 && score_type <= PB_SCORE_BF16, "unknown type of scores %lld", (long long)score_type);
     if (n_rows_of(o) == 0) return no_totals(loss, kl, clipped, stream);
     PB_REQUIRE(scores && grad, "scores or gradient is null");
-    PB_TRY(check_scratch(workspace, workspace_bytes, scratch_bytes(o)));
+    PB_TRY(objective_check_workspace(o, workspace, workspace_bytes));
     if (score_type == PB_SCORE_F32) return launch_objective<float>(o, scores, grad, loss, kl, clipped, workspace, stream);
     if (score_type == PB_SCORE_F16) return launch_objective<__half>(o, scores, grad, loss, kl, clipped, workspace, stream);
     return launch_objective<__nv_bfloat16>(o, scores, grad, loss, kl, clipped, workspace, stream);
+}
+
+int objective_check_workspace(const pb_objective* o, const void* workspace, int64_t workspace_bytes) {
+    return check_scratch(workspace, workspace_bytes, scratch_bytes(o));
 }
 
 int objective_check(const pb_objective* o, int64_t n_rows) {

@@ -768,3 +768,25 @@ def test_fit_whose_gradient_overflows_later_keeps_the_trees_before():
     # (the leaf of the chosen rows: 10 (1 - 1/12) 100 / (100 + lambda), up to the float32 of advantage and old)
     want = 1e-37 * np.exp(87.5) * (11 / 12) * 100 / 101
     assert abs(value.max() / want - 1) < 1e-4
+
+
+def test_a_refused_round_leaves_the_state_as_it_was():
+    """Too small a workspace: nothing is launched, in particular not the last round's step of the predictions."""
+    import ctypes as C
+    from packboost_b200 import backends as B
+    X, era, rng = _table(seed=12)
+    objective, _ = _objectives(len(X), era, rng)[0]
+    want = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=4, objective=objective)
+    got = PackBoost(PackBoostConfig(**CFG))
+    got._start(X, None, era, objective=objective)
+    tr = got._trainer
+    for r in range(4):
+        got._boost_one_round(r, 4)
+        before = tr.preds.clone()
+        struct, scratch, nbytes = tr._objective_args()
+        for address, size, error in ((scratch, nbytes - 1, RuntimeError), (None, nbytes, ValueError), (scratch + 4, nbytes, ValueError)):
+            with pytest.raises(error, match="workspace"):
+                B.check(B.lib().pb_round_begin_objective(C.byref(tr.st), struct, 1, address, size, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(tr.preds, before)
+    got._finish()
+    _same_trees(want, got)
