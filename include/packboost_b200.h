@@ -504,8 +504,8 @@ int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_typ
 int pb_round_begin_objective(const pb_train_state* st, const pb_objective* o, int64_t apply_previous, void* workspace,
                              int64_t workspace_bytes, void* stream);
 
-/* pb_loop_submit with such a round.  What the descriptor says stays the same as long as its address and the
- * workspace's do (a round captured with them is replayed). */
+/* pb_loop_submit with such a round.  A captured round is replayed as long as the descriptor, what it points at on the
+ * host and the workspace say the same, and captured again when they do not. */
 int pb_loop_submit_objective(void* loop, const pb_train_state* st, const pb_objective* o, void* workspace,
                              int64_t workspace_bytes, int64_t slot, const int32_t* lists_host, int32_t* lists_dev,
                              int64_t k, void* log_host, int64_t apply_previous, int64_t use_graph, void* stream);

@@ -3,6 +3,8 @@
 // arrays.  Through the interpreter these steps cost 0.3 to 0.4 ms a round, more than a small table's
 // round takes on the device.
 
+#include <string.h>
+
 #include <new>
 
 #include "common.cuh"
@@ -13,24 +15,47 @@ namespace {
 
 constexpr int kLoopSlots = 8;
 
-struct RoundLoop {
-    cudaEvent_t logged[kLoopSlots] = {};
-    cudaGraphExec_t exec = nullptr;
-    bool no_graph = false;  // a capture failed: rounds are launched one kernel at a time
-    int64_t graph_k = 0, graph_launches = 0, replays = 0;
-    const void *graph_objective = nullptr, *graph_workspace = nullptr;  // what the captured round learns from
-    ~RoundLoop() {
-        if (exec) cudaGraphExecDestroy(exec);
-        for (auto e : logged)
-            if (e) cudaEventDestroy(e);
-    }
-};
-
 // What a round learns from: the squared difference to the targets, or an objective with its scratch.
 struct RoundLoss {
     const pb_objective* objective;
     void* workspace;
     int64_t workspace_bytes;
+};
+
+// The same by value: all that the launches of a round take from it, wherever its descriptors lie on the host.
+struct LossValues {
+    pb_objective objective;
+    pb_pairs pairs;
+    pb_groups groups;
+    void* workspace;
+    int64_t workspace_bytes;
+};
+
+LossValues values_of(const RoundLoss& loss) {
+    LossValues v;
+    memset(&v, 0, sizeof(v));  // (without an objective: all zero; one has a workspace)
+    if (!loss.objective) return v;
+    v.objective = *loss.objective;
+    if (v.objective.kind == PB_OBJECTIVE_PREFERENCE && v.objective.pairs) v.pairs = *v.objective.pairs;
+    if (v.objective.kind != PB_OBJECTIVE_PREFERENCE && v.objective.groups) v.groups = *v.objective.groups;
+    v.objective.pairs = nullptr;
+    v.objective.groups = nullptr;
+    v.workspace = loss.workspace;
+    v.workspace_bytes = loss.workspace_bytes;
+    return v;
+}
+
+struct RoundLoop {
+    cudaEvent_t logged[kLoopSlots] = {};
+    cudaGraphExec_t exec = nullptr;
+    bool no_graph = false;  // a capture failed: rounds are launched one kernel at a time
+    int64_t graph_k = 0, graph_launches = 0, replays = 0;
+    LossValues graph_loss = {};  // what the captured round learns from
+    ~RoundLoop() {
+        if (exec) cudaGraphExecDestroy(exec);
+        for (auto e : logged)
+            if (e) cudaEventDestroy(e);
+    }
 };
 
 // lists: device [max_depth][3][k]: global ids, local rows, positions of the sampled features
@@ -64,8 +89,7 @@ int capture_round(RoundLoop* loop, const pb_train_state* st, const RoundLoss& lo
     if (rc) return rc;
     if (e != cudaSuccess) return fail_cuda(e, "round graph");
     loop->graph_k = k;
-    loop->graph_objective = loss.objective;
-    loop->graph_workspace = loss.workspace;
+    loop->graph_loss = values_of(loss);
     loop->graph_launches = pb_launch_count() - before;
     return PB_OK;
 }
@@ -103,8 +127,8 @@ static int submit_round(void* loop_, const pb_train_state* st, const RoundLoss& 
     PB_CUDA_TRY(cudaMemcpyAsync(lists_dev, lists_host, (size_t)(st->max_depth * 3 * k) * 4, cudaMemcpyHostToDevice, stream));
     // the launches of a round are the same every time: from the second round on they are replayed
     const bool graph = use_graph && apply_previous;
-    if (graph && !loop->no_graph &&
-        (!loop->exec || loop->graph_k != k || loop->graph_objective != loss.objective || loop->graph_workspace != loss.workspace)) {
+    const LossValues values = values_of(loss);
+    if (graph && !loop->no_graph && (!loop->exec || loop->graph_k != k || memcmp(&loop->graph_loss, &values, sizeof(values)) != 0)) {
         if (loop->exec) cudaGraphExecDestroy(loop->exec);
         loop->exec = nullptr;
         if (capture_round(loop, st, loss, lists_dev, k) != PB_OK) {

@@ -790,3 +790,26 @@ def test_a_refused_round_leaves_the_state_as_it_was():
         assert torch.equal(tr.preds, before)
     got._finish()
     _same_trees(want, got)
+
+
+def test_a_descriptor_that_changes_in_its_place(monkeypatch):
+    """Rounds that are replayed learn from what the descriptor says now, not from what it said when one was captured."""
+    X, era, rng = _table(seed=13)
+    objective, _ = _objectives(len(X), era, rng)[0]
+
+    def fit(change, graphs):
+        monkeypatch.setenv("PACKBOOST_CUDA_GRAPH", graphs)
+        b = PackBoost(PackBoostConfig(**CFG))
+        b._start(X, None, era, objective=objective)
+        for r in range(8):
+            if change and r == 4:
+                b._trainer.objective.struct.beta = 0.05
+            b._boost_one_round(r, 8)
+        replays = b._trainer.graph_replays
+        b._finish()
+        return b, replays
+
+    (plain, none), (replayed, some), (other, _) = fit(True, "0"), fit(True, "1"), fit(False, "1")
+    assert none == 0 and some >= 6
+    _same_trees(plain, replayed)
+    assert not np.array_equal(plain.train_predictions(), other.train_predictions())
