@@ -38,11 +38,15 @@ import torch
 
 from . import backends as B
 
-# (what torch.cuda.current_device, current_stream().cuda_stream and is_current_stream_capturing come down to; a call of ten
-# microseconds notices the rest)
-_device_now = getattr(torch._C, "_cuda_getDevice", None)
-_stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+
+def _quick(name: str, public):
+    """torch's own binding behind a public function (a call of ten microseconds notices the rest), or that function."""
+    return getattr(torch._C, name, None) or public
+
+
+_device_now = _quick("_cuda_getDevice", torch.cuda.current_device)
+_stream_now = _quick("_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+_capturing = _quick("_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 _SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _MOST = (1 << 31) - (1 << 16)    # rows, and items (two per pair): 32-bit numbers

@@ -813,3 +813,22 @@ def test_a_descriptor_that_changes_in_its_place(monkeypatch):
     assert none == 0 and some >= 6
     _same_trees(plain, replayed)
     assert not np.array_equal(plain.train_predictions(), other.train_predictions())
+
+
+def test_calls_through_the_public_functions(monkeypatch):
+    """Where torch has no quicker ones."""
+    args = _problem(14, 9500)
+    want = _all(*args)
+    monkeypatch.setattr(O, "_device_now", O._quick("_not_there", torch.cuda.current_device))
+    monkeypatch.setattr(O, "_stream_now", O._quick("_not_there", lambda index: torch.cuda.current_stream(index).cuda_stream))
+    monkeypatch.setattr(O, "_capturing", O._quick("_not_there", torch.cuda.is_current_stream_capturing))
+    got = _all(*args)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _all(*args)
+    side.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        _all(*args)

@@ -366,3 +366,11 @@ def test_refused_squared_forms_of_tiny_beta():
         assert B.lib().pb_objective_workspace_bytes(C.byref(o)) > 0
         O._preference_struct(_Stub(2, struct=pairs, total_weight=1.0), beta, 0.0, "logistic", "sum")
     O._preference_struct(_Stub(2, struct=pairs, total_weight=1.0), 1e-15, 0.0, "squared", "sum")
+
+
+def test_public_functions_where_torch_has_no_quicker_ones():
+    def public():
+        return 7
+    assert O._quick("_a_name_that_is_not_there", public) is public
+    for name in ("_device_now", "_stream_now", "_capturing"):
+        assert callable(getattr(O, name))
