@@ -392,7 +392,9 @@ __device__ __forceinline__ float sum_of(Pair32 x) { return x.hi + fminf(x.lo, 1.
 // part of itself would be no number.  (574 groups of a policy: 27.5 us so, 28.1 with a choice after the product, 26.7 without.)
 template <bool BEYOND>
 __device__ __forceinline__ float exp_of(Pair32 x) {
-    const float log2e = 1.44269502f, rest = 1.33687e-8f;  // log2 e as a float, and (log2 e - that) ln 2
+    constexpr float log2e = 1.44269502f, rest = 1.33498e-8f;  // log2 e as a float, and (log2 e - that) ln 2
+    constexpr double off = (1.4426950408889634 - (double)log2e) * 0.6931471805599453 - (double)rest;
+    static_assert(off < 1e-13 && off > -1e-13, "what the float of log2 e leaves out");
     float y = x.hi * log2e;
     if (BEYOND) asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(127.999992f));  // (the largest float below 128)
     float more = fmaf(fmaf(x.hi, log2e, -y), 0.693147181f, x.lo);
@@ -401,9 +403,10 @@ __device__ __forceinline__ float exp_of(Pair32 x) {
     return fmaf(e, more, e);
 }
 
-// exp(x) for x <= 0, to 7e-15 of the value and exactly 1 at 0: with n = rint(x / ln 2), 2^n times the Taylor
-// polynomial of degree 11 at |f| <= ln 2 / 2.  Below -700: 0.  (The log of the sum has to be exact to some 1e-13: a
-// divergence of nearly equal policies is a mean of differences of that size.)
+// exp(x) for x <= 0, exactly 1 at 0: with n = rint(x / ln 2), 2^n times the Taylor polynomial of degree 11 at
+// |f| <= ln 2 / 2.  Off by up to 1.1e-14 of the value from -60 on (7e-15 the rest of the polynomial, and 2.3e-17 a unit of n the one
+// constant for ln 2), by 3.1e-14 near -700; below that: 0.  (The log of the sum has to be exact to some 1e-13: a divergence of nearly
+// equal policies is a mean of differences of that size.)
 __device__ __forceinline__ double exp_negative(double x) {
     const double shift = 6755399441055744.0;  // 1.5 * 2^52: the low word of x + shift is x as an integer
     const double t = fma(x, 1.4426950408889634, shift);
