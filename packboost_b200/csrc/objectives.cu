@@ -1072,7 +1072,7 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
     if (g.n_pieces) {
         PieceSums* sums = reinterpret_cast<PieceSums*>(scratch + kTicketBytes);
         PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceMass>, g.n_pieces, kPieceThreads, 0, early, stream, a, sums, slot, scores, out, totals));
-        if (OP == kPolicy)
+        if constexpr (OP == kPolicy)
             PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceTerms>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
         PB_CUDA_TRY(launch(piece_kernel<T, OP, kPieceOut>, g.n_pieces, kPieceThreads, 0, true, stream, a, sums, slot, scores, out, totals));
     }
