@@ -832,3 +832,46 @@ def test_calls_through_the_public_functions(monkeypatch):
     assert all(torch.equal(g, w) for g, w in zip(got, want))
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         _all(*args)
+
+
+@pytest.mark.parametrize("kind", ["blocks", "many"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+def test_kernels_of_many_groups(kind, dtype, mixed):
+    """Tables of some hundred eras: CTAs of 256 threads for a group each, and for one group after the other; a group with nothing
+    left, and arrays that do not begin on the border of a word."""
+    lengths = KINDS[kind] + ([8192, 5000, 8191] if kind == "blocks" else [])
+    n, n_groups = sum(lengths), len(lengths)
+    rng = np.random.default_rng(n + 1)
+    group = _groups(rng, lengths, mixed)
+    plan = O.RowGroups(group, n_groups)
+    x, s = _scores(rng, n, dtype, 2.0)
+    off = (rng.random(n) < 0.1) | (group == 7)
+    x[_cuda(off)] = -np.inf
+    s[off] = -np.inf
+    t = np.where(off | (rng.random(n) < 0.5), 0.0, rng.random(n)).astype(np.float32)
+    a = np.where(off, np.nan, np.where(rng.random(n) < 0.4, 0.0, rng.normal(size=n))).astype(np.float32)
+    live = np.where(off, 0.0, s)
+    old = ref.log_probs(live + 0.3 * rng.normal(size=n), group, n_groups).astype(np.float32)
+    prior = ref.log_probs(live + 0.5 * rng.normal(size=n), group, n_groups).astype(np.float32)
+    old[off | (a == 0)] = np.nan
+    prior[off] = np.nan
+    l = ref.log_probs(s, group, n_groups)
+    opts = dict(kl_coef=0.1, clip=(0.1, 0.3))
+    want_c = ref.choice(s, group, n_groups, t, "mean")
+    loss_p, grad_p, kl, clipped, err_l, err_g, err_k = ref.policy(s, group, n_groups, np.where(off, 0, a), old, prior, **opts)
+    for shift in (0, 1):
+        def put(v):
+            v = v if isinstance(v, torch.Tensor) else _cuda(v)
+            return torch.cat([v.new_zeros(shift), v])[shift:]
+        y = put(x)
+        assert_close(O.group_log_probs(y, plan), l, ref.U * np.where(np.isfinite(l), np.abs(l), 0))
+        got = O.choice_loss(y, plan, put(t), reduction="mean")
+        assert got.grad.dtype == dtype
+        assert_close(got.loss, want_c[0], want_c[2])
+        assert_close(got.grad, want_c[1], want_c[3])
+        got = O.policy_loss(y, plan, put(a), put(old), reference_log_probs=put(prior), **opts)
+        assert int(got.clipped) == clipped
+        assert_close(got.loss, loss_p, err_l)
+        assert_close(got.kl, kl, err_k)
+        assert_close(got.grad, grad_p, err_g)
