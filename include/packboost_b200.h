@@ -487,13 +487,13 @@ int64_t pb_objective_struct_bytes(int64_t which);
  * zero it leaves so, unless it fails.  Evaluations that may run at the same time need one each. */
 int64_t pb_objective_workspace_bytes(const pb_objective* o);
 
-/* Gradient with respect to the scores [n_rows] (of the scores' type), the loss and, for a policy, the
+/* Gradient with respect to the scores [n_rows] (of the scores' type, and not in their place), the loss and, for a policy, the
  * scaled divergence and the number of rows whose ratio is beyond its border.  `loss`, `kl` and
  * `clipped` are on the device and may be NULL. */
 int pb_objective_evaluate(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss,
                           float* kl, int64_t* clipped, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Log-probabilities of the rows in their groups (of the scores' type; -inf where the score is), with
+/* Log-probabilities of the rows in their groups (of the scores' type, not in their place; -inf where the score is), with
  * scratch of pb_group_log_probs_bytes(g) bytes. */
 int64_t pb_group_log_probs_bytes(const pb_groups* g);
 int pb_group_log_probs(const pb_groups* g, const void* scores, int64_t score_type, void* out, void* workspace,

@@ -1106,6 +1106,13 @@ int check_scratch(const void* workspace, int64_t given, int64_t need) {
     return PB_OK;
 }
 
+// (a row's score is read for other rows too, after its own result is written)
+int check_apart(const void* scores, const void* out, int64_t n_rows, int64_t score_type) {
+    const uintptr_t a = (uintptr_t)scores, b = (uintptr_t)out, bytes = (uintptr_t)n_rows * (score_type == PB_SCORE_F32 ? 4 : 2);
+    PB_REQUIRE(a + bytes <= b || b + bytes <= a, "what is written overlaps the scores");
+    return PB_OK;
+}
+
 }  // namespace
 
 int objective_gradient(const pb_objective* o, const void* scores, int64_t score_type, void* grad, float* loss, float* kl,
@@ -1114,6 +1121,7 @@ int objective_gradient(const pb_objective* o, const void* scores, int64_t score_
     if (n_rows_of(o) == 0) return no_totals(loss, kl, clipped, stream);
     PB_REQUIRE(scores && grad, "scores or gradient is null");
     PB_TRY(objective_check_workspace(o, workspace, workspace_bytes));
+    PB_TRY(check_apart(scores, grad, n_rows_of(o), score_type));
     if (score_type == PB_SCORE_F32) return launch_objective<float>(o, scores, grad, loss, kl, clipped, workspace, stream);
     if (score_type == PB_SCORE_F16) return launch_objective<__half>(o, scores, grad, loss, kl, clipped, workspace, stream);
     return launch_objective<__nv_bfloat16>(o, scores, grad, loss, kl, clipped, workspace, stream);
@@ -1163,6 +1171,7 @@ extern "C" int pb_group_log_probs(const pb_groups* g, const void* scores, int64_
     if (g->n_rows == 0) return PB_OK;
     PB_REQUIRE(scores && out, "scores or output is null");
     if (g->n_pieces) PB_TRY(check_scratch(workspace, workspace_bytes, kTicketBytes + sums_bytes(g)));
+    PB_TRY(check_apart(scores, out, g->n_rows, score_type));
     cudaStream_t stream = (cudaStream_t)stream_;
     GroupArgs a{};
     a.g = *g;

@@ -374,3 +374,18 @@ def test_public_functions_where_torch_has_no_quicker_ones():
     assert O._quick("_a_name_that_is_not_there", public) is public
     for name in ("_device_now", "_stream_now", "_capturing"):
         assert callable(getattr(O, name))
+
+
+def test_library_refuses_results_in_the_place_of_scores():
+    """A row's score is read for other rows after its own result is written."""
+    lib = B.lib()
+    pairs = B.Pairs(n_rows=4, n_slices=1, slices=16, slice_rows=16, other=16)
+    groups = B.Groups(n_rows=4, n_groups=1, n_team_warps=1, team_warps=16, teams=16)
+    for o in (B.Objective(kind=0, pairs=C.pointer(pairs), beta=1.0, scale=1.0),
+              B.Objective(kind=1, groups=C.pointer(groups), target=16, scale=1.0)):
+        for typ, grad in ((0, 1024), (0, 1024 + 12), (0, 1024 - 12), (1, 1024 + 6), (2, 1024 - 6)):
+            with pytest.raises(ValueError, match="overlaps"):
+                B.check(lib.pb_objective_evaluate(C.byref(o), 1024, typ, grad, None, None, None, 4096, 1 << 20, None))
+    for typ, out in ((0, 1024), (0, 1036), (2, 1018)):
+        with pytest.raises(ValueError, match="overlaps"):
+            B.check(lib.pb_group_log_probs(C.byref(groups), 1024, typ, out, None, 0, None))
