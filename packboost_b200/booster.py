@@ -1502,7 +1502,7 @@ class PackBoost:
         earlier model are the old or reference log-probabilities of a ``PolicyObjective``."""
         from .objectives import RowGroups, group_log_probs
         groups = RowGroups(group, device=self._device)
-        if X.shape[0] != groups.n_rows:
+        if len(X) != groups.n_rows:
             raise ValueError("group must align with X rows")
         scores = torch.from_numpy(self.predict(X)).to(self._device)
         return group_log_probs(scores, groups).cpu().numpy()

@@ -875,3 +875,14 @@ def test_kernels_of_many_groups(kind, dtype, mixed):
         assert_close(got.loss, loss_p, err_l)
         assert_close(got.kl, kl, err_k)
         assert_close(got.grad, grad_p, err_g)
+
+
+def test_log_probs_of_whatever_predict_takes():
+    X, era, rng = _table(n=500, seed=15)
+    group = rng.integers(0, 40, 500)
+    b = PackBoost(PackBoostConfig(**CFG)).fit(X, None, era, num_rounds=2, objective=O.ChoiceObjective(rng.random(500), group=group))
+    want = b.predict_log_probs(X, group)
+    for other in (X.tolist(), torch.from_numpy(X), torch.from_numpy(X).cuda(), np.asfortranarray(X)):
+        np.testing.assert_array_equal(b.predict_log_probs(other, group.tolist()), want)
+        with pytest.raises(ValueError, match="align"):
+            b.predict_log_probs(other, group[1:])
