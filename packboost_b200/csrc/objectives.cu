@@ -795,9 +795,10 @@ __global__ void __launch_bounds__(THREADS) block_kernel(GroupArgs a, const int2*
 // Pieces of up to 2048 rows; the sums of a group's pieces go through memory from one launch to the next: sums of
 // exponentials, then (of a policy; a choice's are its targets, known at once) shares, then the gradient.  The rows are read
 // again each time, from L2 mostly, while the launch before still runs.
-struct PieceSums {
-    double z, share;
+struct alignas(16) PieceSums {
+    double z;
     float m, unused;
+    double share, unused2;
 };
 enum PieceStep { kPieceMass, kPieceTerms, kPieceOut };
 constexpr int kPieceThreads = 256;
@@ -856,8 +857,9 @@ __global__ void __launch_bounds__(kPieceThreads) piece_kernel(GroupArgs a, Piece
     float m = -INFINITY;
     double z = 0.0;
     for (int k = threadIdx.x; k < count; k += kPieceThreads) {
-        const float mk = __ldcg(&pieces[first + k].m), top = fmaxf(m, mk);
-        z = rescaled(z, m, top) + rescaled(__ldcg(&pieces[first + k].z), mk, top);
+        const float4 zm = __ldcg(reinterpret_cast<const float4*>(pieces + first + k));  // (z and m in one word)
+        const float mk = zm.z, top = fmaxf(m, mk);
+        z = rescaled(z, m, top) + rescaled(__hiloint2double(__float_as_int(zm.y), __float_as_int(zm.x)), mk, top);
         m = top;
     }
     const double lse = cta_log_sum<kPieceThreads>(m, z, s_m, s_z);
