@@ -443,7 +443,8 @@ typedef struct pb_pairs {
  *  - up to PB_TEAM_ROWS: 1, 2, 4 ... 32 lanes of a warp, the fewest that have at most eight rows each.
  *    `team_warps` holds for every warp its first entry of `teams` and log2 of the lanes (bits 0-7) with the most
  *    rows that a lane has (from bit 8); of `teams` a warp takes 32 >> log2(lanes) entries, of no rows some;
- *  - up to PB_BLOCK_ROWS: a CTA's, in `blocks` (`block_rows`: rows of the longest);
+ *  - up to PB_BLOCK_ROWS: a CTA's, in `blocks` (`block_rows`: rows of the longest; policy, a CTA or pieces: one group of 8 000 rows 11.7
+ *    and 13.6 us, 100 of 5 000 11.9 and 19.1, 574 of 4 700 24.9 and 53.0; log-probabilities of one group of 8 000 rows 6.1 and 4.8);
  *  - longer: pieces of up to PB_PIECE_ROWS: first place, rows, number of the group's first piece, number
  *    of its pieces. */
 #define PB_TEAM_ROWS 256

@@ -801,7 +801,8 @@ class PackBoost:
         ``objective`` (a ``PreferenceObjective``, ``ChoiceObjective`` or ``PolicyObjective`` of
         :mod:`packboost_b200.objectives`, on the rows of ``X``) takes the place of the squared loss; ``y``
         then only serves the correlations of ``round_metrics``, which have a ``train_loss`` beside them, and
-        may be ``None``.  A round whose gradient is not finite ends the fit with a ``RuntimeError``; the trees of
+        may be ``None``.  Hessians are 1, so with ``reduction="mean"`` the leaves are smaller by the number of
+        pairs or groups.  A round whose gradient is not finite ends the fit with a ``RuntimeError``; the trees of
         the rounds before it stay."""
         self._start(X, y, era, feature_names=feature_names, eval_sets=eval_sets, objective=objective)
         for round_idx in range(num_rounds):

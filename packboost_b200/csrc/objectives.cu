@@ -6,8 +6,8 @@
 // whether a policy's ratio is beyond its border must not hang on the rounding of a sum over a whole era, and
 // with a reference near the policy the difference of the two log-probabilities is all there is.
 //
-// Groups of rows in order are bound by the instructions that the SMs issue more than by memory: 32 rows of a policy are 640
-// bytes and some 180 instructions of a warp.
+// Groups of rows in order are bound neither by memory nor by the instructions that the SMs issue, but by waiting: 32 rows of a policy
+// are 640 bytes and some 180 instructions of a warp, half of the time at four a cycle; 2.2 to 2.5 are issued.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -389,7 +389,8 @@ __device__ __forceinline__ float sum_of(Pair32 x) { return x.hi + fminf(x.lo, 1.
 
 // exp(hi + lo): 2^y with y = hi log2 e rounded, by the unit that has 2^x to 2 ulp, times 1 + what y left out.  BEYOND: it may be
 // beyond 32 bits.  y is then held below 128, where 2^y is a number, and what that leaves out makes it infinite: infinity less a
-// part of itself would be no number.  (574 groups of a policy: 27.5 us so, 28.1 with a choice after the product, 26.7 without.)
+// part of itself would be no number.  (574 groups of a policy: 27.5 us so, 28.1 with a choice after the product, 26.7 without.)  The
+// correction is of first order: to float32 as long as |lo| is below 3e-4, that is for log-probabilities above -5 000.
 template <bool BEYOND>
 __device__ __forceinline__ float exp_of(Pair32 x) {
     constexpr float log2e = 1.44269502f, rest = 1.33498e-8f;  // log2 e as a float, and (log2 e - that) ln 2
@@ -962,7 +963,8 @@ int64_t n_parts_of(const pb_pairs* p) {
     const int64_t tasks = p->n_slices > p->n_chunks ? p->n_slices : p->n_chunks;
     return tasks < 148 * 2 * kPairWarps ? (tasks + kPairWarps - 1) / kPairWarps : 148 * 2;
 }
-// CTAs of the launch for longer groups: one each, up to so many that the totals are few against the rows.
+// CTAs of the launch for longer groups: one each, up to so many that the totals are few against the rows.  (8 000 groups of 300 rows, one
+// CTA each and so many: policy 78.5 and 75.4 us, choice 58.5 and 56.3; 2 400 groups: 27.7 and 30.4, 21.5 and 23.1.)
 int64_t block_grid(const pb_groups* g) { return g->n_blocks < 148 * 16 ? g->n_blocks : 148 * 16; }
 
 int64_t n_parts_of(const pb_groups* g, bool policy) { return team_grid(g, policy) + block_grid(g) + g->n_pieces; }
@@ -1051,8 +1053,10 @@ int launch_groups(const GroupArgs& a, const T* scores, T* out, const Totals& tot
     }
     if (g.n_blocks) {
         // Threads of a group: as few as keep an SM busy, since each warp costs its group as much as five rows: 8 warps where an SM has
-        // three groups (574 groups of 4 700 rows: 27 us, 38 with 16), else 16.  (`most`: the first place is rounded down; with a list
-        // of rows the last step's threads have places that are not used.)
+        // three groups, else 16.  Policies with 256 and 512 threads: 100 groups of 5 000 rows 13.5 and 12.0 us, 443 of them 20.4 and 24.2,
+        // 600 of them 28.3 and 34.4, 1 000 of 2 000 rows 21.9 and 28.4.  On the wrong side of the rule: 443 groups of 500 rows (9.7 and
+        // 14.9), 1 000 of 8 000 (73.6 and 66.4).  (`most`: the first place is rounded down; with a list of rows the last step's threads have
+        // places that are not used.)
         const int threads = g.n_blocks >= 148 * 3 ? 256 : 512;
         const int most = (int)(g.block_rows + 7) / 4 * 4 + (g.rows ? threads * kBlockRows : 0);
         const size_t smem = OP == kLogProbs ? 0 : (size_t)most * 8;
