@@ -374,7 +374,7 @@ struct Pair32 {  // hi + lo
 };
 
 // a - b without rounding, plus a small `lo`.  Where hi is infinite, lo comes out as NaN; fminf(lo, 1) is then 1, with which sums
-// and exp come out right, and changes nothing else: lo is above 1 only where hi is beyond 2^24.
+// and exp come out right, and changes nothing else: lo is above 1 only where hi is beyond 2^24 (see Normaliser).
 __device__ __forceinline__ Pair32 difference(float a, float b, float lo) {
     const float t = a - b, v = t - a;
     return Pair32{t, (a - (t - v)) - (b + v) + lo};
@@ -403,6 +403,18 @@ __device__ __forceinline__ float exp_of(Pair32 x) {
     const float e = exp2_of(y);
     return fmaf(e, more, e);
 }
+
+// The log of a group's sum, for differences from it.  Of a large log its float leaves out what is no longer small against the
+// difference: of three scores of 1e8 the probabilities were -0.1.  From 4 096 on scores and log are therefore both taken
+// relative to its float: the scores near it, which are all that have a probability, stay exact.  Below, what the float leaves out is at
+// most 1.3e-4, whose square is none of float32's.
+struct Normaliser {
+    float zero;
+    Pair32 log;  // from zero on
+    __device__ __forceinline__ explicit Normaliser(double lse64)
+        : zero(fabs(lse64) < 4096.0 ? 0.f : (float)lse64), log(split(lse64 - (double)zero)) {}
+    __device__ __forceinline__ Pair32 log_prob(float s) const { return difference(s - zero, log.hi, -log.lo); }
+};
 
 // exp(x) for x <= 0, exactly 1 at 0: with n = rint(x / ln 2), 2^n times the Taylor polynomial of degree 11 at
 // |f| <= ln 2 / 2.  Off by up to 1.1e-14 of the value from -60 on (7e-15 the rest of the polynomial, and 2.3e-17 a unit of n the one
@@ -540,7 +552,7 @@ struct Rows {
     // inputs, and the old log-probability of a row that was not taken, may be anything.
     template <bool FULL>
     __device__ __forceinline__ void terms(double lse64) {
-        const Pair32 lse = split(lse64);
+        const Normaliser lse(lse64);
         float part = 0.f, part_loss = 0.f, part_kl = 0.f;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
@@ -551,7 +563,7 @@ struct Rows {
             }
             if (on<FULL>(u)) {
                 const bool live = s[u] != -INFINITY;
-                const Pair32 l = difference(s[u], lse.hi, -lse.lo);
+                const Pair32 l = lse.log_prob(s[u]);
                 const float p = live ? exp_of<false>(l) : 0.f;
                 float fixed, own;
                 if (OP == kChoice) {
@@ -626,10 +638,10 @@ struct Rows {
 
     template <bool FULL>
     __device__ __forceinline__ void log_probs(double lse64, T* out) const {
-        const Pair32 lse = split(lse64);
+        const Normaliser lse(lse64);
         float l[N];
 #pragma unroll
-        for (int u = 0; u < N; ++u) l[u] = sum_of(difference(s[u], lse.hi, -lse.lo));
+        for (int u = 0; u < N; ++u) l[u] = sum_of(lse.log_prob(s[u]));
         put<FULL>(l, out);
     }
 };

@@ -21,7 +21,9 @@ and as what a fit learns from::
     booster.fit(X, None, era, num_rounds=100, objective=PreferenceObjective(chosen, rejected, beta=1.0))
 
 Scores are float32, float16 or bfloat16 and gradients have their type; sums are held in 64 bits, of up to eight terms
-each in 32, in an order that does not change from run to run.  The results are not attached to an
+each in 32, in an order that does not change from run to run.  The log of a group's sum of exponentials is one
+64-bit number: scores of a group beyond some 1e9 lose digits of their probabilities, and a group whose rows all
+have the type's lowest number has none; what masks a row is -inf.  The results are not attached to an
 autograd graph: the gradient is there already.  Calls only enqueue work on the current stream of the scores'
 device and may be captured into a CUDA graph; ``RowPairs`` and ``RowGroups`` wait for their own layout, may be
 used from any stream, and have to outlive the graphs that use them.  A layout takes 0.4 to 2 ms (millions of

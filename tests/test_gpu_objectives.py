@@ -886,3 +886,46 @@ def test_log_probs_of_whatever_predict_takes():
         np.testing.assert_array_equal(b.predict_log_probs(other, group.tolist()), want)
         with pytest.raises(ValueError, match="align"):
             b.predict_log_probs(other, group[1:])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+@pytest.mark.parametrize("offset,step,dtype", [(1e5, 2.0 ** -7, torch.float32), (-3e6, 0.25, torch.float32), (1e8, 8.0, torch.float32),
+                                               (-1e9, 64.0, torch.float32), (5e4, 32.0, torch.float16), (-1e9, 2.0 ** 23, torch.bfloat16)])
+def test_groups_far_from_zero(kind, mixed, offset, step, dtype):
+    """Only differences within a group count: scores at the 1e9 below zero of a mask that is a number, or with a large offset.
+    Every other group lies there, the others do not."""
+    lengths = KINDS[kind]
+    n, n_groups = sum(lengths), len(lengths)
+    rng = np.random.default_rng(n + 2)
+    group = _groups(rng, lengths, mixed)
+    far = group % 2 == 0
+    # near its offset a score is a whole number of steps of the type, of which half of the rows take none
+    base = float(torch.tensor(offset).to(dtype))
+    more = np.where(rng.random(n) < 0.5, 0, rng.integers(0, max(2, int(4 / step)), n)) * step
+    x = torch.from_numpy(np.where(far, base + more, rng.normal(size=n)).astype(np.float32)).to(dtype)
+    s = x.double().numpy() - np.where(far, base, 0.0)          # (exact: what the formulas see)
+    if dtype is torch.float32:
+        np.testing.assert_array_equal(s[far], more[far])
+    x = x.cuda()
+    # The log of the sum is a 64-bit number near the offset: off by half a step of those, twice with the sum's own, relative to
+    # each p and ratio; the bounds have at least two roundings (2 U) for each of them
+    grow = 1 + 2 * abs(base) * 2.0 ** -53 / (2 * ref.U)
+    l = ref.log_probs(s, group, n_groups)
+    plan = O.RowGroups(group, n_groups)
+    assert_close(O.group_log_probs(x, plan), l, ref.U * np.abs(l) + 2 * abs(base) * 2.0 ** -53)
+    t = np.where(rng.random(n) < 0.5, 0.0, rng.random(n)).astype(np.float32)
+    got = O.choice_loss(x, plan, _cuda(t))
+    loss, grad, err_l, err_g = ref.choice(s, group, n_groups, t)
+    assert_close(got.loss, loss, err_l + 2 * abs(base) * 2.0 ** -53 * t.sum())
+    assert_close(got.grad, grad, err_g * grow)
+    # (rows far behind in their group are not taken: their ratio is one of two float32 numbers that are not exact)
+    a = np.where((rng.random(n) < 0.4) | (l < -50), 0.0, rng.normal(size=n)).astype(np.float32)
+    old, prior = ((l + k * rng.normal(size=n)).astype(np.float32) for k in (0.3, 0.5))
+    got = O.policy_loss(x, plan, _cuda(a), _cuda(old), reference_log_probs=_cuda(prior), kl_coef=0.1)
+    loss, grad, kl, clipped, err_l, err_g, err_k = ref.policy(s, group, n_groups, a, old, prior, kl_coef=0.1)
+    off = 2 * abs(base) * 2.0 ** -53 * n          # (of a group's divergence: sum p is 1)
+    assert int(got.clipped) == clipped
+    assert_close(got.loss, loss, err_l * grow + 0.1 * off)
+    assert_close(got.kl, kl, err_k * grow + off)
+    assert_close(got.grad, grad, err_g * grow + 0.1 * 2 * abs(base) * 2.0 ** -53 * 2)
