@@ -929,3 +929,44 @@ def test_groups_far_from_zero(kind, mixed, offset, step, dtype):
     assert_close(got.loss, loss, err_l * grow + 0.1 * off)
     assert_close(got.kl, kl, err_k * grow + off)
     assert_close(got.grad, grad, err_g * grow + 0.1 * 2 * abs(base) * 2.0 ** -53 * 2)
+
+
+def test_pairs_behind_whatever_is_in_front():
+    """The launch of the pairs may begin before the kernel in front has ended, not before anything else: a wait for another stream,
+    a copy from the host, a graph."""
+    rng = np.random.default_rng(51)
+    n = 50_000
+    c, j = _pairs(rng, n, 200_000, 2, n)
+    pairs = O.RowPairs(c, j, n)
+    x, y = (_scores(rng, n, torch.float32)[0] for _ in range(2))
+    want_x, want_y = O.preference_loss(x, pairs), O.preference_loss(y, pairs)
+    host = y.cpu().pin_memory()
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    buffer, source = x.clone(), y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.cuda._sleep(300_000)
+        buffer.copy_(source * 1.0)
+    torch.cuda.synchronize()
+
+    def from_another_stream():
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(3_000_000)
+            buffer.copy_(y * 1.0)
+        main.wait_stream(side)
+
+    def from_the_host():
+        torch.cuda._sleep(300_000)
+        buffer.copy_(host, non_blocking=True)
+
+    for fill in (from_another_stream, from_the_host, graph.replay):
+        for _ in range(3):
+            buffer.copy_(x)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(main):
+                first = O.preference_loss(buffer, pairs)      # (a kernel that lets the next one begin)
+                fill()
+                got = O.preference_loss(buffer, pairs)
+            torch.cuda.synchronize()
+            for g, w in ((first, want_x), (got, want_y)):
+                assert torch.equal(g.loss, w.loss) and torch.equal(g.grad, w.grad)
