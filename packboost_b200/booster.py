@@ -1030,8 +1030,9 @@ class PackBoost:
         head, winners = self._trainer.read_log(ticket)
         if self._trainer.objective is not None and not np.isfinite(head["max_abs_grad"]):
             self._inflight = self._predrawn = None     # (a round that follows stands on this one)
-            self._trainer.release_graph()
-            self._trainer.close_comm()
+            trainer, self._trainer = self._trainer, None   # (with predictions that hold this round's step)
+            trainer.release_graph()
+            trainer.close_comm()
             raise RuntimeError(f"round {len(self._round_depths) + 1}: the objective's gradient is not finite")
         n_ctx = head["n_ctx"][: D + 1].tolist()
         self._last_n_ctx = n_ctx

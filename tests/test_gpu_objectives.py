@@ -970,3 +970,25 @@ def test_pairs_behind_whatever_is_in_front():
             torch.cuda.synchronize()
             for g, w in ((first, want_x), (got, want_y)):
                 assert torch.equal(g.loss, w.loss) and torch.equal(g.grad, w.grad)
+
+
+@pytest.mark.parametrize("ahead", ["0", "1"])
+def test_a_fit_that_ended_answers_with_the_trees_it_has(ahead, monkeypatch):
+    """The predictions of the training rows hold a step of the round that is not there; they are gone with it."""
+    monkeypatch.setenv("PACKBOOST_RUN_AHEAD", ahead)
+    n = 1200
+    group, chosen = np.arange(n) // 12, np.arange(n) % 12 == 0
+    X = np.random.default_rng(10).normal(size=(n, 4)).astype(np.float32)
+    X[:, 0] = chosen
+    args = dict(group=group, clip=(0.2, np.inf))
+    a, old = np.where(chosen, 1e-37, 0.0), np.full(n, -np.log(12.0) - 87.5)
+    cfg, era = PackBoostConfig(**dict(CFG, layer_feature_fraction=1.0)), np.zeros(n, np.int16)
+    b = PackBoost(cfg)
+    with pytest.raises(RuntimeError, match="not finite") as e:
+        b.fit(X, None, era, num_rounds=50, objective=O.PolicyObjective(a, old, **args))
+    done = int(str(e.value).split(":")[0].split()[1]) - 1
+    want = PackBoost(cfg).fit(X, None, era, num_rounds=done, objective=O.PolicyObjective(a, old, **args))
+    _same_trees(b, want)
+    np.testing.assert_array_equal(b.predict(X), want.predict(X))
+    with pytest.raises(RuntimeError):
+        b.train_predictions()
