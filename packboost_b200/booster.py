@@ -1028,7 +1028,7 @@ class PackBoost:
         ticket, state0 = inflight
         D = int(self.config.max_depth)
         head, winners = self._trainer.read_log(ticket)
-        if self._trainer.objective is not None and not np.isfinite(head["max_abs_grad"]):
+        if getattr(self._trainer, "objective", None) is not None and not np.isfinite(head["max_abs_grad"]):
             self._inflight = self._predrawn = None     # (a round that follows stands on this one)
             trainer, self._trainer = self._trainer, None   # (with predictions that hold this round's step)
             trainer.release_graph()
