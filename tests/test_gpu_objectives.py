@@ -992,3 +992,33 @@ def test_a_fit_that_ended_answers_with_the_trees_it_has(ahead, monkeypatch):
     np.testing.assert_array_equal(b.predict(X), want.predict(X))
     with pytest.raises(RuntimeError):
         b.train_predictions()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("mixed", [False, True], ids=["ordered", "mixed"])
+@pytest.mark.parametrize("low", [-5e3, -1e5, -1e7, -1e9])
+def test_taken_rows_far_behind_in_their_group(kind, mixed, low):
+    """Rows under a mask that is a number and that were taken all the same: their ratio is that of the two log-probabilities,
+    however little of their floats is left in the difference."""
+    lengths = [k + 1 for k in KINDS[kind]]
+    n, n_groups = sum(lengths), len(lengths)
+    rng = np.random.default_rng(n + 3)
+    group = _groups(rng, lengths, mixed)
+    x, s = _scores(rng, n, torch.float32)
+    behind = rng.random(n) < 0.3
+    first = np.array([np.flatnonzero(group == g)[0] for g in range(n_groups)])
+    behind[first] = False                       # (a group keeps a row)
+    x[_cuda(behind)] = low
+    s[behind] = float(np.float32(low))
+    l = ref.log_probs(s, group, n_groups)
+    a = np.where(rng.random(n) < 0.4, 0.0, rng.normal(size=n)).astype(np.float32)
+    near = np.where(behind, rng.choice([0.0, 1.0, -1.0, 3.0], n) * float(np.spacing(np.float32(abs(low)))), 0.3 * rng.normal(size=n))
+    old = (l + np.where(np.abs(near) > 60, 0, near)).astype(np.float32)
+    got = O.policy_loss(x, O.RowGroups(group, n_groups), _cuda(a), _cuda(old))
+    loss, grad, _, clipped, err_l, err_g, _ = ref.policy(s, group, n_groups, a, old)
+    # what the float of l leaves out is a float32 number of up to half a step of l's, 32 at 1e9: off by a rounding of it in each of four sums
+    lost = 4 * ref.U * np.where(behind, float(np.spacing(np.float32(abs(low)))), 0.0).max() + 2 * abs(low) * 2.0 ** -53
+    grow = 1 + lost / (2 * ref.U)
+    assert int(got.clipped) == clipped and 0 < clipped
+    assert_close(got.loss, loss, err_l * grow)
+    assert_close(got.grad, grad, err_g * grow)
