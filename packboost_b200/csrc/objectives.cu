@@ -7,7 +7,7 @@
 // with a reference near the policy the difference of the two log-probabilities is all there is.
 //
 // Groups of rows in order are bound neither by memory nor by the instructions that the SMs issue, but by waiting: 32 rows of a policy
-// are 640 bytes and some 180 instructions of a warp, half of the time at four a cycle; 2.2 to 2.5 are issued.
+// are 640 bytes and some 190 instructions of a warp, half of the time at four a cycle; 2.2 to 2.5 are issued.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
