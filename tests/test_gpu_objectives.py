@@ -950,6 +950,7 @@ def test_pairs_behind_whatever_is_in_front():
     torch.cuda.synchronize()
 
     def from_another_stream():
+        side.wait_stream(main)          # (the first call reads what is overwritten)
         with torch.cuda.stream(side):
             torch.cuda._sleep(3_000_000)
             buffer.copy_(y * 1.0)
