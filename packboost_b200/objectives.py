@@ -357,9 +357,10 @@ class RowPairs(_Layout):
     """Pairs of rows, the first preferred to the second, laid out for :func:`preference_loss`.
 
     ``weight`` counts a pair so many times (its product with the pair's loss or slope is a float32);
-    ``reference`` holds the scores of a reference model for all rows (those of compared rows finite; what two rows
-    differ by is kept as a float32, as the difference of their scores is), so that differences of scores become differences of log ratios: where the
-    scores are log-probabilities, or differ from them by something the two rows share, that is the paired log
+    ``reference`` holds the scores of a reference model for all rows (those of compared rows finite; what two
+    rows differ by is kept as a float32, as the difference of their scores is), so that differences of scores
+    become differences of log ratios: where the scores are log-probabilities, or differ from them by something
+    the two rows share, that is the paired log
     ratio of the model to the reference.  A pair may occur more than once; a row is not compared with itself."""
 
     def __init__(self, chosen, rejected, n_rows: int, *, weight=None, reference=None, device=None) -> None:
